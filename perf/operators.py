@@ -327,7 +327,7 @@ def prepare(case, seed):
         else:
             pool.store_dev(case["dtype"], x["k"].data_ptr(), x["v"].data_ptr(), x["slots"].data_ptr(), n)
             state["out"] = torch.empty_like(x["q"])
-            size = pool.workspace_bytes(case["heads"], x["q"].shape[0], x["table"].shape[1], case.get("prefix", 0))
+            size = pool.workspace_bytes(case["heads"], x["q"].shape[0], case.get("prefix", 0))
             state["work"] = torch.empty(size, dtype=torch.uint8, device="cuda")
             if case["kind"] == "sparse":
                 state["chosen"] = torch.empty(x["q"].shape[0], case["kv_heads"], case["top"], dtype=torch.int32, device="cuda")
