@@ -460,6 +460,97 @@ int32_t kronos_cuda_k2tb_save(const char *path, const uint64_t mode_words[6], co
                               const KronosCudaMatrixDesc *lm_head, const uint16_t *embed_bf16, size_t embed_bf16_len,
                               const KronosCudaMatrixDesc *embed_nf4);
 
+/* ---- a pool of cached keys and values for many sequences ----------------------------------------- */
+
+/* The engines keep the cache of one sequence.  A pool keeps rows of ANY number of sequences in pages of page_tokens positions, in the
+ * row formats of the engines' caches (store_hadamard_q8_head*_raw and store_hadamard_q4_head_raw, real_llm.rs:8303-8365, 8646-8701: signed
+ * FWHT-64, then int8 with one fp32 scale per row, or NF4 with one bf16 scale per 64 values; the same codes and scales bit for bit), and
+ * attends over them: sequences name their pages in a table, may share the pages of a common prefix, and may attend to chosen pages only.
+ * One pool holds one layer; which page belongs to whom is the host's to say.
+ *
+ * All buffers named d_* and all pointers inside the argument structs are DEVICE addresses.  Calls are queued on the context's stream and
+ * return without synchronizing; they allocate nothing and may be captured into graphs.  A page or slot outside the pool is skipped (its
+ * positions count as out of sight) and reported by the next synchronizing call.  Results do not depend on timing: the same call gives
+ * the same bits. */
+typedef struct KronosCudaKvPool KronosCudaKvPool;
+
+#define KRONOS_CUDA_TYPE_F32  0u
+#define KRONOS_CUDA_TYPE_BF16 1u
+#define KRONOS_CUDA_TYPE_F16  2u
+
+#define KRONOS_CUDA_POOL_BLOCK_KEYS 1u      /* flag: keep block keys, which kronos_cuda_kv_pool_select_dev reads */
+#define KRONOS_CUDA_POOL_MAX_CHOSEN 32768u
+
+typedef struct KronosCudaKvPoolConfig {
+    uint32_t struct_size;       /* sizeof(KronosCudaKvPoolConfig) */
+    uint32_t kv_heads;          /* 1..256 */
+    uint32_t head_dim;          /* 64 or 128 */
+    uint32_t kv_bits;           /* 8 or 4 */
+    uint32_t page_tokens;       /* 16, 32, 64 or 128 */
+    uint32_t num_pages;
+    uint32_t flags;
+} KronosCudaKvPoolConfig;
+
+/* Rows [token][head][head_dim]: element e of (t, h) lies at data + t * token_stride + h * head_stride + e.  Strides in elements, 0 =
+ * dense; rows on 16-byte boundaries are moved fastest, any element-aligned address is taken. */
+typedef struct KronosCudaRows {
+    void *data;
+    uint64_t token_stride;
+    uint64_t head_stride;
+} KronosCudaRows;
+
+KronosCudaKvPool *kronos_cuda_kv_pool_create(KronosCudaContext *ctx, const KronosCudaKvPoolConfig *config);
+/* Waits for the context's stream.  Graphs and other streams that use the pool must have finished. */
+void kronos_cuda_kv_pool_free(KronosCudaContext *ctx, KronosCudaKvPool *pool);
+size_t kronos_cuda_kv_pool_bytes(const KronosCudaKvPool *pool);
+
+/* Writes the keys and values of n_tok tokens (kv_heads rows each, of `type`) into slots d_slots[t] = page * page_tokens + row; a token with
+ * a slot below 0 is left out.  Slots of one call must differ.  A row that holds a value that is not finite reads back as NaN.
+ * With block keys: writing the LAST row of a page makes the page's block key from the rows the page then holds (rows of a page are
+ * written in order, so that these are the page's own): the mean of its keys as stored, fp32 in row order, quantized as an int8 row.
+ * load reads rows back (code times scale, inverse transform, rounded once to `type`); left-out tokens' rows stay as they are. */
+int32_t kronos_cuda_kv_pool_store_dev(KronosCudaContext *ctx, KronosCudaKvPool *pool, uint32_t type, const KronosCudaRows *d_k,
+                                      const KronosCudaRows *d_v, const int64_t *d_slots, size_t n_tok);
+int32_t kronos_cuda_kv_pool_load_dev(KronosCudaContext *ctx, KronosCudaKvPool *pool, uint32_t type, const KronosCudaRows *d_k,
+                                     const KronosCudaRows *d_v, const int64_t *d_slots, size_t n_tok);
+
+typedef struct KronosCudaPoolAttention {
+    uint32_t struct_size;       /* sizeof(KronosCudaPoolAttention) */
+    uint32_t row_type;          /* of q and out: KRONOS_CUDA_TYPE_* */
+    uint32_t heads;             /* query heads, a multiple of kv_heads; head h reads kv head h / (heads / kv_heads) */
+    uint32_t n_tok;             /* query tokens of all sequences together */
+    uint32_t pages_stride;      /* pages a row of the table has room for */
+    uint32_t prefix_len;        /* positions of the shared prefix, which every token sees; 0 = none */
+    uint32_t top, sinks, local; /* chosen pages per token and kv head; of select: first / last pages always among them */
+    float scale;                /* of the scores; 0 = 1 / sqrt(head_dim) */
+    KronosCudaRows q, out;      /* [n_tok][heads][head_dim]; select writes no out */
+    const int32_t *lens;        /* [n_tok]: positions of its own sequence that a token sees (0: none) */
+    const int32_t *seq;         /* [n_tok]: the token's row of the table; below 0: a padding token, sees nothing of its own.  NULL: row t */
+    const int32_t *pages;       /* [rows][pages_stride]: page of positions [i * page_tokens, ...) of a sequence; entries behind its last are not read */
+    const int32_t *prefix_pages;/* [ceil(prefix_len / page_tokens)] */
+    int32_t *chosen;            /* [n_tok][kv_heads][top]: indices into the token's row of the table */
+    void *workspace;            /* 16-byte aligned, kronos_cuda_kv_pool_workspace bytes; calls that overlap need one each */
+    size_t workspace_bytes;
+} KronosCudaPoolAttention;
+
+/* Bytes of workspace of an attention call of these sizes (select needs none); 0 for sizes that are refused.  Nothing in it has to be
+ * cleared, and nothing is kept there from call to call. */
+size_t kronos_cuda_kv_pool_workspace(const KronosCudaKvPool *pool, uint32_t heads, uint32_t n_tok, uint32_t prefix_len);
+
+/* out = softmax(scale q k^T) v over the prefix and the first lens[t] positions of the token's sequence.  A token that sees nothing gets
+ * zeros.  Queries, weights and sums are fp32; fp32 operands of the products are split in two halves, bf16 / fp16 ones rounded to one. */
+int32_t kronos_cuda_kv_pool_attend_dev(KronosCudaContext *ctx, KronosCudaKvPool *pool, const KronosCudaPoolAttention *args);
+
+/* For every token and kv head the `top` pages of its sequence to attend to, ascending, -1 behind them where the sequence has fewer: the
+ * first `sinks` and the last `local` (>= 1, a last page may be partly filled), and of the others those of the highest score, the lower
+ * index first among equals.  Score = (integer product of the block key and the query) * the key's scale; the query is the sum of the kv
+ * head's queries, quantized as an int8 row.  A page with a key that is not finite comes behind all others. */
+int32_t kronos_cuda_kv_pool_select_dev(KronosCudaContext *ctx, KronosCudaKvPool *pool, const KronosCudaPoolAttention *args);
+
+/* attend over the positions below lens[t] of the chosen pages alone (any order; entries below 0 or behind the sequence's last page are
+ * skipped; a page named twice counts twice). */
+int32_t kronos_cuda_kv_pool_attend_chosen_dev(KronosCudaContext *ctx, KronosCudaKvPool *pool, const KronosCudaPoolAttention *args);
+
 /* ---- no-allocation variant ------------------------------------------------------------------- */
 
 /* Widest matrix (columns) kronos_cuda_linear_noalloc accepts, and the bytes of device memory its

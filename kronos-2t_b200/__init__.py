@@ -7,6 +7,7 @@ from .ffi import (  # noqa: F401
     Context,
     Engine,
     KronosCudaError,
+    KvPool,
     Matrix,
     MatrixDesc,
     bipolar_desc,

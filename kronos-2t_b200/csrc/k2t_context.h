@@ -71,6 +71,7 @@ inline bool sync_and_check(KronosCudaContext *ctx, const char *what) {
                         : flag == 3 ? "a tensor- / expert-parallel exchange gave up waiting for a peer rank (the peer has left or never attached; recreate the engines)"
                         : flag == 4 ? "an expert kernel was handed a route id outside the layer's experts"
                         : flag == 5 ? "the attention kernel was launched for a context longer than it was sized for"
+                        : flag == 6 ? "a page or slot is outside the pool, or a sequence is longer than its row of the table"
                         : "a kernel gave up waiting for its weight pipeline";
         return fail(ctx, std::string(what) + ": " + why + " (results invalid)");
     }

@@ -1,0 +1,123 @@
+// Device side of the pool's storage: where a row lies in its block of 16 positions, types of rows, and the signed transform of a row
+// that is spread over lanes.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "k2t_device.cuh"
+#include "k2t_kv_pool.h"
+
+namespace k2t {
+
+// A block holds 16 rows of keys, 16 rows of values, then their scales ([row] fp32, or [row][group of 64] bf16).  8-bit codes are stored
+// with their sign bit flipped, 4-bit ones as centroid indices, element 2 i in the low half of byte i.
+template <int HD, int BITS> struct PoolBlock {
+    static constexpr uint32_t RB = BITS == 8 ? HD : HD / 2, G = BITS == 8 ? 1 : HD / 64, SC = BITS == 8 ? 64 : HD / 2;
+    static constexpr uint32_t V_AT = POOL_ROWS * RB, KS_AT = 2 * POOL_ROWS * RB, VS_AT = KS_AT + SC, BYTES = KS_AT + 2 * SC;
+};
+
+// Byte `at` of row p (0 .. 15) within 16 rows of RB bytes.  The attention kernel's lanes (n, t) = (lane / 4, lane % 4) read rows 4 (n / 2)
+// + n % 2 (and two further) at pieces t of keys, and rows 4 t + i at piece n of values; the order of rows and the exclusive-or of the
+// 16-byte pieces put the lanes of one shared-memory phase on different banks in both patterns, for each length of a row.
+template <uint32_t RB> __host__ __device__ __forceinline__ constexpr uint32_t row_place(uint32_t p, uint32_t at) {
+    static_assert(RB == 128 || RB == 64 || RB == 32, "row of 32, 64 or 128 bytes");
+    const uint32_t quad = (p >> 2) & 3u;
+    if (RB == 128) return p * 128 + (at ^ (((quad << 1) ^ ((p & 1u) << 2)) << 4));
+    if (RB == 64) return (p ^ (quad & 1u)) * 64 + (at ^ ((2u * ((quad ^ (quad >> 1)) & 1u)) << 4));
+    return (p ^ ((quad >> 1) | ((quad & 1u) << 1))) * 32 + at;
+}
+
+constexpr uint32_t TYPE_F32 = KRONOS_CUDA_TYPE_F32, TYPE_BF16 = KRONOS_CUDA_TYPE_BF16, TYPE_F16 = KRONOS_CUDA_TYPE_F16;
+
+__device__ __forceinline__ float2 unpack2(uint32_t type, uint32_t w) {
+    return type == TYPE_BF16 ? make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)) : __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ uint32_t pack2(uint32_t type, float x, float y) {
+    if (type == TYPE_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// Eight consecutive elements from / to element `at` of rows.
+__device__ __forceinline__ void rows_get8(const RowsArg &a, size_t at, float (&v)[8]) {
+    if (a.type == TYPE_F32) {
+        const float *p = static_cast<const float *>(a.p) + at;
+        if (a.wide) {
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p)), y = __ldcg(reinterpret_cast<const float4 *>(p) + 1);
+            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __ldcg(p + i);
+        }
+        return;
+    }
+    const uint16_t *p = static_cast<const uint16_t *>(a.p) + at;
+    uint32_t w[4];
+    if (a.wide) {
+        const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(p));
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldcg(p + 2 * i) | ((uint32_t)__ldcg(p + 2 * i + 1) << 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2(a.type, w[i]);
+        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void rows_put8(const RowsArg &a, size_t at, const float (&v)[8]) {
+    if (a.type == TYPE_F32) {
+        float *p = static_cast<float *>(a.p) + at;
+        if (a.wide) {
+            reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = v[i];
+        }
+        return;
+    }
+    uint16_t *p = static_cast<uint16_t *>(a.p) + at;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack2(a.type, v[2 * i], v[2 * i + 1]);
+    if (a.wide) {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { p[2 * i] = (uint16_t)w[i]; p[2 * i + 1] = (uint16_t)(w[i] >> 16); }
+    }
+}
+
+// Butterflies over the N elements that a thread holds (distances h0, 2 h0, ..), the lower element a + b, the upper a - b.
+template <int N> __device__ __forceinline__ void butterflies_in(float (&v)[N]) {
+#pragma unroll
+    for (int h = 1; h < N; h *= 2)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if ((i & h) == 0) {
+                const float a = v[i], b = v[i + h];
+                v[i] = __fadd_rn(a, b);
+                v[i + h] = __fsub_rn(a, b);
+            }
+}
+// The same between lanes l and l ^ m, all N elements.
+template <int N> __device__ __forceinline__ void butterflies_across(float (&v)[N], uint32_t m, uint32_t lane) {
+    const bool upper = (lane & m) != 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float o = __shfl_xor_sync(0xffffffffu, v[i], m);
+        v[i] = upper ? __fsub_rn(o, v[i]) : __fadd_rn(v[i], o);
+    }
+}
+__device__ __forceinline__ float flip(float x, uint32_t bit) { return __uint_as_float(__float_as_uint(x) ^ (bit << 31)); }
+
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
+
+constexpr uint32_t POOL_ERR_PAGE = 6;        // a page or slot outside the pool
+__device__ __forceinline__ void pool_bad_page(const PoolView &v) { atomicExch(v.err, POOL_ERR_PAGE); }
+
+}  // namespace k2t

@@ -1,0 +1,28 @@
+// Shared by the kernels of the pool's attention: how the work of a call is laid out in a line, and where partial results lie.
+#pragma once
+#include "k2t_kv_pool.h"
+
+namespace k2t {
+
+// A partial result: rows x head_dim numerators, then (maximum, denominator) of each row.
+struct SplitArgs {
+    PoolAttnArgs a;
+    uint32_t rbo, rbp;           // tiles of 16 rows of a token's item; of a prefix item (0: the line holds no prefix)
+    uint32_t units;              // warps
+    bool direct;                 // every warp has one item
+    float *own, *near;           // partial results of own rows; of the prefix
+
+    __host__ __device__ uint32_t slot_rows(bool prefix) const { const uint32_t g = a.heads / a.pool.d.kv_heads; return prefix || g > 16 ? 16 : g; }
+    __host__ __device__ uint32_t slot_floats(bool prefix) const { return (slot_rows(prefix) * (a.pool.d.head_dim + 2) + 3u) & ~3u; }       // 16-byte boundaries
+    // warps and items both ascend along the line, so their sum numbers the pieces
+    __host__ __device__ float *slot(bool prefix, uint32_t unit, uint32_t item) const {
+        return (prefix ? near : own) + (size_t)((direct ? 0u : unit) + item) * slot_floats(prefix);
+    }
+};
+__host__ __device__ inline uint32_t prefix_blocks(const SplitArgs &p) { return (p.a.prefix_len + POOL_ROWS - 1) / POOL_ROWS; }
+__host__ __device__ inline uint64_t prefix_line(const SplitArgs &p) { return (uint64_t)p.a.pool.d.kv_heads * p.rbp * prefix_blocks(p); }
+// blocks of a warp's part: at least MIN_PART, since a part costs its queries and a partial result
+constexpr uint32_t MIN_PART = 4;
+__host__ __device__ inline uint64_t part_blocks(uint64_t all, uint32_t units) { const uint64_t n = (all + units - 1) / units; return n < MIN_PART ? MIN_PART : n; }
+
+}  // namespace k2t

@@ -71,6 +71,24 @@ class BlockDesc(C.Structure):
                [(n, MatrixDesc) for n in ("in_proj", "decay_proj", "o_proj", "up_proj", "down_proj", "side_gate", "side_proj", "q_up", "kv_up", "router", "shared_down")]
 
 
+TYPES = {"f32": 0, "bf16": 1, "f16": 2}
+POOL_BLOCK_KEYS = 1
+
+
+class KvPoolConfig(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("struct_size", "kv_heads", "head_dim", "kv_bits", "page_tokens", "num_pages", "flags")]
+
+
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_uint64), ("head_stride", C.c_uint64)]
+
+
+class PoolAttention(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("struct_size", "row_type", "heads", "n_tok", "pages_stride", "prefix_len", "top", "sinks", "local")] + \
+               [("scale", C.c_float), ("q", Rows), ("out", Rows)] + [(n, C.c_void_p) for n in ("lens", "seq", "pages", "prefix_pages", "chosen", "workspace")] + \
+               [("workspace_bytes", C.c_size_t)]
+
+
 def load_library():
     """Loads libkronos_cuda.so; raises if it has not been built (no fallback exists)."""
     global _LIB
@@ -147,6 +165,15 @@ def load_library():
     sig("kronos_cuda_engine_debug_words", sz, vp, vp, sz)
     sig("kronos_cuda_engine_read_kv_q4", i32, vp, u32, u32, sz, vp, vp, vp, vp)
     sig("kronos_cuda_engine_read_kv", i32, vp, u32, u32, sz, vp, vp, vp, vp)
+    sig("kronos_cuda_kv_pool_create", vp, vp, C.POINTER(KvPoolConfig))
+    sig("kronos_cuda_kv_pool_free", None, vp, vp)
+    sig("kronos_cuda_kv_pool_bytes", sz, vp)
+    sig("kronos_cuda_kv_pool_store_dev", i32, vp, vp, u32, C.POINTER(Rows), C.POINTER(Rows), vp, sz)
+    sig("kronos_cuda_kv_pool_load_dev", i32, vp, vp, u32, C.POINTER(Rows), C.POINTER(Rows), vp, sz)
+    sig("kronos_cuda_kv_pool_workspace", sz, vp, u32, u32, u32)
+    sig("kronos_cuda_kv_pool_attend_dev", i32, vp, vp, C.POINTER(PoolAttention))
+    sig("kronos_cuda_kv_pool_attend_chosen_dev", i32, vp, vp, C.POINTER(PoolAttention))
+    sig("kronos_cuda_kv_pool_select_dev", i32, vp, vp, C.POINTER(PoolAttention))
     _LIB = L
     return L
 
@@ -340,6 +367,67 @@ class Context:
     def gemv_dev(self, mat, d_xq, d_xs, d_xsum, n_tok, d_out, out_stride=None, d_dots=None):
         self._check(self.L.kronos_cuda_gemv_dev(self.handle, mat.handle, d_xq, d_xs, d_xsum, n_tok, d_out,
                                                 out_stride or mat.rows, d_dots))
+
+
+def _rows(r):
+    """Rows of (address, token stride, head stride in elements), or of an address alone (dense)."""
+    return Rows(*r) if isinstance(r, (tuple, list)) else Rows(r, 0, 0)
+
+
+class KvPool:
+    """Cached keys and values of many sequences in pages (KronosCudaKvPool).  All methods take device addresses and queue on the context's
+    stream; rows of queries, keys, values and outputs are an address (dense [token][head][head_dim]) or (address, token stride, head
+    stride) in elements, their type "f32", "bf16" or "f16"."""
+
+    def __init__(self, ctx, kv_heads, head_dim, kv_bits, page_tokens, num_pages, block_keys=False):
+        self.ctx, self.L, self.handle = ctx, ctx.L, None
+        self.kv_heads, self.head_dim, self.kv_bits, self.page_tokens, self.num_pages = kv_heads, head_dim, kv_bits, page_tokens, num_pages
+        cfg = KvPoolConfig(C.sizeof(KvPoolConfig), kv_heads, head_dim, kv_bits, page_tokens, num_pages, POOL_BLOCK_KEYS if block_keys else 0)
+        self.handle = self.L.kronos_cuda_kv_pool_create(ctx.handle, C.byref(cfg))
+        if not self.handle:
+            raise KronosCudaError(self.L.kronos_cuda_last_error(ctx.handle).decode())
+
+    def free(self):
+        if self.handle:
+            self.L.kronos_cuda_kv_pool_free(self.ctx.handle, self.handle)
+            self.handle = None
+
+    def __del__(self):
+        self.free()
+
+    @property
+    def device_bytes(self):
+        return self.L.kronos_cuda_kv_pool_bytes(self.handle)
+
+    def store_dev(self, dtype, d_k, d_v, d_slots, n_tok):
+        """Rows of n_tok tokens into slots (int64: page * page_tokens + row, below 0: left out)."""
+        self.ctx._check(self.L.kronos_cuda_kv_pool_store_dev(self.ctx.handle, self.handle, TYPES[dtype], C.byref(_rows(d_k)), C.byref(_rows(d_v)), d_slots, n_tok))
+
+    def load_dev(self, dtype, d_slots, n_tok, d_k, d_v):
+        self.ctx._check(self.L.kronos_cuda_kv_pool_load_dev(self.ctx.handle, self.handle, TYPES[dtype], C.byref(_rows(d_k)), C.byref(_rows(d_v)), d_slots, n_tok))
+
+    def workspace_bytes(self, heads, n_tok, prefix_len=0):
+        return self.L.kronos_cuda_kv_pool_workspace(self.handle, heads, n_tok, prefix_len)
+
+    def _tokens(self, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq=None, workspace=(None, 0), d_out=None, scale=0.0, **rest):
+        return PoolAttention(struct_size=C.sizeof(PoolAttention), row_type=TYPES[dtype], heads=heads, n_tok=n_tok, pages_stride=pages_stride, scale=scale, q=_rows(d_q),
+                             out=_rows(d_out), lens=d_lens, seq=d_seq, pages=d_pages, workspace=workspace[0], workspace_bytes=workspace[1], **rest)
+
+    def attend_dev(self, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_out, workspace, d_seq=None, d_prefix_pages=None, prefix_len=0, scale=0.0):
+        """Attention of n_tok query tokens over the shared prefix and the first lens[t] (int32) positions of their sequences; d_pages: int32
+        table [rows][pages_stride], d_seq: each token's row of it (None: row t), workspace: (address, workspace_bytes(..))."""
+        a = self._tokens(dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq, workspace, d_out, scale, prefix_pages=d_prefix_pages, prefix_len=prefix_len)
+        self.ctx._check(self.L.kronos_cuda_kv_pool_attend_dev(self.ctx.handle, self.handle, C.byref(a)))
+
+    def select_dev(self, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, top, d_chosen, sinks=1, local=1, d_seq=None, workspace=(None, 0)):
+        """The `top` pages of each token and kv head by block keys, int32 [n_tok][kv_heads][top]: indices into the token's row of the table."""
+        a = self._tokens(dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq, workspace, top=top, sinks=sinks, local=local, chosen=d_chosen)
+        self.ctx._check(self.L.kronos_cuda_kv_pool_select_dev(self.ctx.handle, self.handle, C.byref(a)))
+
+    def attend_chosen_dev(self, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, top, d_chosen, d_out, workspace, d_seq=None, scale=0.0):
+        """Attention over the chosen pages alone."""
+        a = self._tokens(dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq, workspace, d_out, scale, top=top, chosen=d_chosen)
+        self.ctx._check(self.L.kronos_cuda_kv_pool_attend_chosen_dev(self.ctx.handle, self.handle, C.byref(a)))
 
 
 def desc_of(m):

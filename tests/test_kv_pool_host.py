@@ -1,0 +1,101 @@
+"""The shared pool of cached keys and values without a device: struct layouts, refusals, and the restatement against the oracle."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import kv_pool_ref as ref
+from k2t_internal import internal
+from test_boundary_structs import ctypes_struct, header_struct, rust_struct, same
+
+
+@pytest.mark.parametrize("name,cls", [("KronosCudaKvPoolConfig", "KvPoolConfig"), ("KronosCudaRows", "Rows"), ("KronosCudaPoolAttention", "PoolAttention")])
+def test_struct_layouts_agree(name, cls):
+    from kronos_2t_b200 import ffi
+    h, r, c = header_struct(name), rust_struct(name), ctypes_struct(getattr(ffi, cls))
+    assert len(h) >= 3 and h == r and same(h, c)
+
+
+def config(**over):
+    from kronos_2t_b200 import ffi
+    c = dict(struct_size=C.sizeof(ffi.KvPoolConfig), kv_heads=4, head_dim=128, kv_bits=8, page_tokens=64, num_pages=10, flags=1)
+    c.update(over)
+    return ffi.KvPoolConfig(**c)
+
+
+def arguments(**over):
+    from kronos_2t_b200 import ffi
+    rows = ffi.Rows(1 << 20, 0, 0)
+    a = dict(struct_size=C.sizeof(ffi.PoolAttention), row_type=1, heads=28, n_tok=3, pages_stride=5, q=rows, out=rows, lens=4096, pages=4096, workspace=1 << 20, workspace_bytes=1 << 40)
+    a.update(over)
+    return ffi.PoolAttention(**a)
+
+
+def refusal(cfg, args=None, what=0):
+    f = internal("pool_refusal", C.c_char_p, C.c_void_p, C.c_void_p, C.c_int32)
+    got = f(C.byref(cfg), None if args is None else C.byref(args), what)
+    return None if got is None else got.decode()
+
+
+@pytest.mark.parametrize("over,message", [
+    (dict(struct_size=4), "struct_size"), (dict(kv_heads=0), "kv heads"), (dict(kv_heads=257), "kv heads"), (dict(head_dim=96), "head_dim"), (dict(head_dim=256), "head_dim"),
+    (dict(kv_bits=5), "kv_bits"), (dict(page_tokens=8), "page_tokens"), (dict(page_tokens=48), "page_tokens"), (dict(page_tokens=256), "page_tokens"),
+    (dict(num_pages=0), "pages"), (dict(num_pages=1 << 31), "pages"), (dict(flags=2), "flag")])
+def test_configurations_that_are_refused(over, message):
+    assert refusal(config()) is None
+    assert message in refusal(config(**over))
+
+
+def rows(data, token=0, head=0):
+    from kronos_2t_b200 import ffi
+    return ffi.Rows(data, token, head)
+
+
+@pytest.mark.parametrize("over,message", [
+    (dict(struct_size=4), "struct_size"), (dict(heads=30), "heads"), (dict(heads=0), "heads"), (dict(heads=4 * 257), "heads"), (dict(n_tok=(1 << 20) + 1), "tokens"),
+    (dict(lens=None), "NULL"), (dict(pages=None), "NULL"), (dict(pages_stride=0), "pages_stride"), (dict(prefix_len=5), "without its pages"), (dict(prefix_len=1 << 31, prefix_pages=4096), "prefix"),
+    (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(row_type=3), "type"), (dict(q=rows(None)), "q is NULL"), (dict(out=rows(None)), "out is NULL"),
+    (dict(q=rows((1 << 20) + 1)), "aligned"), (dict(out=rows(1 << 20, 128, 128)), "overlap"), (dict(out=rows(1 << 20, 28 * 128, 64)), "overlap"), (dict(q=rows(1 << 20, 1 << 40)), "stride"),
+    (dict(workspace=None), "workspace"), (dict(workspace=(1 << 20) + 8), "workspace"), (dict(workspace_bytes=64), "workspace"), (dict(top=4), "attend takes no chosen"), (dict(chosen=4096), "attend takes no chosen")])
+def test_attention_calls_that_are_refused(over, message):
+    assert refusal(config(), arguments()) is None
+    assert refusal(config(), arguments(out=rows(1 << 20, 128, 3 * 128))) is None          # heads outermost
+    assert message in refusal(config(), arguments(**over))
+
+
+@pytest.mark.parametrize("what,over,message", [
+    (1, dict(chosen=None), "chosen is NULL"), (1, dict(top=0), "top"), (1, dict(top=32769), "top"), (1, dict(prefix_len=3, prefix_pages=4096), "prefix"), (2, dict(local=0), "local"),
+    (2, dict(sinks=4), "sinks"), (2, dict(sinks=0xffffffff), "sinks"), (2, dict(local=0xffffffff), "local"), (2, dict(pages_stride=32769), "32768")])
+def test_choices_that_are_refused(what, over, message):
+    good = dict(chosen=4096, top=4, sinks=1, local=1)
+    assert refusal(config(), arguments(**good), what) is None
+    assert message in refusal(config(), arguments(**{**good, **over}), what)
+
+
+def test_choice_needs_block_keys():
+    assert "block keys" in refusal(config(flags=0), arguments(chosen=4096, top=4, sinks=1, local=1), 2)
+
+
+def test_null_handles_are_tolerated():
+    import kronos_2t_b200 as k2
+    L = k2.load_library()
+    assert L.kronos_cuda_kv_pool_create(None, None) is None
+    L.kronos_cuda_kv_pool_free(None, None)
+    assert L.kronos_cuda_kv_pool_bytes(None) == 0 and L.kronos_cuda_kv_pool_workspace(None, 4, 1, 0) == 0
+    assert L.kronos_cuda_kv_pool_store_dev(None, None, 0, None, None, None, 1) == -1
+    assert L.kronos_cuda_kv_pool_load_dev(None, None, 0, None, None, None, 1) == -1
+    for f in (L.kronos_cuda_kv_pool_attend_dev, L.kronos_cuda_kv_pool_attend_chosen_dev, L.kronos_cuda_kv_pool_select_dev):
+        assert f(None, None, None) == -1
+
+
+def test_restatement_against_the_oracle(oracle):
+    """Transform and 4-bit assignment are the oracle's; the inverse undoes the transform; quantised rows are near what they stand for."""
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((7, 128)).astype(np.float32)
+    want = np.stack([oracle.fwht64(row, 0) for row in x])
+    assert np.array_equal(ref.rotate(x), want)
+    assert np.abs(ref.rotate_back(ref.rotate(x.astype(np.float64))) - x).max() < 1e-12
+    # 8 bits: half a step of max / 127 per transformed value, so its 2-norm over 64 values at most 4 steps of the largest
+    assert np.abs(ref.stored(x, 8) - want).max() <= np.abs(want).max() / 127 * 0.5001
+    # 4 bits: centroids are at most 16 half steps of 1/127 apart from their borders, plus the fitted scale
+    assert np.abs(ref.stored(x, 4) - want).max() <= np.abs(want).max() * 0.25
