@@ -17,7 +17,10 @@
 namespace k2t {
 namespace {
 
-constexpr uint32_t SP_WARPS = 4, SP_STAGES = 4, WAIT_LIMIT = 1u << 22;
+constexpr uint32_t SP_WARPS = 4, SP_STAGES = 3, WAIT_LIMIT = 1u << 22;
+// CTAs on an SM: registers (two for rows of 128 with queries in two halves)
+template <int HD, int QT> struct SplitCtas { static constexpr uint32_t N = HD == 128 && QT == 2 ? 2 : 3; };
+template <int HD, int BITS, int QT> constexpr uint32_t split_smem() { return SP_WARPS * (SP_STAGES * PoolBlock<HD, BITS>::BYTES + QT * HD / 16 * 512); }
 constexpr float LOG2_E = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -152,12 +155,10 @@ __device__ __forceinline__ void get16(const RowsArg &a, size_t at, float (&v)[16
 }
 
 // Rows 'lane / 4' and that + 8: their elements [16 c, 16 c + 16) for c = t, and t + 4 where rows are 128 long; transformed, times a power
-// of two that brings the largest to 2^13 .. 2^14 (so that both terms of an fp32 row are ordinary halves), as operand fragments.
-template <int HD, int TERMS> struct Query {
-    uint32_t a[TERMS][HD / 16][4];
-    float c[2];                        // factor of the scores of the two rows, in powers of two
-};
-template <int HD, int TERMS> __device__ __forceinline__ void load_query(const SplitArgs &p, const Item &it, uint32_t lane, Query<HD, TERMS> &q) {
+// of two that brings the largest to 2^13 .. 2^14 (so that both terms of a row are ordinary halves), as operand fragments: word 2 k + r
+// of fragment i (and of its second term, HD / 16 further) for every lane, 16 bytes a lane.  They lie in shared memory: as 32 or 64
+// registers they left room for two CTAs on an SM where there are three now.  c: factor of the scores of the two rows, in powers of two.
+template <int HD, int QT> __device__ __forceinline__ void load_query(const SplitArgs &p, const Item &it, uint32_t lane, uint32_t *frags, float (&c)[2]) {
     const uint32_t n = lane >> 2, t4 = lane & 3u;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -183,7 +184,7 @@ template <int HD, int TERMS> __device__ __forceinline__ void load_query(const Sp
         // 2^(13 - exponent of top), within what a float holds; its inverse goes into the factor of the scores
         const int e = min(126, max(-126, 13 - (int)((__float_as_uint(top) >> 23) & 255u) + 127));
         const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
-        q.c[r] = p.a.scale * LOG2_E * down;
+        c[r] = p.a.scale * LOG2_E * down;
 #pragma unroll
         for (int g = 0; g < HD / 64; ++g)
 #pragma unroll
@@ -192,10 +193,10 @@ template <int HD, int TERMS> __device__ __forceinline__ void load_query(const Sp
                 for (int k = 0; k < 2; ++k) {
                     float x = v[g][4 * w + 2 * k] * up, y = v[g][4 * w + 2 * k + 1] * up;
                     const uint32_t hi = half2_bits(x, y);
-                    q.a[0][4 * g + w][r + 2 * k] = hi;
-                    if constexpr (TERMS == 2) {
+                    frags[((4 * g + w) * 32 + lane) * 4 + r + 2 * k] = hi;
+                    if constexpr (QT == 2) {
                         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-                        q.a[1][4 * g + w][r + 2 * k] = half2_bits(x - f.x, y - f.y);
+                        frags[((HD / 16 + 4 * g + w) * 32 + lane) * 4 + r + 2 * k] = half2_bits(x - f.x, y - f.y);
                     }
                 }
     }
@@ -211,13 +212,13 @@ __device__ __forceinline__ uint32_t centroids4(uint32_t w) {
 __device__ __forceinline__ uint32_t halves_lo(uint32_t x) { return hsub2(prmt(x, 0x64646464u, 0x4140u), 0x64806480u); }
 __device__ __forceinline__ uint32_t halves_hi(uint32_t x) { return hsub2(prmt(x, 0x64646464u, 0x4342u), 0x64806480u); }
 
-template <int HD, int BITS, int TERMS> struct State {
+template <int HD> struct State {
     float o[HD / 8][4], m[2], l[2];
 };
 
 // One block of 16 positions, `valid` of them in sight, at shared address `at`.
-template <int HD, int BITS, int TERMS>
-__device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t lane, const Query<HD, TERMS> &q, State<HD, BITS, TERMS> &st) {
+template <int HD, int BITS, int QT, int PT>
+__device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t lane, uint32_t frags, const float (&c)[2], State<HD> &st) {
     using B = PoolBlock<HD, BITS>;
     constexpr int G = B::G;
     const uint32_t n = lane >> 2, t = lane & 3u;
@@ -228,24 +229,30 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
 #pragma unroll
         for (int j = 0; j < 2; ++j) s[g][j][0] = s[g][j][1] = s[g][j][2] = s[g][j][3] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const uint32_t row = 4 * (n >> 1) + (n & 1u) + 2 * j;
+    for (int g = 0; g < HD / 64; ++g) {
+        uint32_t w[2][4];
 #pragma unroll
-        for (int g = 0; g < HD / 64; ++g) {
-            uint32_t w[4];
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t row = 4 * (n >> 1) + (n & 1u) + 2 * j;
             if (BITS == 8) {
-                lds_words<4>(at + row_place<B::RB>(row, g * 64 + t * 16), w);
+                lds_words<4>(at + row_place<B::RB>(row, g * 64 + t * 16), w[j]);
             } else {
                 uint32_t x[2];
                 lds_words<2>(at + row_place<B::RB>(row, g * 32 + t * 8), x);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) { w[2 * i] = centroids4(x[i]); w[2 * i + 1] = centroids4(x[i] >> 16); }
+                for (int i = 0; i < 2; ++i) { w[j][2 * i] = centroids4(x[i]); w[j][2 * i + 1] = centroids4(x[i] >> 16); }
             }
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t b0 = halves_lo(w[i]), b1 = halves_hi(w[i]);
+        for (int i = 0; i < 4; ++i) {
+            uint32_t a[QT][4];
 #pragma unroll
-                for (int k = 0; k < TERMS; ++k) mma_f16(s[G == 1 ? 0 : g][j], q.a[k][4 * g + i], b0, b1);
+            for (int k = 0; k < QT; ++k) lds_words<4>(frags + ((k * (HD / 16) + 4 * g + i) * 32 + lane) * 16, a[k]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t b0 = halves_lo(w[j][i]), b1 = halves_hi(w[j][i]);
+#pragma unroll
+                for (int k = 0; k < QT; ++k) mma_f16(s[G == 1 ? 0 : g][j], a[k], b0, b1);
             }
         }
     }
@@ -297,7 +304,7 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
         for (int i = 0; i < 4; ++i) {
             float d = s[0][i >> 1][2 * r + (i & 1)] * ks[0][i];
             if (G == 2) d = __fmaf_rn(s[G - 1][i >> 1][2 * r + (i & 1)], ks[G - 1][i], d);
-            x[r][i] = __fmaf_rn(d, q.c[r], lv[i]);
+            x[r][i] = __fmaf_rn(d, c[r], lv[i]);
         }
     const float top0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), top1 = fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3]));
     // the maximum follows only where it has grown by more than 2^8: weights stay within halves, sums are exact in either case
@@ -323,7 +330,7 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
             st.l[r] = __fmaf_rn(x[r][i], iv[i], st.l[r]);
         }
     }
-    uint32_t a[G][TERMS][4];
+    uint32_t a[G][PT][4];
 #pragma unroll
     for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -331,7 +338,7 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
             float u = x[k & 1][k & 2], v = x[k & 1][(k & 2) + 1];
             if (BITS == 4) { u *= part[g][k & 2]; v *= part[g][(k & 2) + 1]; }
             a[g][0][k] = half2_bits(u, v);
-            if constexpr (TERMS == 2) {
+            if constexpr (PT == 2) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&a[g][0][k]));
                 a[g][1][k] = half2_bits(u - f.x, v - f.y);
             }
@@ -364,13 +371,13 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
             for (int g = 0; g < G; ++g) {
                 const uint32_t x0 = G == 1 || (n >> 2) == (uint32_t)g ? b0[e] : 0u, x1 = G == 1 || (n >> 2) == (uint32_t)g ? b1[e] : 0u;
 #pragma unroll
-                for (int y = 0; y < TERMS; ++y) mma_f16(st.o[4 * k + e], a[g][y], x0, x1);
+                for (int y = 0; y < PT; ++y) mma_f16(st.o[4 * k + e], a[g][y], x0, x1);
             }
     }
 }
 
 // The rows of a finished item, normalised and transformed back: the lane holds, of rows n and n + 8, elements (2 t + b) HD / 8 + j.
-template <int HD, int BITS, int TERMS> __device__ __forceinline__ void write_rows(const SplitArgs &p, const Item &it, uint32_t lane, const State<HD, BITS, TERMS> &st) {
+template <int HD> __device__ __forceinline__ void write_rows(const SplitArgs &p, const Item &it, uint32_t lane, const State<HD> &st) {
     constexpr int E = HD / 8;                  // consecutive elements of a lane
     const uint32_t n = lane >> 2, t4 = lane & 3u;
 #pragma unroll
@@ -402,13 +409,14 @@ struct Requests {
     uint32_t asked;            // blocks asked for
 };
 
-template <int HD, int BITS, int TERMS>
-__global__ void __launch_bounds__(SP_WARPS * 32) pool_split_kernel(const __grid_constant__ SplitArgs p) {
+template <int HD, int BITS, int QT, int PT>
+__global__ void __launch_bounds__(SP_WARPS * 32, SplitCtas<HD, QT>::N) pool_split_kernel(const __grid_constant__ SplitArgs p) {
     using B = PoolBlock<HD, BITS>;
     extern __shared__ __align__(128) uint8_t smb[];
     __shared__ __align__(8) uint64_t bars[SP_WARPS][SP_STAGES];
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, unit = blockIdx.x * SP_WARPS + warp;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smb) + warp * SP_STAGES * B::BYTES, bar = (uint32_t)__cvta_generic_to_shared(bars[warp]);
+    uint32_t *frags = reinterpret_cast<uint32_t *>(smb + warp * (QT * HD / 16 * 512));
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smb) + SP_WARPS * (QT * HD / 16 * 512) + warp * SP_STAGES * B::BYTES, bar = (uint32_t)__cvta_generic_to_shared(bars[warp]);
     const PoolShape &d = p.a.pool.d;
     const uint32_t bs = d.page_shift - 4;
     if (lane == 0) {
@@ -476,10 +484,11 @@ __global__ void __launch_bounds__(SP_WARPS * 32) pool_split_kernel(const __grid_
         rq.asked += 1;
     };
     for (uint32_t i = 0; i < SP_STAGES; ++i) request();
-    Query<HD, TERMS> q;
-    State<HD, BITS, TERMS> st;
+    float c[2];
+    State<HD> st;
     auto begin = [&]() {
-        load_query(p, it, lane, q);
+        load_query<HD, QT>(p, it, lane, frags, c);
+        __syncwarp();
 #pragma unroll
         for (int j = 0; j < HD / 8; ++j) st.o[j][0] = st.o[j][1] = st.o[j][2] = st.o[j][3] = 0.0f;
         st.m[0] = st.m[1] = -INFINITY;
@@ -522,7 +531,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32) pool_split_kernel(const __grid_
             landed = __all_sync(0xffffffffu, landed);
             ok = ok && landed;
             phase ^= 1u << stage;
-            block_step<HD, BITS, TERMS>(ring + stage * B::BYTES, valid, lane, q, st);
+            block_step<HD, BITS, QT, PT>(ring + stage * B::BYTES, valid, lane, (uint32_t)__cvta_generic_to_shared(frags), c, st);
         }
         __syncwarp();                          // all lanes are done with the stage
         request();
@@ -646,13 +655,12 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
 // ------------------------------------------------------------------------------------------------ launches
 // One warp per item where there are several items for every warp that the SMs hold: their ends then overlap anyway, and nothing has to
 // be looked up or joined.
-constexpr uint32_t SP_CTAS = 3;
-SplitArgs split_plan(const PoolAttnArgs &a) {
+SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     SplitArgs p{};
     p.a = a;
     const PoolShape &d = a.pool.d;
     const uint32_t group = a.heads / d.kv_heads;
-    const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * ((group + 15) / 16), room = (uint64_t)a.sm_count * SP_CTAS * SP_WARPS;
+    const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * ((group + 15) / 16), room = (uint64_t)a.sm_count * (d.head_dim == 128 && type != TYPE_BF16 ? SplitCtas<128, 2>::N : SplitCtas<128, 1>::N) * SP_WARPS;
     p.rbo = (group + 15) / 16;
     p.rbp = a.prefix_len == 0 ? 0 : (a.n_tok * group + 15) / 16;
     p.direct = p.rbp == 0 && items >= 4 * room;
@@ -662,11 +670,17 @@ SplitArgs split_plan(const PoolAttnArgs &a) {
 size_t own_slots(const SplitArgs &p) { return p.direct ? p.units : p.units + (size_t)p.a.n_tok * p.a.pool.d.kv_heads * p.rbo; }
 size_t near_slots(const SplitArgs &p) { return p.rbp == 0 ? 0 : p.units + (size_t)p.a.pool.d.kv_heads * p.rbp; }
 
-template <int HD, int BITS, int TERMS> cudaError_t split_launch(cudaStream_t s, const SplitArgs &p) {
-    const size_t smem = (size_t)SP_WARPS * SP_STAGES * PoolBlock<HD, BITS>::BYTES;
-    const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(pool_split_kernel<HD, BITS, TERMS>), smem);
+// Halves of an operand: bf16 queries and weights are rounded to one each (11 bits where bf16 has 8); fp16 queries keep two, since a score is a
+// sum of head_dim roundings (one: an output of fp16 rows 2.3 times as far from 64 bits as its own rounding); fp32 keeps two of both.
+template <int HD, int BITS, int QT, int PT> cudaError_t split_go(cudaStream_t s, const SplitArgs &p) {
+    const size_t smem = split_smem<HD, BITS, QT>();
+    const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(pool_split_kernel<HD, BITS, QT, PT>), smem);
     if (e != cudaSuccess) return e;
-    return launch_kernel(pool_split_kernel<HD, BITS, TERMS>, dim3((p.units + SP_WARPS - 1) / SP_WARPS), dim3(SP_WARPS * 32), smem, s, true, p);
+    return launch_kernel(pool_split_kernel<HD, BITS, QT, PT>, dim3((p.units + SP_WARPS - 1) / SP_WARPS), dim3(SP_WARPS * 32), smem, s, true, p);
+}
+template <int HD, int BITS> cudaError_t split_launch(cudaStream_t s, const SplitArgs &p) {
+    const uint32_t type = p.a.q.type;
+    return type == TYPE_F32 ? split_go<HD, BITS, 2, 2>(s, p) : type == TYPE_F16 ? split_go<HD, BITS, 2, 1>(s, p) : split_go<HD, BITS, 1, 1>(s, p);
 }
 
 }  // namespace
@@ -678,19 +692,21 @@ size_t pool_work_bytes(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint3
     a.n_tok = n_tok;
     a.prefix_len = prefix_len;
     a.sm_count = sm_count;
-    const SplitArgs p = split_plan(a);
-    return (own_slots(p) * p.slot_floats(false) + near_slots(p) * p.slot_floats(true)) * 4;
+    size_t most = 0;
+    for (uint32_t type : {TYPE_F32, TYPE_BF16, TYPE_F16}) {
+        const SplitArgs p = split_plan(a, type);
+        most = std::max(most, (own_slots(p) * p.slot_floats(false) + near_slots(p) * p.slot_floats(true)) * 4);
+    }
+    return most;
 }
 
 cudaError_t launch_pool_attend(cudaStream_t s, const PoolAttnArgs &a, uint32_t *launched) {
-    SplitArgs p = split_plan(a);
+    SplitArgs p = split_plan(a, a.q.type);
     p.own = reinterpret_cast<float *>(a.work);
     p.near = p.own + own_slots(p) * p.slot_floats(false);
     const PoolShape &d = a.pool.d;
-    const bool two = a.q.type == TYPE_F32, b8 = d.bits == 8;
-    cudaError_t e;
-    if (d.head_dim == 128) e = b8 ? (two ? split_launch<128, 8, 2>(s, p) : split_launch<128, 8, 1>(s, p)) : two ? split_launch<128, 4, 2>(s, p) : split_launch<128, 4, 1>(s, p);
-    else e = b8 ? (two ? split_launch<64, 8, 2>(s, p) : split_launch<64, 8, 1>(s, p)) : two ? split_launch<64, 4, 2>(s, p) : split_launch<64, 4, 1>(s, p);
+    const bool b8 = d.bits == 8;
+    const cudaError_t e = d.head_dim == 128 ? (b8 ? split_launch<128, 8>(s, p) : split_launch<128, 4>(s, p)) : b8 ? split_launch<64, 8>(s, p) : split_launch<64, 4>(s, p);
     *launched += 1;
     if (e != cudaSuccess || (p.direct && a.prefix_len == 0)) return e;
     *launched += 1;
