@@ -117,6 +117,25 @@ __device__ __forceinline__ float flip(float x, uint32_t bit) { return __uint_as_
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
+__device__ __forceinline__ uint32_t half2_bits(float x, float y) { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }
+__device__ __forceinline__ uint32_t hsub2(uint32_t x, uint32_t y) {
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&y));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+// The power of two that brings a row's largest value to 2^13 .. 2^14, within what a float and its inverse hold.
+__device__ __forceinline__ int query_exponent(float top) { return min(126, max(-126, 140 - (int)((__float_as_uint(top) >> 23) & 255u))); }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Four 4-bit codes (the low 16 bits of w) as bytes 128 + centroid.  A selector with bit 3 set yields a byte's sign, here 0: of the two
+// tables each index finds its magnitude in one and 0 in the other.
+__device__ __forceinline__ uint32_t centroids4(uint32_t w) {
+    constexpr uint32_t HI0 = 0x2C1F1206u, HI1 = 0x7F604B3Au, LO0 = 0x3A4B607Fu, LO1 = 0x06121F2Cu;
+    return (prmt(HI0, HI1, w ^ 0x8888u) | 0x80808080u) - prmt(LO0, LO1, w);
+}
+// Bytes 128 + c as halves c: 0x6400 + byte is 1024 + byte.
+__device__ __forceinline__ uint32_t halves_lo(uint32_t x) { return hsub2(prmt(x, 0x64646464u, 0x4140u), 0x64806480u); }
+__device__ __forceinline__ uint32_t halves_hi(uint32_t x) { return hsub2(prmt(x, 0x64646464u, 0x4342u), 0x64806480u); }
+
 constexpr uint32_t POOL_ERR_PAGE = 6;        // a page or slot outside the pool
 __device__ __forceinline__ void pool_bad_page(const PoolView &v) { atomicExch(v.err, POOL_ERR_PAGE); }
 

@@ -11,6 +11,7 @@
 // results, which pool_merge_kernel joins.
 #include <algorithm>
 
+#include "k2t_flash_tc.cuh"
 #include "k2t_kv_pool.cuh"
 #include "k2t_pool_attn.h"
 
@@ -21,14 +22,7 @@ constexpr uint32_t SP_WARPS = 4, SP_STAGES = 3, WAIT_LIMIT = 1u << 22;
 // CTAs on an SM: registers (two for rows of 128 with queries in two halves)
 template <int HD, int QT> struct SplitCtas { static constexpr uint32_t N = HD == 128 && QT == 2 ? 2 : 3; };
 template <int HD, int BITS, int QT> constexpr uint32_t split_smem() { return SP_WARPS * (SP_STAGES * PoolBlock<HD, BITS>::BYTES + QT * HD / 16 * 512); }
-constexpr float LOG2_E = 1.4426950408889634f;
 
-__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ uint32_t half2_bits(float x, float y) { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }
-__device__ __forceinline__ uint32_t hsub2(uint32_t x, uint32_t y) {
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&y));
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -181,10 +175,9 @@ template <int HD, int QT> __device__ __forceinline__ void load_query(const Split
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // 2^(13 - exponent of top), within what a float holds; its inverse goes into the factor of the scores
-        const int e = min(126, max(-126, 13 - (int)((__float_as_uint(top) >> 23) & 255u) + 127));
-        const float up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
-        c[r] = p.a.scale * LOG2_E * down;
+        const int e = query_exponent(top);
+        const float up = power_of_two(e);
+        c[r] = p.a.scale * LOG2E * power_of_two(-e);
 #pragma unroll
         for (int g = 0; g < HD / 64; ++g)
 #pragma unroll
@@ -201,16 +194,6 @@ template <int HD, int QT> __device__ __forceinline__ void load_query(const Split
                 }
     }
 }
-
-// Four 4-bit codes (the low 16 bits of w) as bytes 128 + centroid.  A selector with bit 3 set yields a byte's sign, here 0: of the two
-// tables each index finds its magnitude in one and 0 in the other.
-__device__ __forceinline__ uint32_t centroids4(uint32_t w) {
-    constexpr uint32_t HI0 = 0x2C1F1206u, HI1 = 0x7F604B3Au, LO0 = 0x3A4B607Fu, LO1 = 0x06121F2Cu;
-    return (prmt(HI0, HI1, w ^ 0x8888u) | 0x80808080u) - prmt(LO0, LO1, w);
-}
-// Bytes 128 + c as halves c: 0x6400 + byte is 1024 + byte.
-__device__ __forceinline__ uint32_t halves_lo(uint32_t x) { return hsub2(prmt(x, 0x64646464u, 0x4140u), 0x64806480u); }
-__device__ __forceinline__ uint32_t halves_hi(uint32_t x) { return hsub2(prmt(x, 0x64646464u, 0x4342u), 0x64806480u); }
 
 template <int HD> struct State {
     float o[HD / 8][4], m[2], l[2];
@@ -314,7 +297,7 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
             float top = r == 0 ? top0 : top1;
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m = fmaxf(st.m[r], top), al = m == -INFINITY ? 1.0f : exp2_fast(st.m[r] - m);
+            const float m = fmaxf(st.m[r], top), al = m == -INFINITY ? 1.0f : exp2_approx(st.m[r] - m);
             st.m[r] = m;
             st.l[r] *= al;
 #pragma unroll
@@ -326,7 +309,7 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
         const float m = st.m[r] == -INFINITY ? 0.0f : st.m[r];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[r][i] = exp2_fast(x[r][i] - m);
+            x[r][i] = exp2_approx(x[r][i] - m);
             st.l[r] = __fmaf_rn(x[r][i], iv[i], st.l[r]);
         }
     }
@@ -574,7 +557,7 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
             }
         }
         const uint64_t far = prefix_line(p), per = part_blocks(far + total * kh * p.rbo, p.units);
-        if (far > 0) {
+        if (far > 0 && !p.flash.on) {
             near_item = h * p.rbp + r / 16;
             const uint64_t b = (uint64_t)near_item * prefix_blocks(p), e = b + prefix_blocks(p);
             near_first = (uint32_t)(b / per);
@@ -587,9 +570,22 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
             if (own_n == 1 && p.a.prefix_len == 0) return;
         }
     }
+    if (p.flash.on) {
+        const FlashArgs &f = p.flash;
+        near_item = h * f.row_tiles + (f.halved ? 0u : r / (2 * FLASH_ROWS));
+        const uint32_t b = near_item * f.tiles, e = b + f.tiles;
+        near_first = b / f.part;
+        near_n = ((e - 1) / f.part + 1 - near_first) << (f.halved ? 1 : 0);
+    }
     const uint32_t n = near_n + own_n;
     auto slot = [&](uint32_t i, uint32_t &row, uint32_t &rows) -> const float * {
         const bool near = i < near_n;
+        if (near && p.flash.on) {             // two tiles of rows, or two streams over the same rows
+            const uint32_t second = p.flash.halved ? i & 1u : r / FLASH_ROWS & 1u;
+            row = r % FLASH_ROWS;
+            rows = FLASH_ROWS;
+            return p.near + (size_t)(near_first + (p.flash.halved ? i >> 1 : i) + near_item) * flash_slot_floats(HD) + second * (flash_slot_floats(HD) / 2);
+        }
         row = near ? r % 16 : in % 16;
         rows = p.slot_rows(near);
         return near ? p.slot(true, near_first + i, near_item) : p.slot(false, own_first + i - near_n, own_item);
@@ -619,7 +615,7 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
             const float2 x = __ldcg(reinterpret_cast<const float2 *>(s + row * HD) + lane);
             v[0] = x.x; v[1] = x.y;
         }
-        const float w = exp2_fast(ml.x - top);
+        const float w = exp2_approx(ml.x - top);
         l = __fmaf_rn(w, ml.y, l);
 #pragma unroll
         for (int k = 0; k < E; ++k) o[k] = __fmaf_rn(w, v[k], o[k]);
@@ -662,13 +658,26 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     const uint32_t group = a.heads / d.kv_heads;
     const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * ((group + 15) / 16), room = (uint64_t)a.sm_count * (d.head_dim == 128 && type != TYPE_BF16 ? SplitCtas<128, 2>::N : SplitCtas<128, 1>::N) * SP_WARPS;
     p.rbo = (group + 15) / 16;
-    p.rbp = a.prefix_len == 0 ? 0 : (a.n_tok * group + 15) / 16;
+    const uint32_t rows = a.n_tok * group;
+    p.flash.on = a.prefix_len > 0 && rows > 16;          // more than one tile of this kernel: k2t_pool_flash.cu
+    if (p.flash.on) {
+        FlashArgs &f = p.flash;
+        f.halved = rows <= FLASH_ROWS;
+        f.row_tiles = (rows + 2 * FLASH_ROWS - 1) / (2 * FLASH_ROWS);
+        f.items = d.kv_heads * f.row_tiles;
+        f.tiles = (a.prefix_len + 63) / 64;
+        f.part = (uint32_t)std::max<uint64_t>(FLASH_MIN_PART, ((uint64_t)f.items * f.tiles + a.sm_count - 1) / a.sm_count);
+    }
+    p.rbp = a.prefix_len == 0 || p.flash.on ? 0 : (rows + 15) / 16;
     p.direct = p.rbp == 0 && items >= 4 * room;
     p.units = (uint32_t)(p.direct ? items : room);
     return p;
 }
 size_t own_slots(const SplitArgs &p) { return p.direct ? p.units : p.units + (size_t)p.a.n_tok * p.a.pool.d.kv_heads * p.rbo; }
-size_t near_slots(const SplitArgs &p) { return p.rbp == 0 ? 0 : p.units + (size_t)p.a.pool.d.kv_heads * p.rbp; }
+size_t near_floats(const SplitArgs &p) {
+    if (p.flash.on) return ((size_t)p.a.sm_count + p.flash.items) * flash_slot_floats(p.a.pool.d.head_dim);
+    return p.rbp == 0 ? 0 : (p.units + (size_t)p.a.pool.d.kv_heads * p.rbp) * p.slot_floats(true);
+}
 
 // Halves of an operand: bf16 queries and weights are rounded to one each (11 bits where bf16 has 8); fp16 queries keep two, since a score is a
 // sum of head_dim roundings (one: an output of fp16 rows 2.3 times as far from 64 bits as its own rounding); fp32 keeps two of both.
@@ -695,7 +704,7 @@ size_t pool_work_bytes(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint3
     size_t most = 0;
     for (uint32_t type : {TYPE_F32, TYPE_BF16, TYPE_F16}) {
         const SplitArgs p = split_plan(a, type);
-        most = std::max(most, (own_slots(p) * p.slot_floats(false) + near_slots(p) * p.slot_floats(true)) * 4);
+        most = std::max(most, (own_slots(p) * p.slot_floats(false) + near_floats(p)) * 4);
     }
     return most;
 }
@@ -706,7 +715,13 @@ cudaError_t launch_pool_attend(cudaStream_t s, const PoolAttnArgs &a, uint32_t *
     p.near = p.own + own_slots(p) * p.slot_floats(false);
     const PoolShape &d = a.pool.d;
     const bool b8 = d.bits == 8;
-    const cudaError_t e = d.head_dim == 128 ? (b8 ? split_launch<128, 8>(s, p) : split_launch<128, 4>(s, p)) : b8 ? split_launch<64, 8>(s, p) : split_launch<64, 4>(s, p);
+    cudaError_t e = cudaSuccess;
+    if (p.flash.on) {
+        e = launch_pool_flash(s, p);
+        if (e != cudaSuccess) return e;
+        *launched += 1;
+    }
+    e = d.head_dim == 128 ? (b8 ? split_launch<128, 8>(s, p) : split_launch<128, 4>(s, p)) : b8 ? split_launch<64, 8>(s, p) : split_launch<64, 4>(s, p);
     *launched += 1;
     if (e != cudaSuccess || (p.direct && a.prefix_len == 0)) return e;
     *launched += 1;

@@ -4,6 +4,16 @@
 
 namespace k2t {
 
+// The prefix over many rows (k2t_pool_flash.cu): items are (kv head, 2 FLASH_ROWS rows), tiles of 64 positions; a line of items * tiles, `part` of it
+// a CTA.  halved: an item has at most FLASH_ROWS rows, and its tiles are dealt out to two streams over the same rows.
+constexpr uint32_t FLASH_ROWS = 128, FLASH_MIN_PART = 2;
+struct FlashArgs {
+    bool on, halved;
+    uint32_t items, row_tiles, tiles, part;
+};
+// partial results of a CTA and item: two of FLASH_ROWS rows
+__host__ __device__ constexpr uint32_t flash_slot_floats(uint32_t head_dim) { return 2 * FLASH_ROWS * (head_dim + 2); }
+
 // A partial result: rows x head_dim numerators, then (maximum, denominator) of each row.
 struct SplitArgs {
     PoolAttnArgs a;
@@ -11,6 +21,7 @@ struct SplitArgs {
     uint32_t units;              // warps
     bool direct;                 // every warp has one item
     float *own, *near;           // partial results of own rows; of the prefix
+    FlashArgs flash;
 
     __host__ __device__ uint32_t slot_rows(bool prefix) const { const uint32_t g = a.heads / a.pool.d.kv_heads; return prefix || g > 16 ? 16 : g; }
     __host__ __device__ uint32_t slot_floats(bool prefix) const { return (slot_rows(prefix) * (a.pool.d.head_dim + 2) + 3u) & ~3u; }       // 16-byte boundaries
@@ -24,5 +35,7 @@ __host__ __device__ inline uint64_t prefix_line(const SplitArgs &p) { return (ui
 // blocks of a warp's part: at least MIN_PART, since a part costs its queries and a partial result
 constexpr uint32_t MIN_PART = 4;
 __host__ __device__ inline uint64_t part_blocks(uint64_t all, uint32_t units) { const uint64_t n = (all + units - 1) / units; return n < MIN_PART ? MIN_PART : n; }
+
+cudaError_t launch_pool_flash(cudaStream_t s, const SplitArgs &p);
 
 }  // namespace k2t

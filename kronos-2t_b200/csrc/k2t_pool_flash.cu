@@ -1,0 +1,561 @@
+// Attention of many query rows over the pages of a shared prefix: the rows of all tokens against the same keys and values, on the
+// tensor-memory cores.  The mathematics is that of k2t_pool_attn.cu (weights that carry the values' scales, codes as exact halves).
+//   * A CTA takes a stretch of an item (kv head, 256 rows) of the prefix in tiles of 64 positions, as two STREAMS of 128 rows, or, where an
+//     item has no more than 128 rows, of even and odd tiles.  While the softmax warps of one stream work, the products of the other run.
+//   * Four warps bring tiles in: 16 bytes of codes a load, two tiles ahead in registers, expanded to halves in the operand layout (panels
+//     of 64 columns, 128-byte rows, 128-byte swizzle), and the tile's scales as column constants.
+//   * One thread issues S = Q K^T (queries from shared memory) and O += P V (weights from tensor memory, where they overwrite S).
+//   * Eight warps of softmax read S in fragments of 16x256b: a lane then has 4 rows and a quarter of the columns, so that it reads a quarter
+//     of the column constants; O is rescaled only where a row's maximum has grown by more than 2^8.
+// The tiles of all items form one line that is cut into equal parts, one per CTA; partial results are joined by pool_merge_kernel.
+#include "k2t_flash_tc.cuh"
+#include "k2t_kv_pool.cuh"
+#include "k2t_pool_attn.h"
+
+namespace k2t {
+namespace {
+
+constexpr uint32_t FL_KT = 64, FL_SOFT = 8, FL_CONV = 4, FL_WARPS = FL_SOFT + FL_CONV + 1, FL_THREADS = FL_WARPS * 32, FL_WAIT = 1u << 22, FL_COLS = 512;
+
+template <int HD, int BITS, int QT> struct Flash {
+    static constexpr uint32_t PD = HD / 64, G = PoolBlock<HD, BITS>::G, STAGES = HD == 128 && QT == 2 ? 2 : 4;
+    static constexpr uint32_t Q_TILE = PD * FLASH_ROWS * 128, K_TILE = PD * FL_KT * 128, CONST = G == 1 ? 24 : 48;        // bytes; CONST per pair of columns
+    static constexpr uint32_t CONSTS = 1024, FACTORS = CONSTS + STAGES * (FL_KT / 2) * CONST, HEAD = (FACTORS + 2 * FLASH_ROWS * 4 + 1023) / 1024 * 1024;
+    static constexpr uint32_t Q_AT = HEAD, K_AT = Q_AT + 2 * QT * Q_TILE, SMEM = K_AT + STAGES * 2 * K_TILE + 1024;
+};
+
+using u64 = unsigned long long;
+__device__ __forceinline__ u64 pair_of(uint32_t lo, uint32_t hi) { u64 d; asm("mov.b64 %0, {%1,%2};" : "=l"(d) : "r"(lo), "r"(hi)); return d; }
+__device__ __forceinline__ u64 pair_of(float lo, float hi) { return pair_of(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ void unpair(u64 p, float &lo, float &hi) { uint32_t a, b; asm("mov.b64 {%0,%1}, %2;" : "=r"(a), "=r"(b) : "l"(p)); lo = __uint_as_float(a); hi = __uint_as_float(b); }
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) { u64 d; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ u64 add2(u64 a, u64 b) { u64 d; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b)); return d; }
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) { u64 d; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c)); return d; }
+__device__ __forceinline__ void lds_pairs(uint32_t at, u64 &x, u64 &y) { asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(x), "=l"(y) : "r"(at)); }
+__device__ __forceinline__ u64 lds_pair(uint32_t at) { u64 x; asm volatile("ld.shared.b64 %0, [%1];" : "=l"(x) : "r"(at)); return x; }
+
+// 16 lanes of tensor memory in fragments: word 4 i + 2 k + e of a thread is row lane / 4 + 8 k, column 8 i + 2 (lane % 4) + e
+__device__ __forceinline__ void tm_ld_frag64(uint32_t taddr, uint32_t *v) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : K2T_R8(v, 0), K2T_R8(v, 8), K2T_R8(v, 16), K2T_R8(v, 24) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tm_ld_frag32(uint32_t taddr, uint32_t *v) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];" : K2T_R8(v, 0), K2T_R8(v, 8) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tm_st_frag32(uint32_t taddr, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::K2T_I8(v, 0), K2T_I8(v, 8), "r"(taddr) : "memory");
+}
+// 32 words of 16 lanes: word 2 i + k of a thread is row lane / 4 + 8 k, column 4 i + lane % 4
+__device__ __forceinline__ void tm_st_words32(uint32_t taddr, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::K2T_I8(v, 0), K2T_I8(v, 8), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void sts4(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
+struct Segment { uint32_t item, first, last; };          // tiles [first, last) of an item
+// Segment s of a CTA's part of the line; false behind the last.
+__device__ __forceinline__ bool segment_of(const FlashArgs &f, uint32_t s, Segment &g) {
+    const uint32_t x0 = blockIdx.x * f.part, x1 = min(f.items * f.tiles, x0 + f.part);
+    const uint32_t item = x0 / f.tiles + s, b = item * f.tiles;
+    if (b >= x1) return false;
+    g.item = item;
+    g.first = x0 > b ? x0 - b : 0;
+    g.last = min(f.tiles, x1 - b);
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------------ tiles
+// Where the 16-byte unit `unit` of a block's 16 rows lies in the rows: the inverse of row_place.
+template <uint32_t RB> __device__ __forceinline__ void unit_place(uint32_t unit, uint32_t &row, uint32_t &chunk) {
+    const uint32_t r = unit / (RB / 16), c = unit % (RB / 16), quad = (r >> 2) & 3u;
+    row = RB == 128 ? r : RB == 64 ? r ^ (quad & 1u) : r ^ ((quad >> 1) | ((quad & 1u) << 1));
+    chunk = RB == 128 ? c ^ ((quad << 1) ^ ((r & 1u) << 2)) : RB == 64 ? c ^ (2u * ((quad ^ (quad >> 1)) & 1u)) : c;
+}
+
+template <int HD, int BITS, int QT> struct Converter {
+    using B = PoolBlock<HD, BITS>;
+    using F = Flash<HD, BITS, QT>;
+    static constexpr uint32_t UNITS = FL_KT * B::RB / 16, PER = 2 * UNITS / (FL_CONV * 32);        // of keys or values; of a thread, both
+    struct Raw {
+        uint4 w[PER];
+        uint32_t ks[2], vs[2];        // a thread of the first 64: scales of position `thread` (fp32, or up to two bf16 in ks[0] / vs[0])
+        bool seen;
+    };
+    const SplitArgs &p;
+    uint32_t ct;
+
+    // The block that holds position `pos` of the prefix, or null.
+    __device__ __forceinline__ const uint8_t *block(uint32_t head, uint32_t pos) const {
+        const PoolShape &d = p.a.pool.d;
+        if (pos >= p.a.prefix_len) return nullptr;
+        const int32_t page = __ldg(p.a.prefix_pages + (pos >> d.page_shift));
+        if (page < 0 || (uint32_t)page >= d.num_pages) { pool_bad_page(p.a.pool); return nullptr; }
+        return p.a.pool.rows + ((((size_t)page * d.kv_heads + head) << (d.page_shift - 4)) + ((pos & ((1u << d.page_shift) - 1u)) >> 4)) * B::BYTES;
+    }
+    __device__ __forceinline__ void fetch(uint32_t head, uint32_t tile, Raw &r) const {
+#pragma unroll
+        for (uint32_t k = 0; k < PER; ++k) {
+            const uint32_t u = ct + k * FL_CONV * 32, v = u % UNITS, b = v / B::RB;
+            const uint8_t *at = block(head, tile * FL_KT + b * POOL_ROWS);
+            r.w[k] = at != nullptr ? __ldcg(reinterpret_cast<const uint4 *>(at + (u >= UNITS ? B::V_AT : 0u)) + v % B::RB) : make_uint4(0, 0, 0, 0);
+        }
+        r.seen = false;
+        if (ct < FL_KT) {
+            const uint32_t pos = tile * FL_KT + ct, row = ct % POOL_ROWS;
+            const uint8_t *at = block(head, pos);
+            r.seen = at != nullptr;
+            if (at != nullptr) {
+                if (BITS == 8) {
+                    r.ks[0] = __ldcg(reinterpret_cast<const uint32_t *>(at + B::KS_AT) + row);
+                    r.vs[0] = __ldcg(reinterpret_cast<const uint32_t *>(at + B::VS_AT) + row);
+                } else {
+#pragma unroll
+                    for (uint32_t g = 0; g < B::G; ++g) {
+                        r.ks[g] = (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(at + B::KS_AT) + row * B::G + g) << 16;
+                        r.vs[g] = (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(at + B::VS_AT) + row * B::G + g) << 16;
+                    }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void put(uint32_t s_tile, uint8_t *consts, const Raw &r) const {
+#pragma unroll
+        for (uint32_t k = 0; k < PER; ++k) {
+            const uint32_t u = ct + k * FL_CONV * 32, v = u % UNITS, b = v / B::RB;
+            uint32_t row, chunk;
+            unit_place<B::RB>(v % B::RB, row, chunk);
+            const uint32_t rt = b * POOL_ROWS + row, base = s_tile + (u >= UNITS ? F::K_TILE : 0u) + rt * 128;
+            const uint32_t w[4] = {r.w[k].x, r.w[k].y, r.w[k].z, r.w[k].w};
+            if (BITS == 8) {
+                // halves 16 chunk .. + 15: two 16-byte chunks; rows of 128 codes store them in turned order in their second half, which
+                // puts the eight lanes of a store on eight different chunk places
+                const uint32_t panel = base + (chunk >> 2) * (FL_KT * 128), c0 = (chunk & 3u) * 2, x = (rt & 7u);
+                const uint32_t a0 = halves_lo(w[0]), a1 = halves_hi(w[0]), a2 = halves_lo(w[1]), a3 = halves_hi(w[1]);
+                const uint32_t b0 = halves_lo(w[2]), b1 = halves_hi(w[2]), b2 = halves_lo(w[3]), b3 = halves_hi(w[3]);
+                const bool turn = chunk & 4u;
+                sts4(panel + (((c0 + (turn ? 1u : 0u)) ^ x) << 4), turn ? b0 : a0, turn ? b1 : a1, turn ? b2 : a2, turn ? b3 : a3);
+                sts4(panel + (((c0 + (turn ? 0u : 1u)) ^ x) << 4), turn ? a0 : b0, turn ? a1 : b1, turn ? a2 : b2, turn ? a3 : b3);
+            } else {
+                const uint32_t panel = base + (chunk >> 1) * (FL_KT * 128), c0 = (chunk & 1u) * 4, x = (rt & 7u);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t lo = centroids4(w[i]), hi = centroids4(w[i] >> 16);
+                    sts4(panel + (((c0 + i) ^ x) << 4), halves_lo(lo), halves_hi(lo), halves_lo(hi), halves_hi(hi));
+                }
+            }
+        }
+        if (ct < FL_KT) {
+            constexpr uint32_t G = B::G;
+            float ks[2], v[2], lv = -INFINITY, iv = 0.0f, part[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (uint32_t g = 0; g < G; ++g) {
+                ks[g] = r.seen ? __uint_as_float(r.ks[g]) : 0.0f;
+                v[g] = __uint_as_float(r.vs[g]);
+            }
+            if (r.seen) {
+                // a row of zeros: 8-bit codes are 0, and two groups have a factor each; a single group of 4-bit codes, which has neither, is
+                // given a scale below everything that counts
+                const float top = G == 1 ? v[0] : fmaxf(v[0], v[G - 1]), u = v[0] != v[0] ? v[0] : top == 0.0f ? (BITS == 4 && G == 1 ? 0x1p-100f : 1.0f) : top;
+                lv = __log2f(u);
+                iv = __fdividef(1.0f, u);
+#pragma unroll
+                for (uint32_t g = 0; g < G; ++g) part[g] = v[g] * iv;
+            }
+            float *c = reinterpret_cast<float *>(consts);
+            const uint32_t i = ct >> 1, e = ct & 1u;
+            if (G == 1) {
+                c[4 * i + e] = ks[0];
+                c[4 * i + 2 + e] = lv;
+                c[4 * (FL_KT / 2) + 2 * i + e] = iv;
+            } else {
+                c[12 * i + e] = ks[0];
+                c[12 * i + 2 + e] = ks[1];
+                c[12 * i + 4 + e] = lv;
+                c[12 * i + 6 + e] = iv;
+                c[12 * i + 8 + e] = part[0];
+                c[12 * i + 10 + e] = part[1];
+            }
+        }
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ queries
+// Eight warps write the item's rows: transformed, scaled by a power of two, one or two halves; their factors to s_c.
+template <int HD, int BITS, int QT> __device__ __forceinline__ void flash_queries(const SplitArgs &p, const FlashArgs &f, uint32_t item, uint32_t warp, uint32_t lane, uint32_t s_q, float *s_c) {
+    using F = Flash<HD, BITS, QT>;
+    constexpr uint32_t LANES = HD / 8, ROWS = 32 / LANES;
+    const uint32_t group = p.a.heads / p.a.pool.d.kv_heads, all = p.a.n_tok * group, h = item / f.row_tiles, r0 = item % f.row_tiles * 2 * FLASH_ROWS;
+    const uint32_t mine = (f.halved ? FLASH_ROWS : 2 * FLASH_ROWS) / FL_SOFT, l = lane % LANES;
+    const uint32_t signs = p.a.pool.signs[l / 4] >> (l % 4 * 8);
+#pragma unroll 2
+    for (uint32_t i = 0; i < mine; i += ROWS) {
+        const uint32_t row = warp * mine + i + lane / LANES, r = r0 + row;
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, top = 0.0f;
+        if (r < all) rows_get8(p.a.q, r / group * p.a.q.token_stride + (h * group + r % group) * p.a.q.head_stride + l * 8, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = __fmul_rn(flip(v[k], signs >> k & 1u), 0.125f);
+        butterflies_in(v);
+#pragma unroll
+        for (uint32_t m = 1; m < 8; m <<= 1) butterflies_across(v, m, lane);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
+#pragma unroll
+        for (uint32_t m = LANES / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+        const int e = query_exponent(top);
+        const float up = power_of_two(e);
+        if (l == 0) s_c[row] = p.a.scale * LOG2E * power_of_two(-e);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float x = v[2 * k] * up, y = v[2 * k + 1] * up;
+            hi[k] = half2_bits(x, y);
+            const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&hi[k]));
+            lo[k] = half2_bits(x - g.x, y - g.y);
+        }
+        const uint32_t at = s_q + row / FLASH_ROWS * QT * F::Q_TILE + (l / 8) * (FLASH_ROWS * 128) + row % FLASH_ROWS * 128 + (((l % 8) ^ (row & 7u)) << 4);
+        sts4(at, hi[0], hi[1], hi[2], hi[3]);
+        if (QT == 2) sts4(at + F::Q_TILE, lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+
+template <int HD, int BITS, int QT, int PT>
+__global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_constant__ SplitArgs p) {
+    using F = Flash<HD, BITS, QT>;
+    constexpr uint32_t G = F::G, STAGES = F::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw), sbase = (raw + 1023u) & ~1023u;
+    uint8_t *smem = smem_raw + (sbase - raw);
+    const FlashArgs &f = p.flash;
+    // barriers: tiles landed / free; of each stream: S ready (two buffers), weights ready (two), O updated; queries; end of a segment; end
+    const uint32_t b_full = sbase, b_free = b_full + 8 * STAGES, b_s = b_free + 8 * STAGES, b_p = b_s + 32, b_o = b_p + 32, b_q = b_o + 16, b_end = b_q + 8, b_last = b_end + 8;
+    volatile uint32_t *s_tmem = reinterpret_cast<volatile uint32_t *>(smem + 512), *s_abort = reinterpret_cast<volatile uint32_t *>(smem + 516);
+    float *s_c = reinterpret_cast<float *>(smem + F::FACTORS);
+    const uint32_t s_q = sbase + F::Q_AT, s_k = sbase + F::K_AT;
+    if (tid == 0) {
+        for (uint32_t i = 0; i < STAGES; ++i) { mbar_init(b_full + 8 * i, FL_CONV); mbar_init(b_free + 8 * i, 1); }
+        for (uint32_t i = 0; i < 4; ++i) { mbar_init(b_s + 8 * i, 1); mbar_init(b_p + 8 * i, 128); }
+        for (uint32_t i = 0; i < 2; ++i) mbar_init(b_o + 8 * i, 1);
+        mbar_init(b_q, FL_SOFT);
+        mbar_init(b_end, 1);
+        mbar_init(b_last, 1);
+        *s_abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == FL_WARPS - 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sbase + 512), "r"(FL_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    pdl_wait();
+    pdl_trigger();
+    // tensor memory of a stream: 128 columns of S (two buffers, or a tile's two groups of 64 elements), HD columns of O
+    const uint32_t t_stream = 128 + HD;
+    Segment g;
+    bool ok = true;
+
+    if (warp >= FL_SOFT && warp < FL_SOFT + FL_CONV) {
+        const Converter<HD, BITS, QT> cv{p, tid - FL_SOFT * 32};
+        uint32_t n = 0;                            // tiles of the CTA so far
+        typename Converter<HD, BITS, QT>::Raw ring[2];
+        // tiles two ahead, over the ends of segments
+        Segment ahead;
+        uint32_t as = 0, at = 0;
+        bool more = segment_of(f, 0, ahead);
+        if (more) at = ahead.first;
+        auto fetch = [&](typename Converter<HD, BITS, QT>::Raw &r) {
+            if (!more) return;
+            cv.fetch(ahead.item / f.row_tiles, at, r);
+            if (++at == ahead.last) {
+                more = segment_of(f, ++as, ahead);
+                if (more) at = ahead.first;
+            }
+        };
+        fetch(ring[0]);
+        fetch(ring[1]);
+        for (uint32_t s = 0; ok && segment_of(f, s, g); ++s)
+            for (uint32_t t = g.first; t < g.last; ++t, ++n) {
+                const uint32_t stage = n % STAGES;
+                if (n >= STAGES) ok = mbar_wait_warp(b_free + 8 * stage, (n / STAGES - 1) & 1u, FL_WAIT, s_abort);
+                if (!ok) break;
+                if (n & 1u) { cv.put(s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST, ring[1]); fetch(ring[1]); }
+                else { cv.put(s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST, ring[0]); fetch(ring[0]); }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(b_full + 8 * stage);
+            }
+    } else if (warp == FL_WARPS - 1) {
+        if (lane == 0) {
+            // fp32 accumulators, fp16 operands; A and B K-major for S, B with its columns consecutive for O
+            constexpr uint32_t id_s = (1u << 4) | ((FL_KT >> 3) << 17) | ((FLASH_ROWS >> 4) << 24);
+            constexpr uint32_t id_o = (1u << 4) | (1u << 16) | (((G == 1 ? HD : 64) >> 3) << 17) | ((FLASH_ROWS >> 4) << 24);
+            uint32_t n0 = 0, done[2] = {0, 0};             // tiles of the CTA before the segment; tiles of the streams before it
+            for (uint32_t s = 0; ok && segment_of(f, s, g); ++s) {
+                const uint32_t n = g.last - g.first, count[2] = {f.halved ? (n + 1) / 2 : n, f.halved ? n / 2 : n};
+                auto tile_of = [&](uint32_t st, uint32_t i) { return n0 + (f.halved ? 2 * i + st : i); };
+                auto scores = [&](uint32_t st, uint32_t i) {
+                    const uint32_t tile = tile_of(st, i), stage = tile % STAGES, use = done[st] + i, buf = G == 1 ? use & 1u : 0u;
+                    if (!mbar_wait_thread(b_full + 8 * stage, (tile / STAGES) & 1u, FL_WAIT, s_abort)) return false;
+                    tc_fence_after();
+                    const uint32_t q = s_q + (f.halved ? 0u : st) * QT * F::Q_TILE, k = s_k + stage * 2 * F::K_TILE, t_s = tmem + st * t_stream + buf * FL_KT;
+#pragma unroll
+                    for (uint32_t c = 0; c < HD / 16; ++c)
+#pragma unroll
+                        for (uint32_t x = 0; x < QT; ++x)
+                            mma_ss(t_s + (G == 2 ? c / 4 * FL_KT : 0u), desc_k(q + x * F::Q_TILE + (c / 4) * FLASH_ROWS * 128 + (c % 4) * 32), desc_k(k + (c / 4) * FL_KT * 128 + (c % 4) * 32), id_s,
+                                   (x == 0 && (G == 2 ? c % 4 : c) == 0) ? 0u : 1u);
+                    tc_commit(b_s + 8 * (2 * st + buf));
+                    return true;
+                };
+                ok = mbar_wait_thread(b_q, s & 1u, FL_WAIT, s_abort);
+                for (uint32_t st = 0; ok && st < 2; ++st)
+                    if (count[st] > 0) ok = scores(st, 0);
+                for (uint32_t i = 0; ok && i < count[0]; ++i) {
+                    for (uint32_t st = 0; ok && st < 2; ++st) {
+                        if (i >= count[st]) continue;
+                        const uint32_t use = done[st] + i, buf = G == 1 ? use & 1u : 0u, tile = tile_of(st, i), stage = tile % STAGES;
+                        if (G == 1 && i + 1 < count[st]) {
+                            // the weights of tile i - 1 lie where S of tile i + 1 goes
+                            if (i >= 1) ok = mbar_wait_thread(b_o + 8 * st, (use - 1) & 1u, FL_WAIT, s_abort);
+                            ok = ok && scores(st, i + 1);
+                            if (!ok) break;
+                        }
+                        ok = mbar_wait_thread(b_p + 8 * (2 * st + buf), (G == 1 ? use >> 1 : use) & 1u, FL_WAIT, s_abort);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t t_p = tmem + st * t_stream + buf * FL_KT, t_o = tmem + st * t_stream + 128, v = s_k + stage * 2 * F::K_TILE + F::K_TILE;
+#pragma unroll
+                        for (uint32_t x = 0; x < G; ++x)
+#pragma unroll
+                            for (uint32_t y = 0; y < PT; ++y)
+#pragma unroll
+                                for (uint32_t k = 0; k < FL_KT / 16; ++k)
+                                    mma_ts(t_o + x * 64, t_p + (x * PT + y) * 32 + k * 8, desc_mn(v + x * FL_KT * 128 + k * 16 * 128, FL_KT * 128), id_o, (i | y | k) != 0 ? 1u : 0u);
+                        if (f.halved || st == 1) tc_commit(b_free + 8 * stage);
+                        tc_commit(b_o + 8 * st);
+                    }
+                    if (G == 2)
+                        for (uint32_t st = 0; ok && st < 2; ++st)
+                            if (i + 1 < count[st]) {
+                                ok = mbar_wait_thread(b_o + 8 * st, (done[st] + i) & 1u, FL_WAIT, s_abort);
+                                ok = ok && scores(st, i + 1);
+                            }
+                }
+                tc_commit(b_end);
+                n0 += n;
+                done[0] += count[0];
+                done[1] += count[1];
+            }
+            tc_commit(b_last);               // also after a wait that gave up: the products in flight end before the CTA leaves
+            for (uint32_t spin = 0; spin < FL_WAIT && !mbar_try_wait(b_last, 0); ++spin) {}
+            if (!ok) atomicCAS(p.a.pool.err, 0u, 1u);
+        }
+    } else {
+        const uint32_t st = warp / 4, quarter = warp % 4, lr = lane >> 2, lc = lane & 3u;
+        const uint32_t group = p.a.heads / p.a.pool.d.kv_heads, all = p.a.n_tok * group;
+        const uint32_t t_s0 = tmem + st * t_stream + ((quarter * 32u) << 16), t_o = t_s0 + 128;
+        uint32_t n0 = 0, done = 0;
+        for (uint32_t s = 0; ok && segment_of(f, s, g); ++s) {
+            flash_queries<HD, BITS, QT>(p, f, g.item, warp, lane, s_q, s_c);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_q);
+            ok = mbar_wait_warp(b_q, s & 1u, FL_WAIT, s_abort);          // the factors of all rows
+            if (!ok) break;
+            const uint32_t n = g.last - g.first, count = f.halved ? (n + 1 - st) / 2 : n;
+            const uint32_t r0 = g.item % f.row_tiles * 2 * FLASH_ROWS + (f.halved ? 0u : st * FLASH_ROWS), left = all > r0 ? all - r0 : 0;          // rows of the stream's tile
+            const bool idle = quarter * 32 >= left;
+            float c[4], m[4], l[4];                // rows quarter * 32 + lr + 8 k
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                c[k] = s_c[(f.halved ? 0u : st * FLASH_ROWS) + quarter * 32 + lr + 8 * k];
+                m[k] = -INFINITY;
+                l[k] = 0.0f;
+            }
+            for (uint32_t i = 0; i < count; ++i) {
+                const uint32_t use = done + i, buf = G == 1 ? use & 1u : 0u, tile = n0 + (f.halved ? 2 * i + st : i), stage = tile % STAGES;
+                ok = mbar_wait_warp(b_s + 8 * (2 * st + buf), (G == 1 ? use >> 1 : use) & 1u, FL_WAIT, s_abort);
+                if (!ok) break;
+                ok = mbar_wait_warp(b_full + 8 * stage, (tile / STAGES) & 1u, FL_WAIT, s_abort);          // this thread's view of the constants
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t s_const = sbase + F::CONSTS + stage * (FL_KT / 2) * F::CONST;
+#pragma unroll
+                for (uint32_t half = 0; half < 2; ++half) {
+                    if (idle) break;
+                    const uint32_t t_s = t_s0 + buf * FL_KT + ((16u * half) << 16);
+                    uint32_t v[G * 32];
+                    tm_ld_frag64(t_s, v);
+                    if (G == 2) tm_ld_frag64(t_s + FL_KT, v + (G - 1) * 32);
+                    tm_ld_wait();
+                    u64 x[8][2];
+                    const u64 ca = pair_of(c[2 * half], c[2 * half]), cb = pair_of(c[2 * half + 1], c[2 * half + 1]);
+                    float ta = -INFINITY, tb = -INFINITY;
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k) {
+                        const uint32_t j = 4 * k + lc;          // pair of columns
+                        u64 ks, lv;
+                        if (G == 1) {
+                            lds_pairs(s_const + j * 16, ks, lv);
+                            x[k][0] = fma2(mul2(pair_of(v[4 * k], v[4 * k + 1]), ca), ks, lv);
+                            x[k][1] = fma2(mul2(pair_of(v[4 * k + 2], v[4 * k + 3]), cb), ks, lv);
+                        } else {
+                            u64 k2;
+                            lds_pairs(s_const + j * 48, ks, k2);
+                            lv = lds_pair(s_const + j * 48 + 16);
+                            constexpr uint32_t H = (G - 1) * 32;
+                            x[k][0] = fma2(fma2(pair_of(v[H + 4 * k], v[H + 4 * k + 1]), k2, mul2(pair_of(v[4 * k], v[4 * k + 1]), ks)), ca, lv);
+                            x[k][1] = fma2(fma2(pair_of(v[H + 4 * k + 2], v[H + 4 * k + 3]), k2, mul2(pair_of(v[4 * k + 2], v[4 * k + 3]), ks)), cb, lv);
+                        }
+                        float lo, hi;
+                        unpair(x[k][0], lo, hi);
+                        ta = fmaxf(ta, fmaxf(lo, hi));
+                        unpair(x[k][1], lo, hi);
+                        tb = fmaxf(tb, fmaxf(lo, hi));
+                    }
+                    if (__any_sync(0xffffffffu, ta > m[2 * half] + 8.0f || tb > m[2 * half + 1] + 8.0f)) {
+#pragma unroll
+                        for (uint32_t o = 1; o < 4; o <<= 1) {
+                            ta = fmaxf(ta, __shfl_xor_sync(0xffffffffu, ta, o));
+                            tb = fmaxf(tb, __shfl_xor_sync(0xffffffffu, tb, o));
+                        }
+                        const float ma = fmaxf(m[2 * half], ta), mb = fmaxf(m[2 * half + 1], tb);
+                        if (i > 0) {
+                            ok = mbar_wait_warp(b_o + 8 * st, (use - 1) & 1u, FL_WAIT, s_abort);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const float aa = ma == -INFINITY ? 1.0f : exp2_approx(m[2 * half] - ma), ab = mb == -INFINITY ? 1.0f : exp2_approx(m[2 * half + 1] - mb);
+#pragma unroll 1
+                            for (uint32_t col = 0; col < HD; col += 32) {
+                                uint32_t o[16];
+                                tm_ld_frag32(t_o + ((16u * half) << 16) + col, o);
+                                tm_ld_wait();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * ((k & 2) ? ab : aa));
+                                tm_st_frag32(t_o + ((16u * half) << 16) + col, o);
+                            }
+                            l[2 * half] *= aa;
+                            l[2 * half + 1] *= ab;
+                        }
+                        m[2 * half] = ma;
+                        m[2 * half + 1] = mb;
+                    }
+                    const float na = m[2 * half] == -INFINITY ? 0.0f : -m[2 * half], nb = m[2 * half + 1] == -INFINITY ? 0.0f : -m[2 * half + 1];
+                    const u64 ma = pair_of(na, na), mb = pair_of(nb, nb);
+                    u64 sa = 0, sb = 0;
+                    uint32_t w[G][PT][16];
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k) {
+                        const uint32_t j = 4 * k + lc;
+                        u64 iv, pa = 0, pb = 0;
+                        if (G == 1) {
+                            iv = lds_pair(s_const + FL_KT / 2 * 16 + j * 8);
+                        } else {
+                            iv = lds_pair(s_const + j * 48 + 24);
+                            lds_pairs(s_const + j * 48 + 32, pa, pb);
+                        }
+#pragma unroll
+                        for (uint32_t r = 0; r < 2; ++r) {
+                            float lo, hi;
+                            unpair(add2(x[k][r], r == 0 ? ma : mb), lo, hi);
+                            lo = exp2_approx(lo);
+                            hi = exp2_approx(hi);
+                            const u64 e = pair_of(lo, hi);
+                            if (r == 0) sa = fma2(e, iv, sa);
+                            else sb = fma2(e, iv, sb);
+#pragma unroll
+                            for (uint32_t y = 0; y < G; ++y) {
+                                if (G == 2) unpair(mul2(e, y == 0 ? pa : pb), lo, hi);
+                                w[y][0][2 * k + r] = half2_bits(lo, hi);
+                                if (PT == 2) {
+                                    const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[y][0][2 * k + r]));
+                                    w[y][PT - 1][2 * k + r] = half2_bits(lo - t.x, hi - t.y);
+                                }
+                            }
+                        }
+                    }
+                    float lo, hi;
+                    unpair(sa, lo, hi);
+                    l[2 * half] += lo + hi;
+                    unpair(sb, lo, hi);
+                    l[2 * half + 1] += lo + hi;
+#pragma unroll
+                    for (uint32_t y = 0; y < G; ++y)
+#pragma unroll
+                        for (uint32_t z = 0; z < PT; ++z) tm_st_words32(t_s + (y * PT + z) * 32, w[y][z]);
+                }
+                if (!ok) break;
+                tm_st_wait();
+                tc_fence_before();
+                mbar_arrive(b_p + 8 * (2 * st + buf));
+            }
+            if (!ok) break;
+            // the segment's last update by a barrier of its own: the phases of b_o may be two behind here, and a parity tells only neighbours apart
+            ok = mbar_wait_warp(b_end, s & 1u, FL_WAIT, s_abort);
+            if (!ok) break;
+            tc_fence_after();
+            float *slot = p.near + (size_t)(blockIdx.x + g.item) * flash_slot_floats(HD) + st * flash_slot_floats(HD) / 2;
+            if (!idle) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (uint32_t o = 1; o < 4; o <<= 1) l[k] += __shfl_xor_sync(0xffffffffu, l[k], o);
+#pragma unroll 1
+                for (uint32_t half = 0; half < 2; ++half)
+#pragma unroll 1
+                    for (uint32_t col = 0; col < HD; col += 32) {
+                        uint32_t o[16];
+                        tm_ld_frag32(t_o + ((16u * half) << 16) + col, o);
+                        tm_ld_wait();
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k) {          // row k & 1, columns of group k / 2
+                            const uint32_t row = quarter * 32 + half * 16 + lr + 8 * (k & 1u);
+                            const float2 val = count == 0 ? make_float2(0.0f, 0.0f) : make_float2(__uint_as_float(o[4 * (k / 2) + 2 * (k & 1u)]), __uint_as_float(o[4 * (k / 2) + 2 * (k & 1u) + 1]));
+                            if (row < left) *reinterpret_cast<float2 *>(slot + row * HD + col + 8 * (k / 2) + 2 * lc) = val;
+                        }
+                    }
+#pragma unroll
+                for (uint32_t k = 0; k < 4; ++k) {
+                    const uint32_t row = quarter * 32 + lr + 8 * k;
+                    if (lc == 0 && row < left) *reinterpret_cast<float2 *>(slot + FLASH_ROWS * HD + 2 * row) = make_float2(m[k], l[k]);
+                }
+            }
+            tc_fence_before();
+            n0 += n;
+            done += count;
+        }
+        if (!ok && lane == 0) atomicCAS(p.a.pool.err, 0u, 1u);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == FL_WARPS - 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(FL_COLS) : "memory");
+    }
+}
+
+template <int HD, int BITS, int QT, int PT> cudaError_t flash_go(cudaStream_t s, const SplitArgs &p) {
+    constexpr uint32_t smem = Flash<HD, BITS, QT>::SMEM;
+    static_assert(smem <= 232448, "shared memory of an SM");
+    const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(pool_flash_kernel<HD, BITS, QT, PT>), smem);
+    if (e != cudaSuccess) return e;
+    const uint32_t line = p.flash.items * p.flash.tiles;
+    return launch_kernel(pool_flash_kernel<HD, BITS, QT, PT>, dim3((line + p.flash.part - 1) / p.flash.part), dim3(FL_THREADS), smem, s, true, p);
+}
+template <int HD, int BITS> cudaError_t flash_type(cudaStream_t s, const SplitArgs &p) {
+    const uint32_t type = p.a.q.type;
+    return type == TYPE_F32 ? flash_go<HD, BITS, 2, 2>(s, p) : type == TYPE_F16 ? flash_go<HD, BITS, 2, 1>(s, p) : flash_go<HD, BITS, 1, 1>(s, p);
+}
+
+}  // namespace
+
+cudaError_t launch_pool_flash(cudaStream_t s, const SplitArgs &p) {
+    const PoolShape &d = p.a.pool.d;
+    return d.head_dim == 128 ? (d.bits == 8 ? flash_type<128, 8>(s, p) : flash_type<128, 4>(s, p)) : d.bits == 8 ? flash_type<64, 8>(s, p) : flash_type<64, 4>(s, p);
+}
+
+}  // namespace k2t

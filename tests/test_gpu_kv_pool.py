@@ -229,6 +229,21 @@ def test_attention_behind_a_shared_prefix(ctx, d, bits, dtype, prefix, kh, heads
     c.check(got, q, lens, seq)
 
 
+@pytest.mark.parametrize("d,bits", SHAPES)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("prefix,kh,heads,seqs", [(3001, 8, 64, 40), (2500, 5, 5, 100), (9000, 1, 6, 45)])
+def test_a_prefix_over_many_rows(ctx, d, bits, dtype, prefix, kh, heads, seqs):
+    """Rows of several tiles, parts that begin and end inside an item, and items of one tile of rows."""
+    rng = np.random.default_rng(seqs)
+    ends = rng.integers(0, 40, seqs)
+    c = Cache(ctx, ends, kh, d, bits, 64, dtype, prefix=prefix, seed=prefix)
+    q = c.queries(seqs, heads)
+    got = c.attend(q, ends)
+    assert np.array_equal(got, c.attend(q, ends))
+    pick = rng.permutation(seqs)[:6]
+    c.check(got[pick], q[pick], ends[pick], pick)
+
+
 @pytest.mark.parametrize("prefix", [0, 70])
 def test_many_short_tokens(ctx, prefix):
     """More items than warps: one warp each."""
