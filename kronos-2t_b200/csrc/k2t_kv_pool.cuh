@@ -122,6 +122,8 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t x, uint32_t y) {
     const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&x), *reinterpret_cast<const __half2 *>(&y));
     return *reinterpret_cast<const uint32_t *>(&h);
 }
+__device__ __forceinline__ float log2_approx(float x) { float y; asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ float rcp_approx(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // The power of two that brings a row's largest value to 2^13 .. 2^14, within what a float and its inverse hold.
 __device__ __forceinline__ int query_exponent(float top) { return min(126, max(-126, 140 - (int)((__float_as_uint(top) >> 23) & 255u))); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }

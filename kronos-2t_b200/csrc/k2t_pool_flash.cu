@@ -34,6 +34,8 @@ __device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) { u64 d; asm("fma.rn.f3
 __device__ __forceinline__ void lds_pairs(uint32_t at, u64 &x, u64 &y) { asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(x), "=l"(y) : "r"(at)); }
 __device__ __forceinline__ u64 lds_pair(uint32_t at) { u64 x; asm volatile("ld.shared.b64 %0, [%1];" : "=l"(x) : "r"(at)); return x; }
 
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+
 // 16 lanes of tensor memory in fragments: word 4 i + 2 k + e of a thread is row lane / 4 + 8 k, column 8 i + 2 (lane % 4) + e
 __device__ __forceinline__ void tm_ld_frag64(uint32_t taddr, uint32_t *v) {
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -66,84 +68,96 @@ __device__ __forceinline__ bool segment_of(const FlashArgs &f, uint32_t s, Segme
 }
 
 // ------------------------------------------------------------------------------------------------ tiles
-// Where the 16-byte unit `unit` of a block's 16 rows lies in the rows: the inverse of row_place.
-template <uint32_t RB> __device__ __forceinline__ void unit_place(uint32_t unit, uint32_t &row, uint32_t &chunk) {
-    const uint32_t r = unit / (RB / 16), c = unit % (RB / 16), quad = (r >> 2) & 3u;
+// Where the 16-byte unit (r, c) of a block's 16 rows lies in the rows: the inverse of row_place.
+template <uint32_t RB> __device__ __forceinline__ void unit_place(uint32_t r, uint32_t c, uint32_t &row, uint32_t &chunk) {
+    const uint32_t quad = (r >> 2) & 3u;
     row = RB == 128 ? r : RB == 64 ? r ^ (quad & 1u) : r ^ ((quad >> 1) | ((quad & 1u) << 1));
     chunk = RB == 128 ? c ^ ((quad << 1) ^ ((r & 1u) << 2)) : RB == 64 ? c ^ (2u * ((quad ^ (quad >> 1)) & 1u)) : c;
 }
 
+// 128 threads.  A thread has the same unit of 16 bytes in every block it reads (a block of keys or values has RB units: one per thread, or
+// a thread reads every second or fourth block), so what it does to a block is loads and stores at fixed distances.
 template <int HD, int BITS, int QT> struct Converter {
     using B = PoolBlock<HD, BITS>;
     using F = Flash<HD, BITS, QT>;
-    static constexpr uint32_t UNITS = FL_KT * B::RB / 16, PER = 2 * UNITS / (FL_CONV * 32);        // of keys or values; of a thread, both
+    static constexpr uint32_t BLOCKS = FL_KT / POOL_ROWS, STEP = 128 / B::RB, PER = BLOCKS / STEP;          // blocks of a tile; between two of a thread; of a thread
+    static_assert(FL_CONV == 4, "128 threads");
     struct Raw {
-        uint4 w[PER];
-        uint32_t ks[2], vs[2];        // a thread of the first 64: scales of position `thread` (fp32, or up to two bf16 in ks[0] / vs[0])
+        uint4 k[PER], v[PER];
+        uint32_t ks[2], vs[2];        // threads below 64: scales of position `thread` (fp32, or of each group)
         bool seen;
     };
     const SplitArgs &p;
-    uint32_t ct;
+    uint32_t ct, lane, first, load_at, store_at, store_x;
 
-    // The block that holds position `pos` of the prefix, or null.
-    __device__ __forceinline__ const uint8_t *block(uint32_t head, uint32_t pos) const {
-        const PoolShape &d = p.a.pool.d;
-        if (pos >= p.a.prefix_len) return nullptr;
-        const int32_t page = __ldg(p.a.prefix_pages + (pos >> d.page_shift));
-        if (page < 0 || (uint32_t)page >= d.num_pages) { pool_bad_page(p.a.pool); return nullptr; }
-        return p.a.pool.rows + ((((size_t)page * d.kv_heads + head) << (d.page_shift - 4)) + ((pos & ((1u << d.page_shift) - 1u)) >> 4)) * B::BYTES;
+    __device__ __forceinline__ Converter(const SplitArgs &args, uint32_t thread) : p(args), ct(thread), lane(thread & 31u) {
+        // eight neighbouring threads: four chunks of two neighbouring rows, whose stores meet in no bank (rows differ in the last bit of the swizzle)
+        const uint32_t u = ct % B::RB;
+        first = ct / B::RB;
+        uint32_t r, c;
+        if (B::RB == 128) { c = (u & 3u) | (u >> 1 & 4u); r = (u >> 2 & 1u) | (u >> 4) << 1; }
+        else { c = u % (B::RB / 16); r = u / (B::RB / 16); }
+        load_at = (r * (B::RB / 16) + c) * 16;
+        uint32_t row, chunk;
+        unit_place<B::RB>(r, c, row, chunk);
+        const uint32_t c0 = BITS == 8 ? chunk * 2 : chunk * 4;          // first 16-byte chunk of halves
+        store_at = (c0 >> 3) * (FL_KT * 128) + row * 128;
+        store_x = (c0 & 7u) ^ (row & 7u);
     }
+    // Lane b < BLOCKS: the place of block b of a tile in the pool, ~0 where nothing of it is in sight.
+    __device__ __forceinline__ uint32_t place(uint32_t head, uint32_t tile) const {
+        const PoolShape &d = p.a.pool.d;
+        const uint32_t pos = tile * FL_KT + lane * POOL_ROWS;
+        if (lane >= BLOCKS || pos >= p.a.prefix_len) return ~0u;
+        const int32_t page = __ldg(p.a.prefix_pages + (pos >> d.page_shift));
+        if (page < 0 || (uint32_t)page >= d.num_pages) { pool_bad_page(p.a.pool); return ~0u; }
+        return (((uint32_t)page * d.kv_heads + head) << (d.page_shift - 4)) + ((pos & ((1u << d.page_shift) - 1u)) >> 4);
+    }
+    __device__ __forceinline__ const uint8_t *block(uint32_t at) const { return p.a.pool.rows + (size_t)(at == ~0u ? 0u : at) * B::BYTES; }          // any, where none is in sight
     __device__ __forceinline__ void fetch(uint32_t head, uint32_t tile, Raw &r) const {
+        const uint32_t mine = place(head, tile);
 #pragma unroll
-        for (uint32_t k = 0; k < PER; ++k) {
-            const uint32_t u = ct + k * FL_CONV * 32, v = u % UNITS, b = v / B::RB;
-            const uint8_t *at = block(head, tile * FL_KT + b * POOL_ROWS);
-            r.w[k] = at != nullptr ? __ldcg(reinterpret_cast<const uint4 *>(at + (u >= UNITS ? B::V_AT : 0u)) + v % B::RB) : make_uint4(0, 0, 0, 0);
+        for (uint32_t i = 0; i < PER; ++i) {
+            const uint8_t *at = block(__shfl_sync(0xffffffffu, mine, first + i * STEP)) + load_at;
+            r.k[i] = __ldcg(reinterpret_cast<const uint4 *>(at));
+            r.v[i] = __ldcg(reinterpret_cast<const uint4 *>(at + B::V_AT));
         }
-        r.seen = false;
+        const uint32_t own = __shfl_sync(0xffffffffu, mine, ct / POOL_ROWS % BLOCKS);
         if (ct < FL_KT) {
-            const uint32_t pos = tile * FL_KT + ct, row = ct % POOL_ROWS;
-            const uint8_t *at = block(head, pos);
-            r.seen = at != nullptr;
-            if (at != nullptr) {
-                if (BITS == 8) {
-                    r.ks[0] = __ldcg(reinterpret_cast<const uint32_t *>(at + B::KS_AT) + row);
-                    r.vs[0] = __ldcg(reinterpret_cast<const uint32_t *>(at + B::VS_AT) + row);
-                } else {
+            const uint32_t row = ct % POOL_ROWS;
+            const uint8_t *at = block(own);
+            r.seen = own != ~0u && tile * FL_KT + ct < p.a.prefix_len;
+            if (BITS == 8) {
+                r.ks[0] = __ldcg(reinterpret_cast<const uint32_t *>(at + B::KS_AT) + row);
+                r.vs[0] = __ldcg(reinterpret_cast<const uint32_t *>(at + B::VS_AT) + row);
+            } else {
 #pragma unroll
-                    for (uint32_t g = 0; g < B::G; ++g) {
-                        r.ks[g] = (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(at + B::KS_AT) + row * B::G + g) << 16;
-                        r.vs[g] = (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(at + B::VS_AT) + row * B::G + g) << 16;
-                    }
+                for (uint32_t g = 0; g < B::G; ++g) {
+                    r.ks[g] = (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(at + B::KS_AT) + row * B::G + g) << 16;
+                    r.vs[g] = (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(at + B::VS_AT) + row * B::G + g) << 16;
                 }
+            }
+        }
+    }
+    __device__ __forceinline__ void expand(uint32_t at, const uint4 &w) const {          // `at`: the thread's row and panel
+        if (BITS == 8) {
+            sts4(at + (store_x << 4), halves_lo(w.x), halves_hi(w.x), halves_lo(w.y), halves_hi(w.y));
+            sts4(at + ((store_x ^ 1u) << 4), halves_lo(w.z), halves_hi(w.z), halves_lo(w.w), halves_hi(w.w));
+        } else {
+            const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t lo = centroids4(x[i]), hi = centroids4(x[i] >> 16);
+                sts4(at + ((store_x ^ i) << 4), halves_lo(lo), halves_hi(lo), halves_lo(hi), halves_hi(hi));
             }
         }
     }
     __device__ __forceinline__ void put(uint32_t s_tile, uint8_t *consts, const Raw &r) const {
 #pragma unroll
-        for (uint32_t k = 0; k < PER; ++k) {
-            const uint32_t u = ct + k * FL_CONV * 32, v = u % UNITS, b = v / B::RB;
-            uint32_t row, chunk;
-            unit_place<B::RB>(v % B::RB, row, chunk);
-            const uint32_t rt = b * POOL_ROWS + row, base = s_tile + (u >= UNITS ? F::K_TILE : 0u) + rt * 128;
-            const uint32_t w[4] = {r.w[k].x, r.w[k].y, r.w[k].z, r.w[k].w};
-            if (BITS == 8) {
-                // halves 16 chunk .. + 15: two 16-byte chunks; rows of 128 codes store them in turned order in their second half, which
-                // puts the eight lanes of a store on eight different chunk places
-                const uint32_t panel = base + (chunk >> 2) * (FL_KT * 128), c0 = (chunk & 3u) * 2, x = (rt & 7u);
-                const uint32_t a0 = halves_lo(w[0]), a1 = halves_hi(w[0]), a2 = halves_lo(w[1]), a3 = halves_hi(w[1]);
-                const uint32_t b0 = halves_lo(w[2]), b1 = halves_hi(w[2]), b2 = halves_lo(w[3]), b3 = halves_hi(w[3]);
-                const bool turn = chunk & 4u;
-                sts4(panel + (((c0 + (turn ? 1u : 0u)) ^ x) << 4), turn ? b0 : a0, turn ? b1 : a1, turn ? b2 : a2, turn ? b3 : a3);
-                sts4(panel + (((c0 + (turn ? 0u : 1u)) ^ x) << 4), turn ? a0 : b0, turn ? a1 : b1, turn ? a2 : b2, turn ? a3 : b3);
-            } else {
-                const uint32_t panel = base + (chunk >> 1) * (FL_KT * 128), c0 = (chunk & 1u) * 4, x = (rt & 7u);
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const uint32_t lo = centroids4(w[i]), hi = centroids4(w[i] >> 16);
-                    sts4(panel + (((c0 + i) ^ x) << 4), halves_lo(lo), halves_hi(lo), halves_lo(hi), halves_hi(hi));
-                }
-            }
+        for (uint32_t i = 0; i < PER; ++i) {
+            const uint32_t at = s_tile + store_at + (first + i * STEP) * (POOL_ROWS * 128);
+            expand(at, r.k[i]);
+            expand(at + F::K_TILE, r.v[i]);
         }
         if (ct < FL_KT) {
             constexpr uint32_t G = B::G;
@@ -157,8 +171,8 @@ template <int HD, int BITS, int QT> struct Converter {
                 // a row of zeros: 8-bit codes are 0, and two groups have a factor each; a single group of 4-bit codes, which has neither, is
                 // given a scale below everything that counts
                 const float top = G == 1 ? v[0] : fmaxf(v[0], v[G - 1]), u = v[0] != v[0] ? v[0] : top == 0.0f ? (BITS == 4 && G == 1 ? 0x1p-100f : 1.0f) : top;
-                lv = __log2f(u);
-                iv = __fdividef(1.0f, u);
+                lv = log2_approx(u);
+                iv = rcp_approx(u);
 #pragma unroll
                 for (uint32_t g = 0; g < G; ++g) part[g] = v[g] * iv;
             }
@@ -259,9 +273,9 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
     bool ok = true;
 
     if (warp >= FL_SOFT && warp < FL_SOFT + FL_CONV) {
-        const Converter<HD, BITS, QT> cv{p, tid - FL_SOFT * 32};
+        const Converter<HD, BITS, QT> cv(p, tid - FL_SOFT * 32);
         uint32_t n = 0;                            // tiles of the CTA so far
-        typename Converter<HD, BITS, QT>::Raw ring[2];
+        typename Converter<HD, BITS, QT>::Raw now, next;
         // tiles two ahead, over the ends of segments
         Segment ahead;
         uint32_t as = 0, at = 0;
@@ -275,19 +289,21 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
                 if (more) at = ahead.first;
             }
         };
-        fetch(ring[0]);
-        fetch(ring[1]);
-        for (uint32_t s = 0; ok && segment_of(f, s, g); ++s)
-            for (uint32_t t = g.first; t < g.last; ++t, ++n) {
-                const uint32_t stage = n % STAGES;
-                if (n >= STAGES) ok = mbar_wait_warp(b_free + 8 * stage, (n / STAGES - 1) & 1u, FL_WAIT, s_abort);
-                if (!ok) break;
-                if (n & 1u) { cv.put(s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST, ring[1]); fetch(ring[1]); }
-                else { cv.put(s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST, ring[0]); fetch(ring[0]); }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(b_full + 8 * stage);
-            }
+        fetch(now);
+        fetch(next);
+        const uint32_t total = min(f.part, f.items * f.tiles - blockIdx.x * f.part);
+#pragma unroll 1
+        for (; n < total; ++n) {
+            const uint32_t stage = n % STAGES;
+            if (n >= STAGES) ok = mbar_wait_warp(b_free + 8 * stage, (n / STAGES - 1) & 1u, FL_WAIT, s_abort);
+            if (!ok) break;
+            cv.put(s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST, now);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_full + 8 * stage);
+            now = next;
+            fetch(next);
+        }
     } else if (warp == FL_WARPS - 1) {
         if (lane == 0) {
             // fp32 accumulators, fp16 operands; A and B K-major for S, B with its columns consecutive for O
@@ -413,9 +429,9 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
                         }
                         float lo, hi;
                         unpair(x[k][0], lo, hi);
-                        ta = fmaxf(ta, fmaxf(lo, hi));
+                        ta = max3(ta, lo, hi);
                         unpair(x[k][1], lo, hi);
-                        tb = fmaxf(tb, fmaxf(lo, hi));
+                        tb = max3(tb, lo, hi);
                     }
                     if (__any_sync(0xffffffffu, ta > m[2 * half] + 8.0f || tb > m[2 * half + 1] + 8.0f)) {
 #pragma unroll
