@@ -4,9 +4,11 @@
 //   numerator O_i = sum_j 2^(x_ij - m_i) codev_j, denominator l_i = sum_j 2^(x_ij - m_i) / vs_j, with the running maximum m_i of x.
 // Positions out of sight have ks = 0, log2 vs = -inf, 1 / vs = 0: no mask per element, and nothing of theirs is multiplied.
 //
-// A WARP is the unit of work.  It holds 16 query rows as operands in registers (m16n8k16, halves) and walks blocks of 16 positions, which
-// a bulk copy each brings into a ring of its own; rows are queries of one kv head, so a cached row is read once for the heads that share
-// it.  The blocks of all items (token, kv head) are one long line cut into equal parts, one per warp: ragged lengths and a single
+// A WARP is the unit of work.  It walks blocks of 16 positions, which a bulk copy each brings into a ring of its own, with 8 or 16 query
+// rows (queries of one kv head, so a cached row is read once for the heads that share it).  Positions are the ROWS of the products
+// (m16n8k16, halves): S^T = K Q^T, O^T = V^T P^T, so eight queries cost one tile where queries as rows would pad them to sixteen; scores,
+// exponentials and accumulators halve with them.  What is left is the expansion of codes to halves, 2.25 instructions a value pair.
+// The blocks of all items (token, kv head) are one long line cut into equal parts, one per warp: ragged lengths and a single
 // long sequence alike keep every warp busy to the end.  An item that lies in one part is finished there; the others leave partial
 // results, which pool_merge_kernel joins.
 #include <algorithm>
@@ -19,19 +21,25 @@ namespace k2t {
 namespace {
 
 constexpr uint32_t SP_WARPS = 4, SP_STAGES = 3, WAIT_LIMIT = 1u << 22;
-// CTAs on an SM: registers (two for rows of 128 with queries in two halves)
-template <int HD, int QT> struct SplitCtas { static constexpr uint32_t N = HD == 128 && QT == 2 ? 2 : 3; };
-template <int HD, int BITS, int QT> constexpr uint32_t split_smem() { return SP_WARPS * (SP_STAGES * PoolBlock<HD, BITS>::BYTES + QT * HD / 16 * 512); }
+// CTAs on an SM, by the registers of a kernel that spills nothing worth naming
+constexpr uint32_t split_ctas(uint32_t hd, bool two_terms, bool two_weights, uint32_t nr) { return hd == 64 || !two_terms ? (nr == 1 ? 4 : 3) : nr == 2 ? 2 : two_weights ? 3 : 4; }
+template <int HD, int BITS> constexpr uint32_t split_smem() { return SP_WARPS * SP_STAGES * PoolBlock<HD, BITS>::BYTES; }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {       // 8 x 8 halves over the warp
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 template <int WORDS> __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t *w) {
     if constexpr (WORDS == 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
     else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
     else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
 }
+__device__ __forceinline__ float lds_f32(uint32_t addr) { float v; asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr)); return v; }
 
 // The sequence of a token and the rows of it that the token sees, cut to what its table holds.
 __device__ __forceinline__ uint32_t seen_rows(const PoolAttnArgs &a, uint32_t t, int32_t &seq) {
@@ -48,11 +56,10 @@ __device__ __forceinline__ uint32_t item_blocks(const SplitArgs &p, uint32_t t) 
     return (seen_rows(p.a, t, seq) + POOL_ROWS - 1) / POOL_ROWS;
 }
 
-// One item of the line: its blocks are [begin, end) there.
+// One item of the line and the block of it that is next.
 struct Item {
-    uint64_t begin, end;
     uint32_t index, t, h, rb;          // of the prefix items: (h, rb)
-    uint32_t len;                      // positions in sight
+    uint32_t next, blocks, len;        // positions in sight: len
     const int32_t *list;               // pages, or choices among the pages of `table`
     const int32_t *table;
     bool prefix;
@@ -62,18 +69,22 @@ __device__ __forceinline__ void item_fill(const SplitArgs &p, Item &it) {
     if (it.prefix) {
         it.list = p.a.prefix_pages;
         it.len = p.a.prefix_len;
+        it.blocks = prefix_blocks(p);
         return;
     }
     int32_t seq;
     it.len = seen_rows(p.a, it.t, seq);
     it.table = p.a.pages + (size_t)max(seq, 0) * p.a.pages_stride;
-    it.list = p.a.chosen != nullptr ? p.a.chosen + ((size_t)it.t * p.a.pool.d.kv_heads + it.h) * p.a.top : it.table;
+    const bool chosen = p.a.chosen != nullptr;
+    it.list = chosen ? p.a.chosen + ((size_t)it.t * p.a.pool.d.kv_heads + it.h) * p.a.top : it.table;
+    it.blocks = chosen ? p.a.top << (p.a.pool.d.page_shift - 4) : (it.len + POOL_ROWS - 1) / POOL_ROWS;
 }
 
 // Sums of the tokens' blocks over a warp: the whole, and the place of the token that holds block `x` of them (counted per kv head and tile).
 __device__ __forceinline__ uint64_t warp_total(const SplitArgs &p, uint32_t lane) {
     if (p.a.chosen != nullptr) return (uint64_t)p.a.n_tok * (p.a.top << (p.a.pool.d.page_shift - 4));
     uint64_t sum = 0;
+#pragma unroll 4
     for (uint32_t t = lane; t < p.a.n_tok; t += 32) sum += item_blocks(p, t);
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
@@ -87,6 +98,7 @@ __device__ __forceinline__ void warp_find(const SplitArgs &p, uint64_t x, uint32
         return;
     }
     uint64_t base = 0;
+#pragma unroll 1
     for (uint32_t t0 = 0; t0 < p.a.n_tok; t0 += 32) {
         const uint32_t n = t0 + lane < p.a.n_tok ? item_blocks(p, t0 + lane) : 0;
         uint64_t upto = n;
@@ -102,60 +114,76 @@ __device__ __forceinline__ void warp_find(const SplitArgs &p, uint64_t x, uint32
         }
         base += __shfl_sync(0xffffffffu, upto, 31);
     }
-    t = p.a.n_tok; before = base; blocks = 0;            // not reached: x lies below the total
+    t = p.a.n_tok; before = base; blocks = 1;            // not reached: x lies below the total
 }
 
 // The item that holds block x of the line: prefix items first, then tokens in order, of a token its kv heads, of those their tiles.
 __device__ __forceinline__ void item_at(const SplitArgs &p, uint64_t x, uint32_t lane, Item &it) {
     const uint64_t far = prefix_line(p);
-    if (x < far) {
+    it.prefix = x < far;
+    if (it.prefix) {
         const uint32_t nb = prefix_blocks(p);
-        it.prefix = true;
         it.index = (uint32_t)(x / nb);
         it.h = it.index / p.rbp;
         it.rb = it.index % p.rbp;
         it.t = 0;
-        it.begin = (uint64_t)it.index * nb;
-        it.end = it.begin + nb;
+        it.next = (uint32_t)(x - (uint64_t)it.index * nb);
     } else {
         const uint32_t per = p.a.pool.d.kv_heads * p.rbo;
         uint32_t blocks;
         uint64_t before;
         warp_find(p, (x - far) / per, lane, it.t, before, blocks);
-        const uint32_t sub = (uint32_t)((x - far - before * per) / blocks);
-        it.prefix = false;
+        const uint64_t in = x - far - before * per;
+        const uint32_t sub = (uint32_t)(in / blocks);
         it.h = sub / p.rbo;
         it.rb = sub % p.rbo;
         it.index = it.t * per + sub;
-        it.begin = far + before * per + (uint64_t)sub * blocks;
-        it.end = it.begin + blocks;
+        it.next = (uint32_t)(in - (uint64_t)sub * blocks);
     }
     item_fill(p, it);
+}
+// The item behind this one; tokens without a block are passed over (the caller knows that there is one).
+__device__ __forceinline__ void item_after(const SplitArgs &p, Item &it) {
+    it.next = 0;
+    it.index += 1;
+    if (it.prefix) {
+        if (++it.rb == p.rbp) { it.rb = 0; it.h += 1; }
+        if (it.h < p.a.pool.d.kv_heads) return;
+        it.prefix = false;
+        it.index = it.t = it.h = it.rb = 0;
+        item_fill(p, it);
+    } else {
+        if (++it.rb == p.rbo) { it.rb = 0; it.h += 1; }
+        if (it.h == p.a.pool.d.kv_heads) { it.h = 0; it.t += 1; }
+        if (it.t < p.a.n_tok) item_fill(p, it);
+    }
+    while (it.blocks == 0 && it.t + 1 < p.a.n_tok) {
+        it.t += 1;
+        it.index += p.a.pool.d.kv_heads * p.rbo;
+        item_fill(p, it);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ the warp's rows
 // Query row i of an item: whether it exists, its token and head.
 __device__ __forceinline__ bool item_row(const SplitArgs &p, const Item &it, uint32_t i, uint32_t &t, uint32_t &head) {
-    const uint32_t group = p.a.heads / p.a.pool.d.kv_heads, r = it.rb * 16 + i;
+    const uint32_t group = p.a.heads / p.a.pool.d.kv_heads, r = it.rb * p.tile + i;
     t = it.prefix ? r / group : it.t;
     head = it.h * group + (it.prefix ? r % group : r);
     return it.prefix ? t < p.a.n_tok : r < group;
 }
 
-// Sixteen consecutive elements from / to rows.
-__device__ __forceinline__ void get16(const RowsArg &a, size_t at, float (&v)[16]) {
-    rows_get8(a, at, *reinterpret_cast<float(*)[8]>(v));
-    rows_get8(a, at + 8, *reinterpret_cast<float(*)[8]>(v + 8));
-}
-
-// Rows 'lane / 4' and that + 8: their elements [16 c, 16 c + 16) for c = t, and t + 4 where rows are 128 long; transformed, times a power
-// of two that brings the largest to 2^13 .. 2^14 (so that both terms of a row are ordinary halves), as operand fragments: word 2 k + r
-// of fragment i (and of its second term, HD / 16 further) for every lane, 16 bytes a lane.  They lie in shared memory: as 32 or 64
-// registers they left room for two CTAs on an SM where there are three now.  c: factor of the scores of the two rows, in powers of two.
-template <int HD, int QT> __device__ __forceinline__ void load_query(const SplitArgs &p, const Item &it, uint32_t lane, uint32_t *frags, float (&c)[2]) {
+// Lane (n, t) = (lane / 4, lane % 4) reads of query row n (and n + 8) the elements [16 t, 16 t + 16) of each 64; transformed, times a
+// power of two that brings the row's largest to 2^13 .. 2^14 (so that both terms of a row are ordinary halves), they are its columns of the
+// second operand: step i of a group of 64 takes words i of every lane.  c: factor of the scores of rows 2 t, 2 t + 1.
+template <int HD, int QT, int NR> struct Query {
+    uint32_t b[NR][QT][HD / 16][2];
+    float c[NR][2];
+};
+template <int HD, int QT, int NR> __device__ __forceinline__ void load_query(const SplitArgs &p, const Item &it, uint32_t lane, Query<HD, QT, NR> &q) {
     const uint32_t n = lane >> 2, t4 = lane & 3u;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int r = 0; r < NR; ++r) {
         uint32_t t, head;
         const bool live = item_row(p, it, n + 8 * r, t, head);
         float v[HD / 64][16], top = 0.0f;
@@ -163,7 +191,11 @@ template <int HD, int QT> __device__ __forceinline__ void load_query(const Split
         for (int g = 0; g < HD / 64; ++g) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[g][i] = 0.0f;
-            if (live) get16(p.a.q, t * p.a.q.token_stride + head * p.a.q.head_stride + g * 64 + t4 * 16, v[g]);
+            if (live) {
+                const size_t at = t * p.a.q.token_stride + head * p.a.q.head_stride + g * 64 + t4 * 16;
+                rows_get8(p.a.q, at, *reinterpret_cast<float(*)[8]>(v[g]));
+                rows_get8(p.a.q, at + 8, *reinterpret_cast<float(*)[8]>(v[g] + 8));
+            }
             const uint32_t signs = p.a.pool.signs[2 * g + (t4 >> 1)] >> ((t4 & 1u) * 16);
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[g][i] = __fmul_rn(flip(v[g][i], signs >> i & 1u), 0.125f);
@@ -176,157 +208,156 @@ template <int HD, int QT> __device__ __forceinline__ void load_query(const Split
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         const int e = query_exponent(top);
-        const float up = power_of_two(e);
-        c[r] = p.a.scale * LOG2E * power_of_two(-e);
+        const float up = power_of_two(e), c = p.a.scale * LOG2E * power_of_two(-e);
+        q.c[r][0] = __shfl_sync(0xffffffffu, c, 8 * t4);
+        q.c[r][1] = __shfl_sync(0xffffffffu, c, 8 * t4 + 4);
 #pragma unroll
         for (int g = 0; g < HD / 64; ++g)
 #pragma unroll
             for (int w = 0; w < 4; ++w)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    float x = v[g][4 * w + 2 * k] * up, y = v[g][4 * w + 2 * k + 1] * up;
+                    const float x = v[g][4 * w + 2 * k] * up, y = v[g][4 * w + 2 * k + 1] * up;
                     const uint32_t hi = half2_bits(x, y);
-                    frags[((4 * g + w) * 32 + lane) * 4 + r + 2 * k] = hi;
+                    q.b[r][0][4 * g + w][k] = hi;
                     if constexpr (QT == 2) {
                         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-                        frags[((HD / 16 + 4 * g + w) * 32 + lane) * 4 + r + 2 * k] = half2_bits(x - f.x, y - f.y);
+                        q.b[r][1][4 * g + w][k] = half2_bits(x - f.x, y - f.y);
                     }
                 }
     }
 }
 
-template <int HD> struct State {
-    float o[HD / 8][4], m[2], l[2];
+// o[r][j]: elements n HD / 8 + 2 j and the next, of query rows 8 r + 2 t and the next; m, l of those rows (l of the lane's positions)
+template <int HD, int NR> struct State {
+    float o[NR][HD / 16][4], m[NR][2], l[NR][2];
 };
 
 // One block of 16 positions, `valid` of them in sight, at shared address `at`.
-template <int HD, int BITS, int QT, int PT>
-__device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t lane, uint32_t frags, const float (&c)[2], State<HD> &st) {
+template <int HD, int BITS, int QT, int PT, int NR>
+__device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t lane, const Query<HD, QT, NR> &q, State<HD, NR> &st) {
     using B = PoolBlock<HD, BITS>;
     constexpr int G = B::G;
     const uint32_t n = lane >> 2, t = lane & 3u;
-    // scores of positions 4 (n / 2) + n % 2 (first tile of columns) and two further (second), per group of 64 elements
-    float s[G][2][4];
+    // Row i of the products is position 4 (i / 2) + i % 2 for the first eight, two further for the others: the lane has rows n and n + 8.
+    const uint32_t p0 = 4 * (n >> 1) + (n & 1u);
+    float s[NR][G][4];                     // rows n, n + 8 of queries 2 t, 2 t + 1, of each group of 64 elements that has a scale
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) s[g][j][0] = s[g][j][1] = s[g][j][2] = s[g][j][3] = 0.0f;
+        for (int g = 0; g < G; ++g) s[r][g][0] = s[r][g][1] = s[r][g][2] = s[r][g][3] = 0.0f;
 #pragma unroll
     for (int g = 0; g < HD / 64; ++g) {
         uint32_t w[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const uint32_t row = 4 * (n >> 1) + (n & 1u) + 2 * j;
             if (BITS == 8) {
-                lds_words<4>(at + row_place<B::RB>(row, g * 64 + t * 16), w[j]);
+                lds_words<4>(at + row_place<B::RB>(p0 + 2 * j, g * 64 + t * 16), w[j]);
             } else {
                 uint32_t x[2];
-                lds_words<2>(at + row_place<B::RB>(row, g * 32 + t * 8), x);
+                lds_words<2>(at + row_place<B::RB>(p0 + 2 * j, g * 32 + t * 8), x);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) { w[j][2 * i] = centroids4(x[i]); w[j][2 * i + 1] = centroids4(x[i] >> 16); }
             }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t a[QT][4];
+            const uint32_t a[4] = {halves_lo(w[0][i]), halves_lo(w[1][i]), halves_hi(w[0][i]), halves_hi(w[1][i])};
 #pragma unroll
-            for (int k = 0; k < QT; ++k) lds_words<4>(frags + ((k * (HD / 16) + 4 * g + i) * 32 + lane) * 16, a[k]);
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int k = 0; k < QT; ++k) mma_f16(s[r][G == 1 ? 0 : g], a, q.b[r][k][4 * g + i][0], q.b[r][k][4 * g + i][1]);
+        }
+    }
+    // constants of positions p0 and p0 + 2
+    float ks[G][2], lv[2], iv[2], part[G][2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t pos = p0 + 2 * j;
+        float v[G], top;
+        if (BITS == 8) {
+            ks[0][j] = lds_f32(at + B::KS_AT + pos * 4);
+            v[0] = lds_f32(at + B::VS_AT + pos * 4);
+        } else if (G == 2) {
+            uint32_t a, b;
+            lds_words<1>(at + B::KS_AT + pos * 4, &a);
+            lds_words<1>(at + B::VS_AT + pos * 4, &b);
+            ks[0][j] = __uint_as_float(a << 16); ks[G - 1][j] = __uint_as_float(a & 0xFFFF0000u);
+            v[0] = __uint_as_float(b << 16); v[G - 1] = __uint_as_float(b & 0xFFFF0000u);
+        } else {
+            uint32_t a, b;                     // two positions a word
+            lds_words<1>(at + B::KS_AT + (pos & ~1u) * 2, &a);
+            lds_words<1>(at + B::VS_AT + (pos & ~1u) * 2, &b);
+            ks[0][j] = __uint_as_float(pos & 1u ? a & 0xFFFF0000u : a << 16);
+            v[0] = __uint_as_float(pos & 1u ? b & 0xFFFF0000u : b << 16);
+        }
+        top = G == 1 ? v[0] : fmaxf(v[0], v[G - 1]);          // scales are not negative, and all groups of a row are NaN or none
+        if (top == 0.0f) top = 1.0f;               // a row of zeros: 8-bit codes are 0, groups of 4 bits have a factor
+        if (pos < valid) {
+            lv[j] = log2_approx(top);
+            iv[j] = rcp_approx(top);
+#pragma unroll
+            for (int g = 0; g < G; ++g) part[g][j] = v[g] * iv[j];
+        } else {
+            lv[j] = -INFINITY;
+            iv[j] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < G; ++g) ks[g][j] = part[g][j] = 0.0f;
+        }
+    }
+    float x[NR][4], top[NR][2];                // [position p0 | p0 + 2][query 2 t | 2 t + 1]
+    bool grows = false;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float d = s[r][0][e] * ks[0][e >> 1];
+            if (G == 2) d = __fmaf_rn(s[r][G - 1][e], ks[G - 1][e >> 1], d);
+            x[r][e] = __fmaf_rn(d, q.c[r][e & 1], lv[e >> 1]);
+        }
+        top[r][0] = fmaxf(x[r][0], x[r][2]);
+        top[r][1] = fmaxf(x[r][1], x[r][3]);
+        grows |= top[r][0] > st.m[r][0] + 8.0f || top[r][1] > st.m[r][1] + 8.0f;
+    }
+    // the maximum follows only where it has grown by more than 2^8: weights stay within halves, sums are exact in either case
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float y = top[r][e];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
+                const float m = fmaxf(st.m[r][e], y), al = m == -INFINITY ? 1.0f : exp2_approx(st.m[r][e] - m);
+                st.m[r][e] = m;
+                st.l[r][e] *= al;
+#pragma unroll
+                for (int j = 0; j < HD / 16; ++j) { st.o[r][j][e] *= al; st.o[r][j][2 + e] *= al; }
+            }
+    }
+    uint32_t b[NR][G][PT][2];                  // weights as the second operand: transposed, the lane's positions are 4 t .. 4 t + 3 of query n
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float m = st.m[r][e & 1] == -INFINITY ? 0.0f : st.m[r][e & 1];
+            x[r][e] = exp2_approx(x[r][e] - m);
+            st.l[r][e & 1] = __fmaf_rn(x[r][e], iv[e >> 1], st.l[r][e & 1]);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const uint32_t b0 = halves_lo(w[j][i]), b1 = halves_hi(w[j][i]);
-#pragma unroll
-                for (int k = 0; k < QT; ++k) mma_f16(s[G == 1 ? 0 : g][j], a[k], b0, b1);
+                const float u = BITS == 4 ? x[r][2 * j] * part[g][j] : x[r][2 * j], v = BITS == 4 ? x[r][2 * j + 1] * part[g][j] : x[r][2 * j + 1];
+                const uint32_t hi = half2_bits(u, v);
+                b[r][g][0][j] = transposed(hi);
+                if constexpr (PT == 2) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+                    b[r][g][PT - 1][j] = transposed(half2_bits(u - f.x, v - f.y));
+                }
             }
-        }
     }
-    // the lane's columns are positions 4 t .. 4 t + 3
-    float ks[G][4], lv[4], iv[4], part[G][4];
-    if (BITS == 8) {
-        const float4 a = lds_f32x4(at + B::KS_AT + t * 16), b = lds_f32x4(at + B::VS_AT + t * 16);
-        const float va[4] = {b.x, b.y, b.z, b.w};
-        ks[0][0] = a.x; ks[0][1] = a.y; ks[0][2] = a.z; ks[0][3] = a.w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float v = va[i] == 0.0f ? 1.0f : va[i];          // a row of zeros: its codes are 0 as well
-            lv[i] = __log2f(v);
-            iv[i] = __fdividef(1.0f, v);
-        }
-    } else {
-        uint32_t a[2 * G], b[2 * G];
-        lds_words<2 * G>(at + B::KS_AT + t * 8 * G, a);
-        lds_words<2 * G>(at + B::VS_AT + t * 8 * G, b);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v[G], top = 0.0f;                // scales are not negative, and all groups of a row are NaN or none
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-                const int e = i * G + g;
-                ks[g][i] = __uint_as_float(e & 1 ? a[e / 2] & 0xFFFF0000u : a[e / 2] << 16);
-                v[g] = __uint_as_float(e & 1 ? b[e / 2] & 0xFFFF0000u : b[e / 2] << 16);
-                top = fmaxf(top, v[g]);
-            }
-            const float u = v[0] != v[0] ? v[0] : top == 0.0f ? 1.0f : top;
-            lv[i] = __log2f(u);
-            iv[i] = __fdividef(1.0f, u);
-#pragma unroll
-            for (int g = 0; g < G; ++g) part[g][i] = v[g] * iv[i];
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (4 * t + i >= valid) {
-#pragma unroll
-            for (int g = 0; g < G; ++g) { ks[g][i] = 0.0f; part[g][i] = 0.0f; }
-            lv[i] = -INFINITY;
-            iv[i] = 0.0f;
-        }
-    float x[2][4];                     // row, position
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float d = s[0][i >> 1][2 * r + (i & 1)] * ks[0][i];
-            if (G == 2) d = __fmaf_rn(s[G - 1][i >> 1][2 * r + (i & 1)], ks[G - 1][i], d);
-            x[r][i] = __fmaf_rn(d, c[r], lv[i]);
-        }
-    const float top0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])), top1 = fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3]));
-    // the maximum follows only where it has grown by more than 2^8: weights stay within halves, sums are exact in either case
-    if (__any_sync(0xffffffffu, top0 > st.m[0] + 8.0f || top1 > st.m[1] + 8.0f)) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            float top = r == 0 ? top0 : top1;
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float m = fmaxf(st.m[r], top), al = m == -INFINITY ? 1.0f : exp2_approx(st.m[r] - m);
-            st.m[r] = m;
-            st.l[r] *= al;
-#pragma unroll
-            for (int j = 0; j < HD / 8; ++j) { st.o[j][2 * r] *= al; st.o[j][2 * r + 1] *= al; }
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const float m = st.m[r] == -INFINITY ? 0.0f : st.m[r];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[r][i] = exp2_approx(x[r][i] - m);
-            st.l[r] = __fmaf_rn(x[r][i], iv[i], st.l[r]);
-        }
-    }
-    uint32_t a[G][PT][4];
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {          // fragment word k: row k & 1, positions 2 (k / 2) and the next
-            float u = x[k & 1][k & 2], v = x[k & 1][(k & 2) + 1];
-            if (BITS == 4) { u *= part[g][k & 2]; v *= part[g][(k & 2) + 1]; }
-            a[g][0][k] = half2_bits(u, v);
-            if constexpr (PT == 2) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&a[g][0][k]));
-                a[g][1][k] = half2_bits(u - f.x, v - f.y);
-            }
-        }
-    // values of positions 4 t .. 4 t + 3; column n of tile j is element n HD / 8 + j
+    // values: columns of the first operand are positions, two of them a word; rows n and n + 8 of tile j are elements n HD / 8 + 2 j, + 1
     constexpr int W = HD / 32;                 // words of four elements
     uint32_t v[4][W];
 #pragma unroll
@@ -341,67 +372,62 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
             for (int k = 0; k < W / 2; ++k) { v[i][2 * k] = centroids4(y[k]); v[i][2 * k + 1] = centroids4(y[k] >> 16); }
         }
     }
-    // element j lies in group 0 where n HD / 8 < 64: lanes of one tile hold columns of both groups, so a tile is multiplied for each
-    // group's weights into its own half of the columns -- by lanes' values set to zero outside the group
 #pragma unroll
     for (int k = 0; k < W; ++k) {
         const uint32_t lo01 = prmt(v[0][k], v[1][k], 0x5140u), lo23 = prmt(v[2][k], v[3][k], 0x5140u), hi01 = prmt(v[0][k], v[1][k], 0x7362u), hi23 = prmt(v[2][k], v[3][k], 0x7362u);
-        const uint32_t b0[4] = {halves_lo(lo01), halves_hi(lo01), halves_lo(hi01), halves_hi(hi01)};
-        const uint32_t b1[4] = {halves_lo(lo23), halves_hi(lo23), halves_lo(hi23), halves_hi(hi23)};
+        const uint32_t first[4] = {halves_lo(lo01), halves_hi(lo01), halves_lo(lo23), halves_hi(lo23)}, second[4] = {halves_lo(hi01), halves_hi(hi01), halves_lo(hi23), halves_hi(hi23)};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const uint32_t x0 = G == 1 || (n >> 2) == (uint32_t)g ? b0[e] : 0u, x1 = G == 1 || (n >> 2) == (uint32_t)g ? b1[e] : 0u;
+                // the elements of lanes n < 4 are the first group's: each group's weights meet the other group's rows as zeros
+                uint32_t a[4];
 #pragma unroll
-                for (int y = 0; y < PT; ++y) mma_f16(st.o[4 * k + e], a[g][y], x0, x1);
+                for (int i = 0; i < 4; ++i) a[i] = G == 1 || (n >> 2) == (uint32_t)g ? (e == 0 ? first[i] : second[i]) : 0u;
+#pragma unroll
+                for (int r = 0; r < NR; ++r)
+#pragma unroll
+                    for (int y = 0; y < PT; ++y) mma_f16(st.o[r][2 * k + e], a, b[r][g][y][0], b[r][g][y][1]);
             }
     }
 }
 
-// The rows of a finished item, normalised and transformed back: the lane holds, of rows n and n + 8, elements (2 t + b) HD / 8 + j.
-template <int HD> __device__ __forceinline__ void write_rows(const SplitArgs &p, const Item &it, uint32_t lane, const State<HD> &st) {
+// A finished item's rows, normalised and transformed back.
+template <int HD, int NR> __device__ __forceinline__ void write_rows(const SplitArgs &p, const Item &it, uint32_t lane, const State<HD, NR> &st) {
     constexpr int E = HD / 8;                  // consecutive elements of a lane
-    const uint32_t n = lane >> 2, t4 = lane & 3u;
+    const uint32_t n = lane >> 2, t4 = lane & 3u, signs = p.a.pool.signs[n * E >> 5] >> (n * E & 31u);
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        uint32_t t, head;
-        const bool live = item_row(p, it, n + 8 * r, t, head);
-        const float inv = st.l[r] == 0.0f ? 0.0f : 1.0f / st.l[r];
-        float v[2 * E];
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int j = 0; j < E; ++j) { v[j] = st.o[j][2 * r] * inv; v[E + j] = st.o[j][2 * r + 1] * inv; }
-        butterflies_in(v);
-        butterflies_across(v, 1, lane);
-        if (HD == 64) butterflies_across(v, 2, lane);
-        const uint32_t at = 2 * t4 * E, signs = p.a.pool.signs[at >> 5] >> (at & 31u);
+        for (int e = 0; e < 2; ++e) {
+            uint32_t t, head;
+            const bool live = item_row(p, it, 8 * r + 2 * t4 + e, t, head);
+            const float inv = st.l[r][e] == 0.0f ? 0.0f : 1.0f / st.l[r][e];
+            float v[E];
 #pragma unroll
-        for (int i = 0; i < 2 * E; ++i) v[i] = flip(v[i] * 0.125f, signs >> i & 1u);
-        if (live)
+            for (int j = 0; j < E / 2; ++j) { v[2 * j] = st.o[r][j][e] * inv; v[2 * j + 1] = st.o[r][j][2 + e] * inv; }
+            butterflies_in(v);
 #pragma unroll
-            for (int i = 0; i < 2 * E; i += 8)
-                rows_put8(p.a.out, t * p.a.out.token_stride + head * p.a.out.head_stride + at + i, *reinterpret_cast<const float(*)[8]>(v + i));
-    }
+            for (uint32_t m = 4; m < 4 * 64 / E; m <<= 1) butterflies_across(v, m, lane);
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] = flip(v[i] * 0.125f, signs >> i & 1u);
+            if (live)
+#pragma unroll
+                for (int i = 0; i < E; i += 8)
+                    rows_put8(p.a.out, t * p.a.out.token_stride + head * p.a.out.head_stride + n * E + i, *reinterpret_cast<const float(*)[8]>(v + i));
+        }
 }
 
-// Copies of blocks into the warp's ring, ahead of the steps: the item and block to ask for next, and 32 pages of its list over the lanes.
-struct Requests {
-    Item it;
-    uint64_t x, end;           // next block of the line, end of the warp's part
-    int32_t page, first;       // the lane's page of the list and the position it begins at (of a chosen one; else unused)
-    uint32_t asked;            // blocks asked for
-};
-
-template <int HD, int BITS, int QT, int PT>
-__global__ void __launch_bounds__(SP_WARPS * 32, SplitCtas<HD, QT>::N) pool_split_kernel(const __grid_constant__ SplitArgs p) {
+template <int HD, int BITS, int QT, int PT, int NR>
+__global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2, NR)) pool_split_kernel(const __grid_constant__ SplitArgs p) {
     using B = PoolBlock<HD, BITS>;
     extern __shared__ __align__(128) uint8_t smb[];
     __shared__ __align__(8) uint64_t bars[SP_WARPS][SP_STAGES];
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, unit = blockIdx.x * SP_WARPS + warp;
-    uint32_t *frags = reinterpret_cast<uint32_t *>(smb + warp * (QT * HD / 16 * 512));
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smb) + SP_WARPS * (QT * HD / 16 * 512) + warp * SP_STAGES * B::BYTES, bar = (uint32_t)__cvta_generic_to_shared(bars[warp]);
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smb) + warp * SP_STAGES * B::BYTES, bar = (uint32_t)__cvta_generic_to_shared(bars[warp]);
     const PoolShape &d = p.a.pool.d;
-    const uint32_t bs = d.page_shift - 4;
+    const uint32_t bs = d.page_shift - 4, in_page = (1u << bs) - 1u;
+    const bool listed = p.a.chosen == nullptr;
     if (lane == 0) {
         for (uint32_t i = 0; i < SP_STAGES; ++i) mbar_init(bar + 8 * i, 1);
         fence_mbar_init();
@@ -409,117 +435,119 @@ __global__ void __launch_bounds__(SP_WARPS * 32, SplitCtas<HD, QT>::N) pool_spli
     __syncwarp();
     pdl_wait();
     pdl_trigger();
-    Requests rq;
-    rq.asked = 0;
+    Item it;
+    uint32_t left;                             // blocks of the warp's part
     if (p.direct) {             // the warp's part is one item, which may hold no block at all
         const uint32_t per = d.kv_heads * p.rbo;
         if (unit >= p.a.n_tok * per) return;
-        rq.it.prefix = false;
-        rq.it.index = unit;
-        rq.it.t = unit / per;
-        rq.it.h = unit % per / p.rbo;
-        rq.it.rb = unit % p.rbo;
-        rq.it.begin = rq.x = 0;
-        item_fill(p, rq.it);
-        rq.it.end = rq.end = p.a.chosen != nullptr ? p.a.top << bs : (rq.it.len + POOL_ROWS - 1) / POOL_ROWS;
+        it.prefix = false;
+        it.index = unit;
+        it.t = unit / per;
+        it.h = unit % per / p.rbo;
+        it.rb = unit % p.rbo;
+        it.next = 0;
+        item_fill(p, it);
+        left = it.blocks;
     } else {
-        const uint64_t all = prefix_line(p) + warp_total(p, lane) * d.kv_heads * p.rbo, per = part_blocks(all, p.units);
-        rq.x = (uint64_t)unit * per;
-        rq.end = min(all, rq.x + per);
-        if (rq.x >= rq.end) return;
-        item_at(p, rq.x, lane, rq.it);
+        const uint64_t all = prefix_line(p) + warp_total(p, lane) * d.kv_heads * p.rbo, part = part_blocks(all, p.units), x = (uint64_t)unit * part;
+        if (x >= all) return;
+        left = (uint32_t)min(part, all - x);
+        item_at(p, x, lane, it);
     }
-    Item it = rq.it;
-    const uint64_t start = rq.x, end = rq.end;
-    uint64_t x = start;
-    uint32_t held = 0, phase = 0;              // a byte per stage: positions in sight; a bit per stage: parity of its next copy
-    bool fresh = true;                         // the lanes' pages are to be read
+    Item ask = it;                             // what is asked for next, ahead of what is worked on
+    uint32_t to_ask = left, asked = 0, held = 0, phase = 0;          // a byte per stage: positions in sight; a bit per stage: parity of its next copy
+    int32_t page = 0, first = 0;               // over the lanes: 32 pages of the list, and where a chosen one begins (below 0: nothing in sight)
+    bool fresh = true;
 
     auto request = [&]() {                     // one block, into stage asked % SP_STAGES
-        if (rq.x >= rq.end) return;
-        if (rq.x >= rq.it.end) { item_at(p, rq.x, lane, rq.it); fresh = true; }
-        const uint32_t b = (uint32_t)(rq.x - rq.it.begin), entry = b >> bs;
+        if (to_ask == 0) return;
+        if (ask.next == ask.blocks) { item_after(p, ask); fresh = true; }
+        const uint32_t b = ask.next, entry = b >> bs;
         if (fresh || (b & ((32u << bs) - 1u)) == 0) {
             fresh = false;
-            const uint32_t e = (entry & ~31u) + lane, pages = (rq.it.len + (1u << d.page_shift) - 1) >> d.page_shift;
-            rq.page = -1;
-            rq.first = 0;
-            if (rq.it.prefix || p.a.chosen == nullptr) {
-                if (e < pages) rq.page = __ldcg(rq.it.list + e);
-                else rq.page = 0;
+            const uint32_t e = (entry & ~31u) + lane, pages = (ask.len + (1u << d.page_shift) - 1) >> d.page_shift;
+            page = first = 0;
+            if (listed || ask.prefix) {
+                if (e < pages) page = __ldcg(ask.list + e);
             } else {
-                const int32_t c = e < p.a.top ? __ldcg(rq.it.list + e) : -1;
-                if (c >= 0 && (uint32_t)c < pages) { rq.page = __ldcg(rq.it.table + c); rq.first = c; }
-                else { rq.page = 0; rq.first = -1; }
+                const int32_t c = e < p.a.top ? __ldcg(ask.list + e) : -1;
+                first = c >= 0 && (uint32_t)c < pages ? c : -1;
+                if (first >= 0) page = __ldcg(ask.table + c);
             }
-            if (rq.page < 0 || (uint32_t)rq.page >= d.num_pages) { pool_bad_page(p.a.pool); rq.page = 0; rq.first = -1; }
+            if (page < 0 || (uint32_t)page >= d.num_pages) { pool_bad_page(p.a.pool); page = 0; first = -1; }
         }
-        const int32_t page = __shfl_sync(0xffffffffu, rq.page, entry & 31u), first = __shfl_sync(0xffffffffu, rq.first, entry & 31u);
-        const bool listed = rq.it.prefix || p.a.chosen == nullptr;
-        const uint64_t pos = listed ? (uint64_t)b * POOL_ROWS : ((uint64_t)max(first, 0) << d.page_shift) + (uint64_t)(b & ((1u << bs) - 1u)) * POOL_ROWS;
-        const uint32_t valid = first < 0 || pos >= rq.it.len ? 0 : (uint32_t)min((uint64_t)POOL_ROWS, rq.it.len - pos), stage = rq.asked % SP_STAGES;
+        const int32_t pg = __shfl_sync(0xffffffffu, page, entry & 31u), begins = __shfl_sync(0xffffffffu, first, entry & 31u);
+        const uint32_t pos = listed || ask.prefix ? b * POOL_ROWS : ((uint32_t)max(begins, 0) << d.page_shift) + (b & in_page) * POOL_ROWS;
+        const uint32_t valid = begins < 0 || pos >= ask.len ? 0 : min(POOL_ROWS, ask.len - pos), stage = asked % SP_STAGES;
         held = (held & ~(255u << (8 * stage))) | valid << (8 * stage);
         if (valid != 0 && lane == 0) {
             mbar_expect_tx(bar + 8 * stage, B::BYTES);
-            bulk_g2s(ring + stage * B::BYTES, p.a.pool.rows + (((size_t)page * d.kv_heads + rq.it.h << bs) + (b & ((1u << bs) - 1u))) * B::BYTES, B::BYTES, bar + 8 * stage);
+            bulk_g2s(ring + stage * B::BYTES, p.a.pool.rows + ((((size_t)pg * d.kv_heads + ask.h) << bs) + (b & in_page)) * B::BYTES, B::BYTES, bar + 8 * stage);
         }
-        rq.x += 1;
-        rq.asked += 1;
+        ask.next += 1;
+        to_ask -= 1;
+        asked += 1;
     };
+#pragma unroll 1
     for (uint32_t i = 0; i < SP_STAGES; ++i) request();
-    float c[2];
-    State<HD> st;
-    auto begin = [&]() {
-        load_query<HD, QT>(p, it, lane, frags, c);
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < HD / 8; ++j) st.o[j][0] = st.o[j][1] = st.o[j][2] = st.o[j][3] = 0.0f;
-        st.m[0] = st.m[1] = -INFINITY;
-        st.l[0] = st.l[1] = 0.0f;
-    };
-    auto finish = [&]() {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 1);
-            st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 2);
-        }
-        if (p.a.prefix_len == 0 && it.begin >= start && it.end <= end) { write_rows(p, it, lane, st); return; }
-        float *slot = p.slot(it.prefix, unit, it.index);
-        const uint32_t n = lane >> 2, t4 = lane & 3u, rows = p.slot_rows(it.prefix);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const uint32_t row = n + 8 * r;
-            if (row >= rows) continue;
-            float *o = slot + row * HD + 2 * t4 * (HD / 8);
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int j = 0; j < HD / 8; j += 4)
-                    *reinterpret_cast<float4 *>(o + b * (HD / 8) + j) = make_float4(st.o[j][2 * r + b], st.o[j + 1][2 * r + b], st.o[j + 2][2 * r + b], st.o[j + 3][2 * r + b]);
-            if (t4 == 0) *reinterpret_cast<float2 *>(slot + rows * HD + 2 * row) = make_float2(st.m[r], st.l[r]);
-        }
-    };
-    begin();
+    Query<HD, QT, NR> q;
+    State<HD, NR> st;
     bool ok = true;
-    for (uint32_t i = 0; x < end; ++i, ++x) {
-        if (x >= it.end) {
-            finish();
-            item_at(p, x, lane, it);
-            begin();
+    uint32_t i = 0;
+    // items of the part
+#pragma unroll 1
+    for (;;) {
+        load_query<HD, QT, NR>(p, it, lane, q);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) st.o[r][j][0] = st.o[r][j][1] = st.o[r][j][2] = st.o[r][j][3] = 0.0f;
+            st.m[r][0] = st.m[r][1] = -INFINITY;
+            st.l[r][0] = st.l[r][1] = 0.0f;
         }
-        const uint32_t stage = i % SP_STAGES, valid = held >> (8 * stage) & 255u;
-        if (valid != 0) {
-            bool landed = mbar_try_wait(bar + 8 * stage, phase >> stage & 1u) != 0;
-            for (uint32_t spin = 0; spin < WAIT_LIMIT && !landed; ++spin) landed = mbar_try_wait(bar + 8 * stage, phase >> stage & 1u) != 0;
-            landed = __all_sync(0xffffffffu, landed);
-            ok = ok && landed;
-            phase ^= 1u << stage;
-            block_step<HD, BITS, QT, PT>(ring + stage * B::BYTES, valid, lane, (uint32_t)__cvta_generic_to_shared(frags), c, st);
+        const uint32_t here = min(left, it.blocks - it.next);
+        const bool whole = here == it.blocks;
+        left -= here;
+#pragma unroll 1
+        for (const uint32_t stop = i + here; i < stop; ++i) {
+            const uint32_t stage = i % SP_STAGES, valid = held >> (8 * stage) & 255u;
+            if (valid != 0) {
+                bool landed = mbar_try_wait(bar + 8 * stage, phase >> stage & 1u) != 0;
+                for (uint32_t spin = 0; spin < WAIT_LIMIT && !landed; ++spin) landed = mbar_try_wait(bar + 8 * stage, phase >> stage & 1u) != 0;
+                landed = __all_sync(0xffffffffu, landed);
+                ok = ok && landed;
+                phase ^= 1u << stage;
+                block_step<HD, BITS, QT, PT, NR>(ring + stage * B::BYTES, valid, lane, q, st);
+            }
+            __syncwarp();                          // all lanes are done with the stage
+            request();
         }
-        __syncwarp();                          // all lanes are done with the stage
-        request();
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) st.l[r][e] += __shfl_xor_sync(0xffffffffu, st.l[r][e], o);
+        if (whole && p.a.prefix_len == 0) {
+            write_rows(p, it, lane, st);
+        } else {
+            float *slot = p.slot(it.prefix, unit, it.index);
+            const uint32_t n = lane >> 2, t4 = lane & 3u, rows = p.slot_rows(it.prefix);
+#pragma unroll
+            for (int r = 0; r < NR; ++r)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t row = 8 * r + 2 * t4 + e;
+                    if (row >= rows) continue;
+#pragma unroll
+                    for (int j = 0; j < HD / 16; j += 2)
+                        *reinterpret_cast<float4 *>(slot + row * HD + n * (HD / 8) + 2 * j) = make_float4(st.o[r][j][e], st.o[r][j][2 + e], st.o[r][j + 1][e], st.o[r][j + 1][2 + e]);
+                    if (n == 0) *reinterpret_cast<float2 *>(slot + rows * HD + 2 * row) = make_float2(st.m[r][e], st.l[r][e]);
+                }
+        }
+        if (left == 0) break;
+        item_after(p, it);
     }
-    finish();
     if (!ok && lane == 0) atomicCAS(p.a.pool.err, 0u, 1u);
 }
 
@@ -535,7 +563,7 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
     pdl_trigger();
     // pieces of the prefix item, then of the token's own: [first, last) of the warps for each
     uint32_t near_first = 0, near_n = 0, near_item = 0, own_first = 0, own_n = 0;
-    const uint32_t own_item = (t * kh + h) * p.rbo + in / 16, r = t * group + in;
+    const uint32_t own_item = (t * kh + h) * p.rbo + in / p.tile, r = t * group + in;
     if (p.direct) {
         own_n = item_blocks(p, t) > 0 ? 1 : 0;
     } else {
@@ -558,13 +586,13 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
         }
         const uint64_t far = prefix_line(p), per = part_blocks(far + total * kh * p.rbo, p.units);
         if (far > 0 && !p.flash.on) {
-            near_item = h * p.rbp + r / 16;
+            near_item = h * p.rbp + r / p.tile;
             const uint64_t b = (uint64_t)near_item * prefix_blocks(p), e = b + prefix_blocks(p);
             near_first = (uint32_t)(b / per);
             near_n = (uint32_t)((e - 1) / per) + 1 - near_first;
         }
         if (mine > 0) {
-            const uint64_t b = far + before * kh * p.rbo + (uint64_t)(h * p.rbo + in / 16) * mine, e = b + mine;
+            const uint64_t b = far + before * kh * p.rbo + (uint64_t)(h * p.rbo + in / p.tile) * mine, e = b + mine;
             own_first = (uint32_t)(b / per);
             own_n = (uint32_t)((e - 1) / per) + 1 - own_first;
             if (own_n == 1 && p.a.prefix_len == 0) return;
@@ -586,7 +614,7 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
             rows = FLASH_ROWS;
             return p.near + (size_t)(near_first + (p.flash.halved ? i >> 1 : i) + near_item) * flash_slot_floats(HD) + second * (flash_slot_floats(HD) / 2);
         }
-        row = near ? r % 16 : in % 16;
+        row = (near ? r : in) % p.tile;
         rows = p.slot_rows(near);
         return near ? p.slot(true, near_first + i, near_item) : p.slot(false, own_first + i - near_n, own_item);
     };
@@ -656,8 +684,6 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     p.a = a;
     const PoolShape &d = a.pool.d;
     const uint32_t group = a.heads / d.kv_heads;
-    const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * ((group + 15) / 16), room = (uint64_t)a.sm_count * (d.head_dim == 128 && type != TYPE_BF16 ? SplitCtas<128, 2>::N : SplitCtas<128, 1>::N) * SP_WARPS;
-    p.rbo = (group + 15) / 16;
     const uint32_t rows = a.n_tok * group;
     p.flash.on = a.prefix_len > 0 && rows > 16;          // more than one tile of this kernel: k2t_pool_flash.cu
     if (p.flash.on) {
@@ -668,7 +694,11 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
         f.tiles = (a.prefix_len + 63) / 64;
         f.part = (uint32_t)std::max<uint64_t>(FLASH_MIN_PART, ((uint64_t)f.items * f.tiles + a.sm_count - 1) / a.sm_count);
     }
-    p.rbp = a.prefix_len == 0 || p.flash.on ? 0 : (rows + 15) / 16;
+    const bool near = a.prefix_len > 0 && !p.flash.on;
+    p.tile = group > 8 || (near && rows > 8) ? 16 : 8;
+    p.rbo = (group + p.tile - 1) / p.tile;
+    p.rbp = near ? (rows + p.tile - 1) / p.tile : 0;
+    const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * p.rbo, room = (uint64_t)a.sm_count * split_ctas(d.head_dim, type != TYPE_BF16, type == TYPE_F32, p.tile / 8) * SP_WARPS;
     p.direct = p.rbp == 0 && items >= 4 * room;
     p.units = (uint32_t)(p.direct ? items : room);
     return p;
@@ -681,16 +711,17 @@ size_t near_floats(const SplitArgs &p) {
 
 // Halves of an operand: bf16 queries and weights are rounded to one each (11 bits where bf16 has 8); fp16 queries keep two, since a score is a
 // sum of head_dim roundings (one: an output of fp16 rows 2.3 times as far from 64 bits as its own rounding); fp32 keeps two of both.
-template <int HD, int BITS, int QT, int PT> cudaError_t split_go(cudaStream_t s, const SplitArgs &p) {
-    const size_t smem = split_smem<HD, BITS, QT>();
-    const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(pool_split_kernel<HD, BITS, QT, PT>), smem);
+template <int HD, int BITS, int QT, int PT, int NR> cudaError_t split_go(cudaStream_t s, const SplitArgs &p) {
+    const size_t smem = split_smem<HD, BITS>();
+    const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(pool_split_kernel<HD, BITS, QT, PT, NR>), smem);
     if (e != cudaSuccess) return e;
-    return launch_kernel(pool_split_kernel<HD, BITS, QT, PT>, dim3((p.units + SP_WARPS - 1) / SP_WARPS), dim3(SP_WARPS * 32), smem, s, true, p);
+    return launch_kernel(pool_split_kernel<HD, BITS, QT, PT, NR>, dim3((p.units + SP_WARPS - 1) / SP_WARPS), dim3(SP_WARPS * 32), smem, s, true, p);
 }
-template <int HD, int BITS> cudaError_t split_launch(cudaStream_t s, const SplitArgs &p) {
+template <int HD, int BITS, int NR> cudaError_t split_type(cudaStream_t s, const SplitArgs &p) {
     const uint32_t type = p.a.q.type;
-    return type == TYPE_F32 ? split_go<HD, BITS, 2, 2>(s, p) : type == TYPE_F16 ? split_go<HD, BITS, 2, 1>(s, p) : split_go<HD, BITS, 1, 1>(s, p);
+    return type == TYPE_F32 ? split_go<HD, BITS, 2, 2, NR>(s, p) : type == TYPE_F16 ? split_go<HD, BITS, 2, 1, NR>(s, p) : split_go<HD, BITS, 1, 1, NR>(s, p);
 }
+template <int HD, int BITS> cudaError_t split_launch(cudaStream_t s, const SplitArgs &p) { return p.tile == 8 ? split_type<HD, BITS, 1>(s, p) : split_type<HD, BITS, 2>(s, p); }
 
 }  // namespace
 

@@ -17,13 +17,13 @@ __host__ __device__ constexpr uint32_t flash_slot_floats(uint32_t head_dim) { re
 // A partial result: rows x head_dim numerators, then (maximum, denominator) of each row.
 struct SplitArgs {
     PoolAttnArgs a;
-    uint32_t rbo, rbp;           // tiles of 16 rows of a token's item; of a prefix item (0: the line holds no prefix)
+    uint32_t tile, rbo, rbp;     // query rows of a warp, 8 or 16; tiles of a token and kv head; of the prefix (0: the line holds none)
     uint32_t units;              // warps
     bool direct;                 // every warp has one item
     float *own, *near;           // partial results of own rows; of the prefix
     FlashArgs flash;
 
-    __host__ __device__ uint32_t slot_rows(bool prefix) const { const uint32_t g = a.heads / a.pool.d.kv_heads; return prefix || g > 16 ? 16 : g; }
+    __host__ __device__ uint32_t slot_rows(bool prefix) const { const uint32_t g = a.heads / a.pool.d.kv_heads; return prefix || g > tile ? tile : g; }
     __host__ __device__ uint32_t slot_floats(bool prefix) const { return (slot_rows(prefix) * (a.pool.d.head_dim + 2) + 3u) & ~3u; }       // 16-byte boundaries
     // warps and items both ascend along the line, so their sum numbers the pieces
     __host__ __device__ float *slot(bool prefix, uint32_t unit, uint32_t item) const {
