@@ -25,23 +25,6 @@ template <int LANES> __device__ __forceinline__ bool any_over(bool b, uint32_t l
     return (__ballot_sync(0xffffffffu, b) >> (lane & ~(uint32_t)(LANES - 1)) & ((1u << LANES) - 1u)) != 0;
 }
 
-// Eight lanes hold 64 values, eight each; (1/8) H64 D x, butterflies in the order 1, 2, .. 32.
-__device__ __forceinline__ void transform8(float (&v)[8], uint32_t signs, uint32_t lane) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(flip(v[i], signs >> i & 1u), 0.125f);
-    butterflies_in(v);
-#pragma unroll
-    for (uint32_t m = 1; m < 8; m <<= 1) butterflies_across(v, m, lane);
-}
-__device__ __forceinline__ void transform8_back(float (&v)[8], uint32_t signs, uint32_t lane) {
-    butterflies_in(v);
-#pragma unroll
-    for (uint32_t m = 1; m < 8; m <<= 1) butterflies_across(v, m, lane);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = flip(__fmul_rn(v[i], 0.125f), signs >> i & 1u);
-}
-__device__ __forceinline__ uint32_t signs8(const PoolView &p, uint32_t at) { return p.signs[at >> 5] >> (at & 31u) & 0xFFu; }
-
 // A row over LANES lanes, eight values each, as 8-bit codes: what all quantised rows of 8 bits share.  `scale` is NaN for a row that is
 // not finite (its codes are 0).
 template <int LANES> __device__ __forceinline__ void quantise8(const float (&v)[8], uint32_t lane, int (&code)[8], float &scale) {

@@ -104,16 +104,30 @@ template <int N> __device__ __forceinline__ void butterflies_in(float (&v)[N]) {
                 v[i + h] = __fsub_rn(a, b);
             }
 }
-// The same between lanes l and l ^ m, all N elements.
+// The same between lanes l and l ^ m, all N elements: the other's value plus or minus one's own, rounded once.
 template <int N> __device__ __forceinline__ void butterflies_across(float (&v)[N], uint32_t m, uint32_t lane) {
-    const bool upper = (lane & m) != 0;
+    const float sign = (lane & m) != 0 ? -1.0f : 1.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float o = __shfl_xor_sync(0xffffffffu, v[i], m);
-        v[i] = upper ? __fsub_rn(o, v[i]) : __fadd_rn(v[i], o);
-    }
+    for (int i = 0; i < N; ++i) v[i] = __fmaf_rn(v[i], sign, __shfl_xor_sync(0xffffffffu, v[i], m));
 }
-__device__ __forceinline__ float flip(float x, uint32_t bit) { return __uint_as_float(__float_as_uint(x) ^ (bit << 31)); }
+__device__ __forceinline__ float flip(float x, uint32_t signs, int i) { return __uint_as_float(__float_as_uint(x) ^ (signs << (31 - i) & 0x80000000u)); }         // by bit i
+
+// Eight lanes hold 64 values, eight each; (1/8) H64 D x, butterflies in the order 1, 2, .. 32.
+__device__ __forceinline__ void transform8(float (&v)[8], uint32_t signs, uint32_t lane) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(flip(v[i], signs, i), 0.125f);
+    butterflies_in(v);
+#pragma unroll
+    for (uint32_t m = 1; m < 8; m <<= 1) butterflies_across(v, m, lane);
+}
+__device__ __forceinline__ void transform8_back(float (&v)[8], uint32_t signs, uint32_t lane) {
+    butterflies_in(v);
+#pragma unroll
+    for (uint32_t m = 1; m < 8; m <<= 1) butterflies_across(v, m, lane);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = flip(__fmul_rn(v[i], 0.125f), signs, i);
+}
+__device__ __forceinline__ uint32_t signs8(const PoolView &p, uint32_t at) { return p.signs[at >> 5] >> (at & 31u) & 0xFFu; }
 
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 

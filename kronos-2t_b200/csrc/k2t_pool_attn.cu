@@ -4,12 +4,12 @@
 //   numerator O_i = sum_j 2^(x_ij - m_i) codev_j, denominator l_i = sum_j 2^(x_ij - m_i) / vs_j, with the running maximum m_i of x.
 // Positions out of sight have ks = 0, log2 vs = -inf, 1 / vs = 0: no mask per element, and nothing of theirs is multiplied.
 //
-// A WARP is the unit of work.  It walks blocks of 16 positions, which a bulk copy each brings into a ring of its own, with 8 or 16 query
-// rows (queries of one kv head, so a cached row is read once for the heads that share it).  Positions are the ROWS of the products
+// A CTA works with 8 or 16 query rows (queries of one kv head, so a cached row is read once for the heads that share it).  Its four warps
+// take every fourth block of 16 positions, which bulk copies bring into a ring of each warp's own, and join their results at the end of an item.  Positions are the ROWS of the products
 // (m16n8k16, halves): S^T = K Q^T, O^T = V^T P^T, so eight queries cost one tile where queries as rows would pad them to sixteen; scores,
 // exponentials and accumulators halve with them.  What is left is the expansion of codes to halves, 2.25 instructions a value pair.
-// The blocks of all items (token, kv head) are one long line cut into equal parts, one per warp: ragged lengths and a single
-// long sequence alike keep every warp busy to the end.  An item that lies in one part is finished there; the others leave partial
+// The blocks of all items (token, kv head) are one long line cut into equal parts, one per CTA: ragged lengths and a single
+// long sequence alike keep every CTA busy to the end.  An item that lies in one part is finished there; the others leave partial
 // results, which pool_merge_kernel joins.
 #include <algorithm>
 
@@ -20,10 +20,15 @@
 namespace k2t {
 namespace {
 
-constexpr uint32_t SP_WARPS = 4, SP_STAGES = 3, WAIT_LIMIT = 1u << 22;
+constexpr uint32_t SP_WARPS = 4, SP_STAGES = 2, WAIT_LIMIT = 1u << 22;
 // CTAs on an SM, by the registers of a kernel that spills nothing worth naming
 constexpr uint32_t split_ctas(uint32_t hd, bool two_terms, bool two_weights, uint32_t nr) { return hd == 64 || !two_terms ? (nr == 1 ? 4 : 3) : nr == 2 ? 2 : two_weights ? 3 : 4; }
-template <int HD, int BITS> constexpr uint32_t split_smem() { return SP_WARPS * SP_STAGES * PoolBlock<HD, BITS>::BYTES; }
+// Shared memory: the warps' rings, the queries as halves, and the warps' results of eight rows (rows HD + 4 floats apart, so that lanes of
+// neighbouring rows meet in other banks).
+template <int HD, int BITS, int QT, int NR> struct SplitSmem {
+    static constexpr uint32_t PITCH = HD + 4, QUERY = SP_WARPS * SP_STAGES * PoolBlock<HD, BITS>::BYTES, JOIN = QUERY + NR * QT * 8 * HD * 2,
+                              ML = JOIN + SP_WARPS * 8 * PITCH * 4, FACTOR = ML + SP_WARPS * 8 * 8, BYTES = FACTOR + NR * 8 * 4;
+};
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -173,57 +178,61 @@ __device__ __forceinline__ bool item_row(const SplitArgs &p, const Item &it, uin
     return it.prefix ? t < p.a.n_tok : r < group;
 }
 
-// Lane (n, t) = (lane / 4, lane % 4) reads of query row n (and n + 8) the elements [16 t, 16 t + 16) of each 64; transformed, times a
-// power of two that brings the row's largest to 2^13 .. 2^14 (so that both terms of a row are ordinary halves), they are its columns of the
-// second operand: step i of a group of 64 takes words i of every lane.  c: factor of the scores of rows 2 t, 2 t + 1.
+// The tile's rows, HD / 8 lanes each: transformed, times a power of two that brings the row's largest to 2^13 .. 2^14 (so that both terms of a
+// row are ordinary halves), to shared memory: [row][term][element], the 16-byte chunks of a row turned by its number; and their factors.
+template <int HD, int QT, int NR> __device__ __forceinline__ void put_queries(const SplitArgs &p, const Item &it, uint32_t tid, uint8_t *s_query, float *s_factor) {
+    constexpr uint32_t LANES = HD / 8;
+    const uint32_t lane = tid & 31u, l = tid % LANES, signs = p.a.pool.signs[l / 4] >> (l % 4 * 8);
+#pragma unroll
+    for (uint32_t row0 = 0; row0 < 8 * NR; row0 += SP_WARPS * 32 / LANES) {
+        const uint32_t row = row0 + tid / LANES;
+        if (row0 + (tid & ~31u) / LANES >= 8 * NR) break;          // whole warps
+        uint32_t t, head;
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, top = 0.0f;
+        if (item_row(p, it, row, t, head)) rows_get8(p.a.q, t * p.a.q.token_stride + head * p.a.q.head_stride + l * 8, v);
+        transform8(v, signs, lane);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+#pragma unroll
+        for (uint32_t m = LANES / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+        const int e = query_exponent(top);
+        const float up = power_of_two(e);
+        if (l == 0) s_factor[row] = p.a.scale * LOG2E * power_of_two(-e);
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = v[2 * i] * up, y = v[2 * i + 1] * up;
+            hi[i] = half2_bits(x, y);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
+            lo[i] = half2_bits(x - f.x, y - f.y);
+        }
+        uint4 *to = reinterpret_cast<uint4 *>(s_query + row * QT * HD * 2) + (l ^ (row & 7u));
+        to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (QT == 2) to[HD / 8] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+}
+// Lane (n, t) = (lane / 4, lane % 4) takes of query row n (and n + 8) the elements [16 t, 16 t + 16) of each 64 as its columns of the second
+// operand: step i of a group of 64 is elements 4 i .. 4 i + 3 of every lane.  c: factor of the scores of rows 2 t, 2 t + 1.
 template <int HD, int QT, int NR> struct Query {
     uint32_t b[NR][QT][HD / 16][2];
     float c[NR][2];
 };
-template <int HD, int QT, int NR> __device__ __forceinline__ void load_query(const SplitArgs &p, const Item &it, uint32_t lane, Query<HD, QT, NR> &q) {
+template <int HD, int QT, int NR> __device__ __forceinline__ void get_queries(uint32_t s_query, uint32_t s_factor, uint32_t lane, Query<HD, QT, NR> &q) {
     const uint32_t n = lane >> 2, t4 = lane & 3u;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
-        uint32_t t, head;
-        const bool live = item_row(p, it, n + 8 * r, t, head);
-        float v[HD / 64][16], top = 0.0f;
+        q.c[r][0] = lds_f32(s_factor + (8 * r + 2 * t4) * 4);
+        q.c[r][1] = lds_f32(s_factor + (8 * r + 2 * t4 + 1) * 4);
 #pragma unroll
-        for (int g = 0; g < HD / 64; ++g) {
+        for (int k = 0; k < QT; ++k)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[g][i] = 0.0f;
-            if (live) {
-                const size_t at = t * p.a.q.token_stride + head * p.a.q.head_stride + g * 64 + t4 * 16;
-                rows_get8(p.a.q, at, *reinterpret_cast<float(*)[8]>(v[g]));
-                rows_get8(p.a.q, at + 8, *reinterpret_cast<float(*)[8]>(v[g] + 8));
-            }
-            const uint32_t signs = p.a.pool.signs[2 * g + (t4 >> 1)] >> ((t4 & 1u) * 16);
+            for (int g = 0; g < HD / 64; ++g)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[g][i] = __fmul_rn(flip(v[g][i], signs >> i & 1u), 0.125f);
-            butterflies_in(v[g]);
-            butterflies_across(v[g], 1, lane);
-            butterflies_across(v[g], 2, lane);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(v[g][i]));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = query_exponent(top);
-        const float up = power_of_two(e), c = p.a.scale * LOG2E * power_of_two(-e);
-        q.c[r][0] = __shfl_sync(0xffffffffu, c, 8 * t4);
-        q.c[r][1] = __shfl_sync(0xffffffffu, c, 8 * t4 + 4);
-#pragma unroll
-        for (int g = 0; g < HD / 64; ++g)
-#pragma unroll
-            for (int w = 0; w < 4; ++w)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float x = v[g][4 * w + 2 * k] * up, y = v[g][4 * w + 2 * k + 1] * up;
-                    const uint32_t hi = half2_bits(x, y);
-                    q.b[r][0][4 * g + w][k] = hi;
-                    if constexpr (QT == 2) {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-                        q.b[r][1][4 * g + w][k] = half2_bits(x - f.x, y - f.y);
-                    }
+                for (int x = 0; x < 2; ++x) {
+                    uint32_t w[4];
+                    lds_words<4>(s_query + ((n + 8 * r) * QT + k) * HD * 2 + (((g * 8 + t4 * 2 + x) ^ n) << 4), w);
+                    q.b[r][k][4 * g + 2 * x][0] = w[0]; q.b[r][k][4 * g + 2 * x][1] = w[1];
+                    q.b[r][k][4 * g + 2 * x + 1][0] = w[2]; q.b[r][k][4 * g + 2 * x + 1][1] = w[3];
                 }
     }
 }
@@ -392,39 +401,14 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
     }
 }
 
-// A finished item's rows, normalised and transformed back.
-template <int HD, int NR> __device__ __forceinline__ void write_rows(const SplitArgs &p, const Item &it, uint32_t lane, const State<HD, NR> &st) {
-    constexpr int E = HD / 8;                  // consecutive elements of a lane
-    const uint32_t n = lane >> 2, t4 = lane & 3u, signs = p.a.pool.signs[n * E >> 5] >> (n * E & 31u);
-#pragma unroll
-    for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            uint32_t t, head;
-            const bool live = item_row(p, it, 8 * r + 2 * t4 + e, t, head);
-            const float inv = st.l[r][e] == 0.0f ? 0.0f : 1.0f / st.l[r][e];
-            float v[E];
-#pragma unroll
-            for (int j = 0; j < E / 2; ++j) { v[2 * j] = st.o[r][j][e] * inv; v[2 * j + 1] = st.o[r][j][2 + e] * inv; }
-            butterflies_in(v);
-#pragma unroll
-            for (uint32_t m = 4; m < 4 * 64 / E; m <<= 1) butterflies_across(v, m, lane);
-#pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = flip(v[i] * 0.125f, signs >> i & 1u);
-            if (live)
-#pragma unroll
-                for (int i = 0; i < E; i += 8)
-                    rows_put8(p.a.out, t * p.a.out.token_stride + head * p.a.out.head_stride + n * E + i, *reinterpret_cast<const float(*)[8]>(v + i));
-        }
-}
-
 template <int HD, int BITS, int QT, int PT, int NR>
 __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2, NR)) pool_split_kernel(const __grid_constant__ SplitArgs p) {
     using B = PoolBlock<HD, BITS>;
+    using S = SplitSmem<HD, BITS, QT, NR>;
     extern __shared__ __align__(128) uint8_t smb[];
     __shared__ __align__(8) uint64_t bars[SP_WARPS][SP_STAGES];
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, unit = blockIdx.x * SP_WARPS + warp;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smb) + warp * SP_STAGES * B::BYTES, bar = (uint32_t)__cvta_generic_to_shared(bars[warp]);
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, unit = blockIdx.x;
+    const uint32_t sbase = (uint32_t)__cvta_generic_to_shared(smb), ring = sbase + warp * SP_STAGES * B::BYTES, bar = (uint32_t)__cvta_generic_to_shared(bars[warp]);
     const PoolShape &d = p.a.pool.d;
     const uint32_t bs = d.page_shift - 4, in_page = (1u << bs) - 1u;
     const bool listed = p.a.chosen == nullptr;
@@ -436,10 +420,9 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2
     pdl_wait();
     pdl_trigger();
     Item it;
-    uint32_t left;                             // blocks of the warp's part
-    if (p.direct) {             // the warp's part is one item, which may hold no block at all
+    uint32_t left;                             // blocks of the CTA's part
+    if (p.direct) {             // the part is one item, which may hold no block at all
         const uint32_t per = d.kv_heads * p.rbo;
-        if (unit >= p.a.n_tok * per) return;
         it.prefix = false;
         it.index = unit;
         it.t = unit / per;
@@ -454,17 +437,26 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2
         left = (uint32_t)min(part, all - x);
         item_at(p, x, lane, it);
     }
-    Item ask = it;                             // what is asked for next, ahead of what is worked on
-    uint32_t to_ask = left, asked = 0, held = 0, phase = 0;          // a byte per stage: positions in sight; a bit per stage: parity of its next copy
+    // What the warp asks for next: block ask.next of an item, every fourth up to ask_end; ask_left blocks of the part lie behind that item.
+    Item ask = it;
+    uint32_t ask_end = it.next + min(left, it.blocks - it.next), ask_left = left - (ask_end - it.next);
+    ask.next += warp;
+    uint32_t asked = 0, held = 0, phase = 0;          // a byte per stage: positions in sight; a bit per stage: parity of its next copy
     int32_t page = 0, first = 0;               // over the lanes: 32 pages of the list, and where a chosen one begins (below 0: nothing in sight)
-    bool fresh = true;
+    uint32_t pages_at = ~0u;                   // which 32
 
     auto request = [&]() {                     // one block, into stage asked % SP_STAGES
-        if (to_ask == 0) return;
-        if (ask.next == ask.blocks) { item_after(p, ask); fresh = true; }
+        while (ask.next >= ask_end) {
+            if (ask_left == 0) return;
+            item_after(p, ask);
+            ask_end = min(ask_left, ask.blocks);
+            ask_left -= ask_end;
+            ask.next = warp;
+            pages_at = ~0u;
+        }
         const uint32_t b = ask.next, entry = b >> bs;
-        if (fresh || (b & ((32u << bs) - 1u)) == 0) {
-            fresh = false;
+        if (pages_at != entry >> 5) {
+            pages_at = entry >> 5;
             const uint32_t e = (entry & ~31u) + lane, pages = (ask.len + (1u << d.page_shift) - 1) >> d.page_shift;
             page = first = 0;
             if (listed || ask.prefix) {
@@ -484,12 +476,13 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2
             mbar_expect_tx(bar + 8 * stage, B::BYTES);
             bulk_g2s(ring + stage * B::BYTES, p.a.pool.rows + ((((size_t)pg * d.kv_heads + ask.h) << bs) + (b & in_page)) * B::BYTES, B::BYTES, bar + 8 * stage);
         }
-        ask.next += 1;
-        to_ask -= 1;
+        ask.next += SP_WARPS;
         asked += 1;
     };
 #pragma unroll 1
     for (uint32_t i = 0; i < SP_STAGES; ++i) request();
+    float *s_factor = reinterpret_cast<float *>(smb + S::FACTOR), *s_join = reinterpret_cast<float *>(smb + S::JOIN);
+    float2 *s_ml = reinterpret_cast<float2 *>(smb + S::ML);
     Query<HD, QT, NR> q;
     State<HD, NR> st;
     bool ok = true;
@@ -497,7 +490,9 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2
     // items of the part
 #pragma unroll 1
     for (;;) {
-        load_query<HD, QT, NR>(p, it, lane, q);
+        put_queries<HD, QT, NR>(p, it, tid, smb + S::QUERY, s_factor);
+        __syncthreads();
+        get_queries<HD, QT, NR>(sbase + S::QUERY, sbase + S::FACTOR, lane, q);
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
 #pragma unroll
@@ -509,7 +504,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2
         const bool whole = here == it.blocks;
         left -= here;
 #pragma unroll 1
-        for (const uint32_t stop = i + here; i < stop; ++i) {
+        for (uint32_t b = warp; b < here; b += SP_WARPS, ++i) {
             const uint32_t stage = i % SP_STAGES, valid = held >> (8 * stage) & 255u;
             if (valid != 0) {
                 bool landed = mbar_try_wait(bar + 8 * stage, phase >> stage & 1u) != 0;
@@ -522,28 +517,51 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2
             __syncwarp();                          // all lanes are done with the stage
             request();
         }
+        // the four warps' results, eight rows at a time; then HD / 8 threads have a row
+        const uint32_t n = lane >> 2, t4 = lane & 3u, row = tid / (HD / 8), l = tid % (HD / 8);
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+        for (int r = 0; r < NR; ++r) {
+            if (r > 0) __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) st.l[r][e] += __shfl_xor_sync(0xffffffffu, st.l[r][e], o);
-        if (whole && p.a.prefix_len == 0) {
-            write_rows(p, it, lane, st);
-        } else {
-            float *slot = p.slot(it.prefix, unit, it.index);
-            const uint32_t n = lane >> 2, t4 = lane & 3u, rows = p.slot_rows(it.prefix);
+                float *to = s_join + (warp * 8 + 2 * t4 + e) * S::PITCH + n * (HD / 8);
 #pragma unroll
-            for (int r = 0; r < NR; ++r)
+                for (int j = 0; j < HD / 16; j += 2) *reinterpret_cast<float4 *>(to + 2 * j) = make_float4(st.o[r][j][e], st.o[r][j][2 + e], st.o[r][j + 1][e], st.o[r][j + 1][2 + e]);
+                if (n == 0) s_ml[warp * 8 + 2 * t4 + e] = make_float2(st.m[r][e], st.l[r][e]);
+            }
+            __syncthreads();
+            if (row < 8) {                     // whole warps
+                float m = -INFINITY, sum = 0.0f, v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t row = 8 * r + 2 * t4 + e;
-                    if (row >= rows) continue;
+                for (int w = 0; w < (int)SP_WARPS; ++w) m = fmaxf(m, s_ml[w * 8 + row].x);
+                const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-                    for (int j = 0; j < HD / 16; j += 2)
-                        *reinterpret_cast<float4 *>(slot + row * HD + n * (HD / 8) + 2 * j) = make_float4(st.o[r][j][e], st.o[r][j][2 + e], st.o[r][j + 1][e], st.o[r][j + 1][2 + e]);
-                    if (n == 0) *reinterpret_cast<float2 *>(slot + rows * HD + 2 * row) = make_float2(st.m[r][e], st.l[r][e]);
+                for (int w = 0; w < (int)SP_WARPS; ++w) {
+                    const float2 ml = s_ml[w * 8 + row];
+                    const float f = exp2_approx(ml.x - base);
+                    const float4 *from = reinterpret_cast<const float4 *>(s_join + (w * 8 + row) * S::PITCH + l * 8);
+                    const float4 a = from[0], c = from[1];
+                    sum = __fmaf_rn(f, ml.y, sum);
+                    v[0] = __fmaf_rn(f, a.x, v[0]); v[1] = __fmaf_rn(f, a.y, v[1]); v[2] = __fmaf_rn(f, a.z, v[2]); v[3] = __fmaf_rn(f, a.w, v[3]);
+                    v[4] = __fmaf_rn(f, c.x, v[4]); v[5] = __fmaf_rn(f, c.y, v[5]); v[6] = __fmaf_rn(f, c.z, v[6]); v[7] = __fmaf_rn(f, c.w, v[7]);
                 }
+                if (whole && p.a.prefix_len == 0) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] *= inv;
+                    transform8_back(v, p.a.pool.signs[l / 4] >> (l % 4 * 8), lane);
+                    uint32_t t, head;
+                    if (item_row(p, it, 8 * r + row, t, head)) rows_put8(p.a.out, t * p.a.out.token_stride + head * p.a.out.head_stride + l * 8, v);
+                } else if (8 * r + row < p.slot_rows(it.prefix)) {
+                    const uint32_t rows = p.slot_rows(it.prefix);
+                    float *slot = p.slot(it.prefix, unit, it.index), *o = slot + (8 * r + row) * HD + l * 8;
+                    reinterpret_cast<float4 *>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    reinterpret_cast<float4 *>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+                    if (l == 0) *reinterpret_cast<float2 *>(slot + rows * HD + 2 * (8 * r + row)) = make_float2(m, sum);
+                }
+            }
         }
         if (left == 0) break;
         item_after(p, it);
@@ -552,40 +570,49 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2
 }
 
 // ------------------------------------------------------------------------------------------------ partial results
-// CTA = (token, head).  out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, transformed back.  Items that one warp finished are left alone.
-constexpr uint32_t MERGE_WARPS = 4;
-template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge_kernel(const __grid_constant__ SplitArgs p) {
+// `ways` warps (1 .. 8) share a row (token, head): out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, transformed back.  Items that one CTA
+// finished are left alone.
+constexpr uint32_t MERGE_WARPS = 8;
+template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge_kernel(const __grid_constant__ SplitArgs p, uint32_t ways) {
     constexpr int E = HD / 32;
     __shared__ float s_o[MERGE_WARPS][HD], s_l[MERGE_WARPS];
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kh = p.a.pool.d.kv_heads, group = p.a.heads / kh;
-    const uint32_t t = blockIdx.x / p.a.heads, head = blockIdx.x % p.a.heads, h = head / group, in = head % group;
+    __shared__ uint64_t s_sum[MERGE_WARPS][2];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kh = p.a.pool.d.kv_heads, group = p.a.heads / kh, rows_here = MERGE_WARPS / ways;
+    const uint32_t all_rows = p.a.n_tok * p.a.heads, row0 = blockIdx.x * rows_here, id = min(all_rows - 1, row0 + warp / ways);
+    const uint32_t t0 = row0 / p.a.heads, t = id / p.a.heads, head = id % p.a.heads, h = head / group, in = head % group;
     pdl_wait();
     pdl_trigger();
-    // pieces of the prefix item, then of the token's own: [first, last) of the warps for each
+    // pieces of the prefix item, then of the token's own: [first, first + n) of the CTAs for each
     uint32_t near_first = 0, near_n = 0, near_item = 0, own_first = 0, own_n = 0;
     const uint32_t own_item = (t * kh + h) * p.rbo + in / p.tile, r = t * group + in;
+    const uint64_t mine = item_blocks(p, t);
     if (p.direct) {
-        own_n = item_blocks(p, t) > 0 ? 1 : 0;
+        own_n = mine > 0 ? 1 : 0;
     } else {
-        uint64_t total = 0, before = 0;
-        const uint64_t mine = item_blocks(p, t);
+        uint64_t total, before;
         if (p.a.chosen != nullptr) {
             total = p.a.n_tok * mine;
             before = t * mine;
-        } else {
-            for (uint32_t k = lane; k < p.a.n_tok; k += 32) {
+        } else {                               // the CTA sums up to its first token, a warp the few up to its own
+            uint64_t sum[2] = {0, 0};
+            for (uint32_t k = threadIdx.x; k < p.a.n_tok; k += MERGE_WARPS * 32) {
                 const uint32_t n = item_blocks(p, k);
-                total += n;
-                before += k < t ? n : 0;
+                sum[0] += n;
+                sum[1] += k < t0 ? n : 0;
             }
 #pragma unroll
             for (int m = 16; m > 0; m >>= 1) {
-                total += __shfl_xor_sync(0xffffffffu, total, m);
-                before += __shfl_xor_sync(0xffffffffu, before, m);
+                sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], m);
+                sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], m);
             }
+            if (lane == 0) { s_sum[warp][0] = sum[0]; s_sum[warp][1] = sum[1]; }
+            __syncthreads();
+            total = before = 0;
+            for (uint32_t k = 0; k < MERGE_WARPS; ++k) { total += s_sum[k][0]; before += s_sum[k][1]; }
+            for (uint32_t k = t0; k < t; ++k) before += item_blocks(p, k);
         }
         const uint64_t far = prefix_line(p), per = part_blocks(far + total * kh * p.rbo, p.units);
-        if (far > 0 && !p.flash.on) {
+        if (far > 0) {
             near_item = h * p.rbp + r / p.tile;
             const uint64_t b = (uint64_t)near_item * prefix_blocks(p), e = b + prefix_blocks(p);
             near_first = (uint32_t)(b / per);
@@ -595,7 +622,6 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
             const uint64_t b = far + before * kh * p.rbo + (uint64_t)(h * p.rbo + in / p.tile) * mine, e = b + mine;
             own_first = (uint32_t)(b / per);
             own_n = (uint32_t)((e - 1) / per) + 1 - own_first;
-            if (own_n == 1 && p.a.prefix_len == 0) return;
         }
     }
     if (p.flash.on) {
@@ -605,7 +631,8 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
         near_first = b / f.part;
         near_n = ((e - 1) / f.part + 1 - near_first) << (f.halved ? 1 : 0);
     }
-    const uint32_t n = near_n + own_n;
+    const bool finished = own_n == 1 && p.a.prefix_len == 0;
+    const uint32_t n = finished ? 0 : near_n + own_n;
     auto slot = [&](uint32_t i, uint32_t &row, uint32_t &rows) -> const float * {
         const bool near = i < near_n;
         if (near && p.flash.on) {             // two tiles of rows, or two streams over the same rows
@@ -631,7 +658,7 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = 0.0f;
 #pragma unroll 4
-    for (uint32_t i = warp; i < n; i += MERGE_WARPS) {
+    for (uint32_t i = warp % ways; i < n; i += ways) {
         uint32_t row, rows;
         const float *s = slot(i, row, rows);
         const float2 ml = __ldcg(reinterpret_cast<const float2 *>(s + rows * HD) + row);
@@ -652,32 +679,24 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
     for (int k = 0; k < E; ++k) s_o[warp][lane * E + k] = o[k];
     if (lane == 0) s_l[warp] = l;
     __syncthreads();
-    if (warp != 0) return;
-    float v[8];
-    if (lane >= HD / 8) return;
-    l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    if (warp % ways != 0 || finished || row0 + warp / ways >= all_rows) return;
+    l = 0.0f;
+    const uint32_t c = lane % (HD / 8);        // eight elements a lane, every HD / 8 lanes alike
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (uint32_t w = warp; w < warp + ways; ++w) {
+        l += s_l[w];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += s_o[w][c * 8 + i];
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = ((s_o[0][lane * 8 + i] + s_o[1][lane * 8 + i]) + (s_o[2][lane * 8 + i] + s_o[3][lane * 8 + i])) * inv;
-    butterflies_in(v);
-    constexpr uint32_t LANES = HD / 8, MASK = LANES == 16 ? 0xFFFFu : 0xFFu;
-#pragma unroll
-    for (uint32_t m = 1; m < 8; m <<= 1) {
-        const bool upper = (lane & m) != 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float y = __shfl_xor_sync(MASK, v[i], m);
-            v[i] = upper ? y - v[i] : v[i] + y;
-        }
-    }
-    const uint32_t signs = p.a.pool.signs[lane / 4] >> (lane % 4 * 8);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = flip(v[i] * 0.125f, signs >> i & 1u);
-    rows_put8(p.a.out, t * p.a.out.token_stride + head * p.a.out.head_stride + lane * 8, v);
+    for (int i = 0; i < 8; ++i) v[i] *= inv;
+    transform8_back(v, p.a.pool.signs[c / 4] >> (c % 4 * 8), lane);
+    if (lane < HD / 8) rows_put8(p.a.out, t * p.a.out.token_stride + head * p.a.out.head_stride + c * 8, v);
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-// One warp per item where there are several items for every warp that the SMs hold: their ends then overlap anyway, and nothing has to
+// One CTA per item where there are several items for every CTA that the SMs hold: their ends then overlap anyway, and nothing has to
 // be looked up or joined.
 SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     SplitArgs p{};
@@ -698,7 +717,7 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     p.tile = group > 8 || (near && rows > 8) ? 16 : 8;
     p.rbo = (group + p.tile - 1) / p.tile;
     p.rbp = near ? (rows + p.tile - 1) / p.tile : 0;
-    const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * p.rbo, room = (uint64_t)a.sm_count * split_ctas(d.head_dim, type != TYPE_BF16, type == TYPE_F32, p.tile / 8) * SP_WARPS;
+    const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * p.rbo, room = (uint64_t)a.sm_count * split_ctas(d.head_dim, type != TYPE_BF16, type == TYPE_F32, p.tile / 8);
     p.direct = p.rbp == 0 && items >= 4 * room;
     p.units = (uint32_t)(p.direct ? items : room);
     return p;
@@ -712,10 +731,11 @@ size_t near_floats(const SplitArgs &p) {
 // Halves of an operand: bf16 queries and weights are rounded to one each (11 bits where bf16 has 8); fp16 queries keep two, since a score is a
 // sum of head_dim roundings (one: an output of fp16 rows 2.3 times as far from 64 bits as its own rounding); fp32 keeps two of both.
 template <int HD, int BITS, int QT, int PT, int NR> cudaError_t split_go(cudaStream_t s, const SplitArgs &p) {
-    const size_t smem = split_smem<HD, BITS>();
+    constexpr size_t smem = SplitSmem<HD, BITS, QT, NR>::BYTES;
+    static_assert((smem + 1024) * split_ctas(HD, QT == 2, PT == 2, NR) <= 233472, "shared memory of an SM");
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(pool_split_kernel<HD, BITS, QT, PT, NR>), smem);
     if (e != cudaSuccess) return e;
-    return launch_kernel(pool_split_kernel<HD, BITS, QT, PT, NR>, dim3((p.units + SP_WARPS - 1) / SP_WARPS), dim3(SP_WARPS * 32), smem, s, true, p);
+    return launch_kernel(pool_split_kernel<HD, BITS, QT, PT, NR>, dim3(p.units), dim3(SP_WARPS * 32), smem, s, true, p);
 }
 template <int HD, int BITS, int NR> cudaError_t split_type(cudaStream_t s, const SplitArgs &p) {
     const uint32_t type = p.a.q.type;
@@ -756,8 +776,12 @@ cudaError_t launch_pool_attend(cudaStream_t s, const PoolAttnArgs &a, uint32_t *
     *launched += 1;
     if (e != cudaSuccess || (p.direct && a.prefix_len == 0)) return e;
     *launched += 1;
+    // rows are few where their pieces are many
+    const uint32_t rows = a.n_tok * a.heads;
+    uint32_t ways = MERGE_WARPS;
+    while (ways > 1 && (uint64_t)rows * ways > 4 * MERGE_WARPS * (uint64_t)a.sm_count) ways /= 2;
     const auto merge = d.head_dim == 128 ? pool_merge_kernel<128> : pool_merge_kernel<64>;
-    return launch_kernel(merge, dim3(a.n_tok * a.heads), dim3(MERGE_WARPS * 32), 0, s, true, p);
+    return launch_kernel(merge, dim3((rows + MERGE_WARPS / ways - 1) / (MERGE_WARPS / ways)), dim3(MERGE_WARPS * 32), 0, s, true, p, ways);
 }
 
 }  // namespace k2t

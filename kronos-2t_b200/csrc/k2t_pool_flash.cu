@@ -207,11 +207,7 @@ template <int HD, int BITS, int QT> __device__ __forceinline__ void flash_querie
         const uint32_t row = warp * mine + i + lane / LANES, r = r0 + row;
         float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, top = 0.0f;
         if (r < all) rows_get8(p.a.q, r / group * p.a.q.token_stride + (h * group + r % group) * p.a.q.head_stride + l * 8, v);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = __fmul_rn(flip(v[k], signs >> k & 1u), 0.125f);
-        butterflies_in(v);
-#pragma unroll
-        for (uint32_t m = 1; m < 8; m <<= 1) butterflies_across(v, m, lane);
+        transform8(v, signs, lane);
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
 #pragma unroll
