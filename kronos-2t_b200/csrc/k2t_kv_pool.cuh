@@ -142,15 +142,23 @@ __device__ __forceinline__ float rcp_approx(float x) { float y; asm("rcp.approx.
 __device__ __forceinline__ int query_exponent(float top) { return min(126, max(-126, 140 - (int)((__float_as_uint(top) >> 23) & 255u))); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// Four 4-bit codes (the low 16 bits of w) as bytes 128 + centroid.  A selector with bit 3 set yields a byte's sign, here 0: of the two
-// tables each index finds its magnitude in one and 0 in the other.
-__device__ __forceinline__ uint32_t centroids4(uint32_t w) {
-    constexpr uint32_t HI0 = 0x2C1F1206u, HI1 = 0x7F604B3Au, LO0 = 0x3A4B607Fu, LO1 = 0x06121F2Cu;
-    return (prmt(HI0, HI1, w ^ 0x8888u) | 0x80808080u) - prmt(LO0, LO1, w);
-}
-// Bytes 128 + c as halves c: 0x6400 + byte is 1024 + byte.
-__device__ __forceinline__ uint32_t halves_lo(uint32_t x) { return hsub2(prmt(x, 0x64646464u, 0x4140u), 0x64806480u); }
-__device__ __forceinline__ uint32_t halves_hi(uint32_t x) { return hsub2(prmt(x, 0x64646464u, 0x4342u), 0x64806480u); }
+// Constants of the expansion, kept in registers: left to the compiler they are loaded again for every use where registers are short.
+struct Expand {
+    uint32_t exponent, hi0, hi1, lo0, lo1;
+    __device__ __forceinline__ Expand() {
+        asm volatile("mov.b32 %0, 0x64646464;" : "=r"(exponent));
+        asm volatile("mov.b32 %0, 0x2C1F1206;" : "=r"(hi0));
+        asm volatile("mov.b32 %0, 0x7F604B3A;" : "=r"(hi1));
+        asm volatile("mov.b32 %0, 0x3A4B607F;" : "=r"(lo0));
+        asm volatile("mov.b32 %0, 0x06121F2C;" : "=r"(lo1));
+    }
+    // Bytes 128 + c (the lower or upper two) as halves c: 0x6400 + byte is 1024 + byte.
+    __device__ __forceinline__ uint32_t halves_lo(uint32_t x) const { return hsub2(prmt(x, exponent, 0x4140u), 0x64806480u); }
+    __device__ __forceinline__ uint32_t halves_hi(uint32_t x) const { return hsub2(prmt(x, exponent, 0x4342u), 0x64806480u); }
+    // Four 4-bit codes (the low 16 bits of w) as bytes 128 + centroid.  A selector with bit 3 set yields a byte's sign, here 0: of the two
+    // tables each index finds its magnitude in one and 0 in the other.
+    __device__ __forceinline__ uint32_t centroids4(uint32_t w) const { return (prmt(hi0, hi1, w ^ 0x8888u) | 0x80808080u) - prmt(lo0, lo1, w); }
+};
 
 constexpr uint32_t POOL_ERR_PAGE = 6;        // a page or slot outside the pool
 __device__ __forceinline__ void pool_bad_page(const PoolView &v) { atomicExch(v.err, POOL_ERR_PAGE); }

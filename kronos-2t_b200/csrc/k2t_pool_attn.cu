@@ -22,7 +22,11 @@ namespace {
 
 constexpr uint32_t SP_WARPS = 4, SP_STAGES = 2, WAIT_LIMIT = 1u << 22;
 // CTAs on an SM, by the registers of a kernel that spills nothing worth naming
-constexpr uint32_t split_ctas(uint32_t hd, bool two_terms, bool two_weights, uint32_t nr) { return hd == 64 || !two_terms ? (nr == 1 ? 4 : 3) : nr == 2 ? 2 : two_weights ? 3 : 4; }
+constexpr uint32_t split_ctas(uint32_t hd, uint32_t bits, bool two_terms, bool two_weights, uint32_t nr) {
+    if (hd == 64) return nr == 1 ? 4 : 3;
+    if (nr == 2) return two_terms || bits == 4 ? 2 : 3;
+    return 4 - (two_weights ? 1 : 0) - (two_terms && bits == 4 ? 1 : 0);
+}
 // Shared memory: the warps' rings, the queries as halves, and the warps' results of eight rows (rows HD + 4 floats apart, so that lanes of
 // neighbouring rows meet in other banks).
 template <int HD, int BITS, int QT, int NR> struct SplitSmem {
@@ -31,12 +35,12 @@ template <int HD, int BITS, int QT, int NR> struct SplitSmem {
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {       // 8 x 8 halves over the warp
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 template <int WORDS> __device__ __forceinline__ void lds_words(uint32_t addr, uint32_t *w) {
@@ -242,9 +246,26 @@ template <int HD, int NR> struct State {
     float o[NR][HD / 16][4], m[NR][2], l[NR][2];
 };
 
+// Where a lane's rows lie in a block: row_place of its rows, of which the second pair of keys and of values lies a fixed distance behind the
+// first (rows of 32 bytes: values by exclusive-or of the row).
+template <int HD, int BITS> struct LanePlaces {
+    using B = PoolBlock<HD, BITS>;
+    static constexpr uint32_t RB = B::RB;
+    uint32_t k[2], v[2];
+    __device__ __forceinline__ explicit LanePlaces(uint32_t lane) {
+        const uint32_t n = lane >> 2, t = lane & 3u, p0 = 4 * (n >> 1) + (n & 1u);
+        k[0] = row_place<RB>(p0, t * (BITS == 8 ? 16 : 8));
+        k[1] = RB == 32 || HD == 64 ? row_place<RB>(p0 + 2, t * (BITS == 8 ? 16 : 8)) : row_place<RB>(p0, RB / 2 + t * (BITS == 8 ? 16 : 8));
+        v[0] = B::V_AT + row_place<RB>(4 * t, n * (RB / 8));
+        v[1] = B::V_AT + row_place<RB>(4 * t + 1, n * (RB / 8));
+    }
+    __device__ __forceinline__ uint32_t key(uint32_t at, int j, int g) const { return HD == 64 ? at + k[j] : at + k[g] + j * 2 * RB; }          // row p0 + 2 j, group g
+    __device__ __forceinline__ uint32_t value(uint32_t at, int i) const { return RB == 32 ? at + (v[0] ^ (i * 32)) : at + v[i & 1] + (i >> 1) * 2 * RB; }          // row 4 t + i
+};
+
 // One block of 16 positions, `valid` of them in sight, at shared address `at`.
 template <int HD, int BITS, int QT, int PT, int NR>
-__device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t lane, const Query<HD, QT, NR> &q, State<HD, NR> &st) {
+__device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t lane, const LanePlaces<HD, BITS> &place, const Expand &ex, const Query<HD, QT, NR> &q, State<HD, NR> &st) {
     using B = PoolBlock<HD, BITS>;
     constexpr int G = B::G;
     const uint32_t n = lane >> 2, t = lane & 3u;
@@ -255,29 +276,45 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
     for (int r = 0; r < NR; ++r)
 #pragma unroll
         for (int g = 0; g < G; ++g) s[r][g][0] = s[r][g][1] = s[r][g][2] = s[r][g][3] = 0.0f;
+    uint32_t kw[HD / 64][2][4];
+#pragma unroll
+    for (int g = 0; g < HD / 64; ++g)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) lds_words<BITS == 8 ? 4 : 2>(place.key(at, j, g), kw[g][j]);
+    uint32_t sc[2][2];                         // scales as they lie: keys, values of p0, p0 + 2
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t off = BITS == 4 && G == 1 ? (p0 & ~1u) * 2 + 4 * j : p0 * 4 + 8 * j;          // of one group of 4 bits two positions share a word
+        lds_words<1>(at + B::KS_AT + off, &sc[0][j]);
+        lds_words<1>(at + B::VS_AT + off, &sc[1][j]);
+    }
 #pragma unroll
     for (int g = 0; g < HD / 64; ++g) {
         uint32_t w[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             if (BITS == 8) {
-                lds_words<4>(at + row_place<B::RB>(p0 + 2 * j, g * 64 + t * 16), w[j]);
-            } else {
-                uint32_t x[2];
-                lds_words<2>(at + row_place<B::RB>(p0 + 2 * j, g * 32 + t * 8), x);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) { w[j][2 * i] = centroids4(x[i]); w[j][2 * i + 1] = centroids4(x[i] >> 16); }
+                for (int i = 0; i < 4; ++i) w[j][i] = kw[g][j][i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) { w[j][2 * i] = ex.centroids4(kw[g][j][i]); w[j][2 * i + 1] = ex.centroids4(kw[g][j][i] >> 16); }
             }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t a[4] = {halves_lo(w[0][i]), halves_lo(w[1][i]), halves_hi(w[0][i]), halves_hi(w[1][i])};
+            const uint32_t a[4] = {ex.halves_lo(w[0][i]), ex.halves_lo(w[1][i]), ex.halves_hi(w[0][i]), ex.halves_hi(w[1][i])};
 #pragma unroll
             for (int r = 0; r < NR; ++r)
 #pragma unroll
                 for (int k = 0; k < QT; ++k) mma_f16(s[r][G == 1 ? 0 : g], a, q.b[r][k][4 * g + i][0], q.b[r][k][4 * g + i][1]);
         }
     }
+    // values of positions 4 t .. 4 t + 3, asked for ahead of the softmax
+    constexpr int W = HD / 32, VW = BITS == 8 ? W : W / 2;          // words of four elements; as they lie
+    uint32_t vw[4][VW];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds_words<VW>(place.value(at, i), vw[i]);
     // constants of positions p0 and p0 + 2
     float ks[G][2], lv[2], iv[2], part[G][2];
 #pragma unroll
@@ -285,20 +322,14 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
         const uint32_t pos = p0 + 2 * j;
         float v[G], top;
         if (BITS == 8) {
-            ks[0][j] = lds_f32(at + B::KS_AT + pos * 4);
-            v[0] = lds_f32(at + B::VS_AT + pos * 4);
+            ks[0][j] = __uint_as_float(sc[0][j]);
+            v[0] = __uint_as_float(sc[1][j]);
         } else if (G == 2) {
-            uint32_t a, b;
-            lds_words<1>(at + B::KS_AT + pos * 4, &a);
-            lds_words<1>(at + B::VS_AT + pos * 4, &b);
-            ks[0][j] = __uint_as_float(a << 16); ks[G - 1][j] = __uint_as_float(a & 0xFFFF0000u);
-            v[0] = __uint_as_float(b << 16); v[G - 1] = __uint_as_float(b & 0xFFFF0000u);
+            ks[0][j] = __uint_as_float(sc[0][j] << 16); ks[G - 1][j] = __uint_as_float(sc[0][j] & 0xFFFF0000u);
+            v[0] = __uint_as_float(sc[1][j] << 16); v[G - 1] = __uint_as_float(sc[1][j] & 0xFFFF0000u);
         } else {
-            uint32_t a, b;                     // two positions a word
-            lds_words<1>(at + B::KS_AT + (pos & ~1u) * 2, &a);
-            lds_words<1>(at + B::VS_AT + (pos & ~1u) * 2, &b);
-            ks[0][j] = __uint_as_float(pos & 1u ? a & 0xFFFF0000u : a << 16);
-            v[0] = __uint_as_float(pos & 1u ? b & 0xFFFF0000u : b << 16);
+            ks[0][j] = __uint_as_float(pos & 1u ? sc[0][j] & 0xFFFF0000u : sc[0][j] << 16);
+            v[0] = __uint_as_float(pos & 1u ? sc[1][j] & 0xFFFF0000u : sc[1][j] << 16);
         }
         top = G == 1 ? v[0] : fmaxf(v[0], v[G - 1]);          // scales are not negative, and all groups of a row are NaN or none
         if (top == 0.0f) top = 1.0f;               // a row of zeros: 8-bit codes are 0, groups of 4 bits have a factor
@@ -347,10 +378,10 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
     uint32_t b[NR][G][PT][2];                  // weights as the second operand: transposed, the lane's positions are 4 t .. 4 t + 3 of query n
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
+        const float base0 = st.m[r][0] == -INFINITY ? 0.0f : st.m[r][0], base1 = st.m[r][1] == -INFINITY ? 0.0f : st.m[r][1];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float m = st.m[r][e & 1] == -INFINITY ? 0.0f : st.m[r][e & 1];
-            x[r][e] = exp2_approx(x[r][e] - m);
+            x[r][e] = exp2_approx(x[r][e] - (e & 1 ? base1 : base0));
             st.l[r][e & 1] = __fmaf_rn(x[r][e], iv[e >> 1], st.l[r][e & 1]);
         }
 #pragma unroll
@@ -367,24 +398,22 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
             }
     }
     // values: columns of the first operand are positions, two of them a word; rows n and n + 8 of tile j are elements n HD / 8 + 2 j, + 1
-    constexpr int W = HD / 32;                 // words of four elements
     uint32_t v[4][W];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t from = at + B::V_AT + row_place<B::RB>(4 * t + i, n * (B::RB / 8));
-        if (BITS == 8) {
-            lds_words<W>(from, v[i]);
-        } else {
-            uint32_t y[W / 2];
-            lds_words<W / 2>(from, y);
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int k = 0; k < W / 2; ++k) { v[i][2 * k] = centroids4(y[k]); v[i][2 * k + 1] = centroids4(y[k] >> 16); }
+        for (int k = 0; k < VW; ++k) {
+            if (BITS == 8) {
+                v[i][k] = vw[i][k];
+            } else {
+                v[i][2 * k] = ex.centroids4(vw[i][k]);
+                v[i][2 * k + 1] = ex.centroids4(vw[i][k] >> 16);
+            }
         }
-    }
 #pragma unroll
     for (int k = 0; k < W; ++k) {
         const uint32_t lo01 = prmt(v[0][k], v[1][k], 0x5140u), lo23 = prmt(v[2][k], v[3][k], 0x5140u), hi01 = prmt(v[0][k], v[1][k], 0x7362u), hi23 = prmt(v[2][k], v[3][k], 0x7362u);
-        const uint32_t first[4] = {halves_lo(lo01), halves_hi(lo01), halves_lo(lo23), halves_hi(lo23)}, second[4] = {halves_lo(hi01), halves_hi(hi01), halves_lo(hi23), halves_hi(hi23)};
+        const uint32_t first[4] = {ex.halves_lo(lo01), ex.halves_hi(lo01), ex.halves_lo(lo23), ex.halves_hi(lo23)}, second[4] = {ex.halves_lo(hi01), ex.halves_hi(hi01), ex.halves_lo(hi23), ex.halves_hi(hi23)};
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -402,7 +431,7 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
 }
 
 template <int HD, int BITS, int QT, int PT, int NR>
-__global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2, NR)) pool_split_kernel(const __grid_constant__ SplitArgs p) {
+__global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, BITS, QT == 2, PT == 2, NR)) pool_split_kernel(const __grid_constant__ SplitArgs p) {
     using B = PoolBlock<HD, BITS>;
     using S = SplitSmem<HD, BITS, QT, NR>;
     extern __shared__ __align__(128) uint8_t smb[];
@@ -483,6 +512,8 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2
     for (uint32_t i = 0; i < SP_STAGES; ++i) request();
     float *s_factor = reinterpret_cast<float *>(smb + S::FACTOR), *s_join = reinterpret_cast<float *>(smb + S::JOIN);
     float2 *s_ml = reinterpret_cast<float2 *>(smb + S::ML);
+    const LanePlaces<HD, BITS> place(lane);
+    const Expand ex;
     Query<HD, QT, NR> q;
     State<HD, NR> st;
     bool ok = true;
@@ -512,7 +543,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, QT == 2, PT == 2
                 landed = __all_sync(0xffffffffu, landed);
                 ok = ok && landed;
                 phase ^= 1u << stage;
-                block_step<HD, BITS, QT, PT, NR>(ring + stage * B::BYTES, valid, lane, q, st);
+                block_step<HD, BITS, QT, PT, NR>(ring + stage * B::BYTES, valid, lane, place, ex, q, st);
             }
             __syncwarp();                          // all lanes are done with the stage
             request();
@@ -717,7 +748,7 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     p.tile = group > 8 || (near && rows > 8) ? 16 : 8;
     p.rbo = (group + p.tile - 1) / p.tile;
     p.rbp = near ? (rows + p.tile - 1) / p.tile : 0;
-    const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * p.rbo, room = (uint64_t)a.sm_count * split_ctas(d.head_dim, type != TYPE_BF16, type == TYPE_F32, p.tile / 8);
+    const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * p.rbo, room = (uint64_t)a.sm_count * split_ctas(d.head_dim, d.bits, type != TYPE_BF16, type == TYPE_F32, p.tile / 8);
     p.direct = p.rbp == 0 && items >= 4 * room;
     p.units = (uint32_t)(p.direct ? items : room);
     return p;
@@ -732,7 +763,7 @@ size_t near_floats(const SplitArgs &p) {
 // sum of head_dim roundings (one: an output of fp16 rows 2.3 times as far from 64 bits as its own rounding); fp32 keeps two of both.
 template <int HD, int BITS, int QT, int PT, int NR> cudaError_t split_go(cudaStream_t s, const SplitArgs &p) {
     constexpr size_t smem = SplitSmem<HD, BITS, QT, NR>::BYTES;
-    static_assert((smem + 1024) * split_ctas(HD, QT == 2, PT == 2, NR) <= 233472, "shared memory of an SM");
+    static_assert((smem + 1024) * split_ctas(HD, BITS, QT == 2, PT == 2, NR) <= 233472, "shared memory of an SM");
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(pool_split_kernel<HD, BITS, QT, PT, NR>), smem);
     if (e != cudaSuccess) return e;
     return launch_kernel(pool_split_kernel<HD, BITS, QT, PT, NR>, dim3(p.units), dim3(SP_WARPS * 32), smem, s, true, p);

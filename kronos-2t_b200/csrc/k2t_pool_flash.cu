@@ -89,6 +89,7 @@ template <int HD, int BITS, int QT> struct Converter {
     };
     const SplitArgs &p;
     uint32_t ct, lane, first, load_at, store_at, store_x;
+    Expand ex;
 
     __device__ __forceinline__ Converter(const SplitArgs &args, uint32_t thread) : p(args), ct(thread), lane(thread & 31u) {
         // eight neighbouring threads: four chunks of two neighbouring rows, whose stores meet in no bank (rows differ in the last bit of the swizzle)
@@ -141,14 +142,14 @@ template <int HD, int BITS, int QT> struct Converter {
     }
     __device__ __forceinline__ void expand(uint32_t at, const uint4 &w) const {          // `at`: the thread's row and panel
         if (BITS == 8) {
-            sts4(at + (store_x << 4), halves_lo(w.x), halves_hi(w.x), halves_lo(w.y), halves_hi(w.y));
-            sts4(at + ((store_x ^ 1u) << 4), halves_lo(w.z), halves_hi(w.z), halves_lo(w.w), halves_hi(w.w));
+            sts4(at + (store_x << 4), ex.halves_lo(w.x), ex.halves_hi(w.x), ex.halves_lo(w.y), ex.halves_hi(w.y));
+            sts4(at + ((store_x ^ 1u) << 4), ex.halves_lo(w.z), ex.halves_hi(w.z), ex.halves_lo(w.w), ex.halves_hi(w.w));
         } else {
             const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
-                const uint32_t lo = centroids4(x[i]), hi = centroids4(x[i] >> 16);
-                sts4(at + ((store_x ^ i) << 4), halves_lo(lo), halves_hi(lo), halves_lo(hi), halves_hi(hi));
+                const uint32_t lo = ex.centroids4(x[i]), hi = ex.centroids4(x[i] >> 16);
+                sts4(at + ((store_x ^ i) << 4), ex.halves_lo(lo), ex.halves_hi(lo), ex.halves_lo(hi), ex.halves_hi(hi));
             }
         }
     }
