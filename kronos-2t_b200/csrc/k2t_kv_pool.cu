@@ -195,15 +195,16 @@ template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_
 // CTA = (token, kv head).  The query is the sum of the head's queries, quantised as an 8-bit row; a page scores the whole-number product
 // with its block key times the key's scale (one rounding, so that scores are the same wherever they are computed).  The order of
 // scores is that of their bits as numbers; the highest `want` of them are found by four passes over their bytes, ties by index.
-constexpr uint32_t SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32;
-
+// Two sizes of CTA: with few (token, kv head) pairs the time is one CTA's chain of loads, and 512 threads have a whole sequence's keys in
+// flight; with many, smaller CTAs have fewer threads idle at their barriers.
 __device__ __forceinline__ uint32_t ordered(float x) {           // NaN behind everything
     if (x != x) return 0;
     const uint32_t b = __float_as_uint(x == 0.0f ? 0.0f : x);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template <int HD> __global__ void __launch_bounds__(SEL_THREADS) pool_select_kernel(const __grid_constant__ PoolAttnArgs a) {
+template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_THREADS) pool_select_kernel(const __grid_constant__ PoolAttnArgs a) {
+    constexpr uint32_t SEL_WARPS = SEL_THREADS / 32;
     extern __shared__ uint32_t s_key[];
     __shared__ __align__(16) int8_t s_q[HD];
     __shared__ uint32_t s_hist[256], s_warp[SEL_WARPS], s_pick[2];
@@ -211,8 +212,8 @@ template <int HD> __global__ void __launch_bounds__(SEL_THREADS) pool_select_ker
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t = blockIdx.x / d.kv_heads, h = blockIdx.x % d.kv_heads, group = a.heads / d.kv_heads;
     pdl_wait();
     pdl_trigger();
-    const uint32_t len = (uint32_t)max(0, __ldcg(a.lens + t));
-    const int32_t seq = a.seq != nullptr ? __ldcg(a.seq + t) : (int32_t)t;
+    const int32_t seen = __ldcg(a.lens + t), seq = a.seq != nullptr ? __ldcg(a.seq + t) : (int32_t)t;
+    const uint32_t len = seq < 0 ? 0u : (uint32_t)max(0, seen);
     uint32_t n = (uint32_t)(((uint64_t)len + (1u << d.page_shift) - 1) >> d.page_shift);
     if (n > a.pages_stride) {
         n = a.pages_stride;
@@ -223,48 +224,77 @@ template <int HD> __global__ void __launch_bounds__(SEL_THREADS) pool_select_ker
         for (uint32_t i = tid; i < a.top; i += SEL_THREADS) out[i] = i < n ? (int32_t)i : -1;
         return;
     }
-    if (warp == 0) {
+    // eight lanes read a block key, four pages at a time; the first ones are on their way while the query is made
+    constexpr uint32_t W = HD / 32, AHEAD = 4;              // words of a lane
+    const int32_t *table = a.pages + (size_t)seq * a.pages_stride;
+    const uint32_t from = a.sinks, to = n - a.local, sub = lane & 7u;          // of these pages the best: n > top >= sinks + local
+    uint32_t key[AHEAD][W];
+    float scale[AHEAD];
+    auto ask = [&](uint32_t i0) {
+        int32_t page[AHEAD];
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; ++u) {
+            const uint32_t i = i0 + u * SEL_WARPS * 4 + lane / 8;
+            page[u] = i < to ? __ldcg(table + i) : 0;
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; ++u) {
+            const bool bad = page[u] < 0 || (uint32_t)page[u] >= d.num_pages;          // scores 0
+            if (bad) pool_bad_page(a.pool);
+            const size_t at = (size_t)(bad ? 0 : page[u]) * d.kv_heads + h;
+            const uint32_t *k = reinterpret_cast<const uint32_t *>(a.pool.block_keys + at * HD) + sub * W;
+            if constexpr (W == 4) {
+                const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(k));
+                key[u][0] = x.x; key[u][1] = x.y; key[u][2] = x.z; key[u][3] = x.w;
+            } else {
+                const uint2 x = __ldcg(reinterpret_cast<const uint2 *>(k));
+                key[u][0] = x.x; key[u][1] = x.y;
+            }
+            const float s = __ldcg(a.pool.block_key_scales + at);
+            scale[u] = bad ? 0.0f : s;
+        }
+    };
+    ask(from + warp * 4);
+    if (warp == SEL_WARPS - 1) {
         constexpr uint32_t LANES = HD / 8;
         const uint32_t l = lane % LANES;
-        float v[8], x[8];
-        for (uint32_t g = 0; g < group; ++g) {
-            rows_get8(a.q, t * a.q.token_stride + (h * group + g) * a.q.head_stride + l * 8, x);
+        float v[8];
+#pragma unroll 1
+        for (uint32_t g0 = 0; g0 < group; g0 += 8) {          // the sum in the order of the heads, eight of them on their way
+            float x[8][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = g == 0 ? x[i] : __fadd_rn(v[i], x[i]);
+            for (uint32_t g = 0; g < 8; ++g)
+                if (g0 + g < group) rows_get8(a.q, t * a.q.token_stride + (h * group + g0 + g) * a.q.head_stride + l * 8, x[g]);
+#pragma unroll
+            for (uint32_t g = 0; g < 8; ++g)
+                if (g0 + g < group)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = g0 + g == 0 ? x[g][i] : __fadd_rn(v[i], x[g][i]);
         }
         transform8(v, signs8(a.pool, l * 8), lane);
         int c[8];
-        float scale;
-        quantise8<LANES>(v, lane, c, scale);
+        float unused;
+        quantise8<LANES>(v, lane, c, unused);
         if (lane < LANES)
 #pragma unroll
             for (int i = 0; i < 8; ++i) s_q[l * 8 + i] = (int8_t)c[i];
     }
     __syncthreads();
-    // eight lanes read a block key
-    const int32_t *table = a.pages + (size_t)seq * a.pages_stride;
-    const uint32_t from = a.sinks, to = n - a.local;          // of these pages the best: n > top >= sinks + local
-    constexpr uint32_t W = HD / 32;              // words of a lane
-    for (uint32_t i0 = from + warp * 4; i0 < to; i0 += SEL_WARPS * 4) {
-        const uint32_t i = i0 + lane / 8;
-        int dot = 0;
-        float s = 0.0f;
-        if (i < to) {
-            const int32_t page = __ldcg(table + i);
-            if (page < 0 || (uint32_t)page >= d.num_pages) {
-                pool_bad_page(a.pool);
-            } else {
-                const size_t at = (size_t)page * d.kv_heads + h;
-                const uint32_t *k = reinterpret_cast<const uint32_t *>(a.pool.block_keys + at * HD) + (lane & 7u) * W;
-                const int *q = reinterpret_cast<const int *>(s_q) + (lane & 7u) * W;
+    int q[W];
 #pragma unroll
-                for (uint32_t j = 0; j < W; ++j) dot = dp4a_ss(__ldcg(k + j), q[j], dot);
-                s = __ldcg(a.pool.block_key_scales + at);
-            }
+    for (uint32_t j = 0; j < W; ++j) q[j] = reinterpret_cast<const int *>(s_q)[sub * W + j];
+    for (uint32_t i0 = from + warp * 4; i0 < to; i0 += AHEAD * SEL_WARPS * 4) {
+        if (i0 != from + warp * 4) ask(i0);
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; ++u) {
+            const uint32_t i = i0 + u * SEL_WARPS * 4 + lane / 8;
+            int dot = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < W; ++j) dot = dp4a_ss(key[u][j], q[j], dot);
+#pragma unroll
+            for (int m = 4; m > 0; m >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, m);
+            if (i < to && sub == 0) s_key[i - from] = ordered(__fmul_rn((float)dot, scale[u]));
         }
-#pragma unroll
-        for (int m = 4; m > 0; m >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, m);
-        if (i < to && (lane & 7u) == 0) s_key[i - from] = ordered(__fmul_rn((float)dot, s));
     }
     __syncthreads();
     const uint32_t m = to - from;
@@ -361,11 +391,13 @@ cudaError_t launch_pool_load(cudaStream_t s, const PoolStoreArgs &a, uint32_t *l
 }
 cudaError_t launch_pool_select(cudaStream_t s, const PoolAttnArgs &a, uint32_t *launched) {
     const size_t smem = (size_t)a.pages_stride * 4;
-    const auto kernel = a.pool.d.head_dim == 128 ? pool_select_kernel<128> : pool_select_kernel<64>;
+    const uint32_t pairs = a.n_tok * a.pool.d.kv_heads;
+    const bool small = pairs >= 4 * a.sm_count && a.pages_stride <= 4096;
+    const auto kernel = a.pool.d.head_dim == 128 ? (small ? pool_select_kernel<128, 128> : pool_select_kernel<128, 512>) : small ? pool_select_kernel<64, 128> : pool_select_kernel<64, 512>;
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
     *launched += 1;
-    return launch_kernel(kernel, dim3(a.n_tok * a.pool.d.kv_heads), dim3(SEL_THREADS), smem, s, true, a);
+    return launch_kernel(kernel, dim3(pairs), dim3(small ? 128 : 512), smem, s, true, a);
 }
 
 }  // namespace k2t

@@ -152,25 +152,26 @@ __device__ __forceinline__ void item_at(const SplitArgs &p, uint64_t x, uint32_t
     item_fill(p, it);
 }
 // The item behind this one; tokens without a block are passed over (the caller knows that there is one).
-__device__ __forceinline__ void item_after(const SplitArgs &p, Item &it) {
+__device__ __forceinline__ bool item_after(const SplitArgs &p, Item &it) {          // whether its list is another one
     it.next = 0;
     it.index += 1;
-    if (it.prefix) {
-        if (++it.rb == p.rbp) { it.rb = 0; it.h += 1; }
-        if (it.h < p.a.pool.d.kv_heads) return;
-        it.prefix = false;
-        it.index = it.t = it.h = it.rb = 0;
-        item_fill(p, it);
-    } else {
-        if (++it.rb == p.rbo) { it.rb = 0; it.h += 1; }
-        if (it.h == p.a.pool.d.kv_heads) { it.h = 0; it.t += 1; }
-        if (it.t < p.a.n_tok) item_fill(p, it);
+    if (++it.rb == (it.prefix ? p.rbp : p.rbo)) { it.rb = 0; it.h += 1; }
+    if (it.h < p.a.pool.d.kv_heads) {
+        if (p.a.chosen == nullptr || it.rb != 0) return false;
+        it.list += p.a.top;
+        return true;
     }
+    it.h = 0;
+    it.t += it.prefix ? 0 : 1;
+    if (it.prefix) it.index = 0;
+    it.prefix = false;
+    if (it.t < p.a.n_tok) item_fill(p, it);
     while (it.blocks == 0 && it.t + 1 < p.a.n_tok) {
         it.t += 1;
         it.index += p.a.pool.d.kv_heads * p.rbo;
         item_fill(p, it);
     }
+    return true;
 }
 
 // ------------------------------------------------------------------------------------------------ the warp's rows
@@ -446,8 +447,13 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, BITS, QT == 2, P
         fence_mbar_init();
     }
     __syncwarp();
-    pdl_wait();
-    pdl_trigger();
+    // Behind the prefix's kernel: that one started its dependents when everything it reads was there, and writes nothing that is read here, so
+    // only the end of this kernel waits for it -- for the merge, which waits for this one alone.
+    const bool behind = p.flash.on;
+    if (!behind) {
+        pdl_wait();
+        pdl_trigger();
+    }
     Item it;
     uint32_t left;                             // blocks of the CTA's part
     if (p.direct) {             // the part is one item, which may hold no block at all
@@ -462,7 +468,10 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, BITS, QT == 2, P
         left = it.blocks;
     } else {
         const uint64_t all = prefix_line(p) + warp_total(p, lane) * d.kv_heads * p.rbo, part = part_blocks(all, p.units), x = (uint64_t)unit * part;
-        if (x >= all) return;
+        if (x >= all) {
+            pdl_wait();
+            return;
+        }
         left = (uint32_t)min(part, all - x);
         item_at(p, x, lane, it);
     }
@@ -477,11 +486,10 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, BITS, QT == 2, P
     auto request = [&]() {                     // one block, into stage asked % SP_STAGES
         while (ask.next >= ask_end) {
             if (ask_left == 0) return;
-            item_after(p, ask);
+            if (item_after(p, ask)) pages_at = ~0u;
             ask_end = min(ask_left, ask.blocks);
             ask_left -= ask_end;
             ask.next = warp;
-            pages_at = ~0u;
         }
         const uint32_t b = ask.next, entry = b >> bs;
         if (pages_at != entry >> 5) {
@@ -598,6 +606,10 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, BITS, QT == 2, P
         item_after(p, it);
     }
     if (!ok && lane == 0) atomicCAS(p.a.pool.err, 0u, 1u);
+    if (behind) {
+        pdl_wait();
+        pdl_trigger();
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ partial results
@@ -749,7 +761,7 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     p.rbo = (group + p.tile - 1) / p.tile;
     p.rbp = near ? (rows + p.tile - 1) / p.tile : 0;
     const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * p.rbo, room = (uint64_t)a.sm_count * split_ctas(d.head_dim, d.bits, type != TYPE_BF16, type == TYPE_F32, p.tile / 8);
-    p.direct = p.rbp == 0 && items >= 4 * room;
+    p.direct = p.rbp == 0 && items >= 3 * room;
     p.units = (uint32_t)(p.direct ? items : room);
     return p;
 }

@@ -203,11 +203,23 @@ template <int HD, int BITS, int QT> __device__ __forceinline__ void flash_querie
     const uint32_t group = p.a.heads / p.a.pool.d.kv_heads, all = p.a.n_tok * group, h = item / f.row_tiles, r0 = item % f.row_tiles * 2 * FLASH_ROWS;
     const uint32_t mine = (f.halved ? FLASH_ROWS : 2 * FLASH_ROWS) / FL_SOFT, l = lane % LANES;
     const uint32_t signs = p.a.pool.signs[l / 4] >> (l % 4 * 8);
-#pragma unroll 2
-    for (uint32_t i = 0; i < mine; i += ROWS) {
-        const uint32_t row = warp * mine + i + lane / LANES, r = r0 + row;
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, top = 0.0f;
-        if (r < all) rows_get8(p.a.q, r / group * p.a.q.token_stride + (h * group + r % group) * p.a.q.head_stride + l * 8, v);
+    constexpr uint32_t AHEAD = 4;              // rows of a lane on their way together
+#pragma unroll 1
+    for (uint32_t i0 = 0; i0 < mine; i0 += ROWS * AHEAD) {
+        float ahead[AHEAD][8];
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; ++u) {
+            const uint32_t r = r0 + warp * mine + i0 + u * ROWS + lane / LANES;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) ahead[u][k] = 0.0f;
+            if (i0 + u * ROWS < mine && r < all) rows_get8(p.a.q, r / group * p.a.q.token_stride + (h * group + r % group) * p.a.q.head_stride + l * 8, ahead[u]);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < AHEAD; ++u) {
+        const uint32_t i = i0 + u * ROWS;
+        if (i >= mine) break;
+        const uint32_t row = warp * mine + i + lane / LANES;
+        float (&v)[8] = ahead[u], top = 0.0f;
         transform8(v, signs, lane);
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
@@ -227,6 +239,7 @@ template <int HD, int BITS, int QT> __device__ __forceinline__ void flash_querie
         const uint32_t at = s_q + row / FLASH_ROWS * QT * F::Q_TILE + (l / 8) * (FLASH_ROWS * 128) + row % FLASH_ROWS * 128 + (((l % 8) ^ (row & 7u)) << 4);
         sts4(at, hi[0], hi[1], hi[2], hi[3]);
         if (QT == 2) sts4(at + F::Q_TILE, lo[0], lo[1], lo[2], lo[3]);
+        }
     }
 }
 
