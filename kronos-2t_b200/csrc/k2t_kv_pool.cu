@@ -8,13 +8,23 @@
 namespace k2t {
 namespace {
 
-__constant__ float CENTROIDS[16] = {-127.f, -96.f, -75.f, -58.f, -44.f, -31.f, -18.f, -6.f, 6.f, 18.f, 31.f, 44.f, 58.f, 75.f, 96.f, 127.f};
+// The nearest of the 16 centroids: its index, and its value (borders halfway between the magnitudes).
 __device__ __forceinline__ uint32_t nearest(float y) {
     const float a = fabsf(y);
     const uint32_t p = a < 37.5f ? (a < 12.0f ? 0u : a < 24.5f ? 1u : 2u) : a < 85.5f ? (a < 51.0f ? 3u : a < 66.5f ? 4u : 5u) : a < 111.5f ? 6u : 7u;
     return y >= 0.0f ? 8u + p : 7u - p;
 }
+__device__ __forceinline__ float nearest_value(float y) {
+    const float a = fabsf(y);
+    const float c = a < 37.5f ? (a < 12.0f ? 6.0f : a < 24.5f ? 18.0f : 31.0f) : a < 85.5f ? (a < 51.0f ? 44.0f : a < 66.5f ? 58.0f : 75.0f) : a < 111.5f ? 96.0f : 127.0f;
+    return y >= 0.0f ? c : -c;
+}
 constexpr float SMALLEST = 1.1920929e-07f;       // 8-bit rows up to here are stored as zeros
+// Rounded to the nearest whole number, the even one of two: the low byte of the result.  |x| <= 2^22.
+__device__ __forceinline__ uint32_t rounded_byte(float x) { return __float_as_uint(__fadd_rn(x, 12582912.0f)); }
+__device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return prmt(prmt(a, b, 0x0040u), prmt(c, d, 0x0040u), 0x5410u); }
+// Byte i of w, which holds 128 + c, as c: 0x4B0000xx is 2^23 + xx.
+__device__ __forceinline__ float signed_byte(uint32_t w, uint32_t i) { return __fsub_rn(__uint_as_float(prmt(w, 0x4B000000u, 0x7540u + i)), 8388736.0f); }
 
 template <int LANES> __device__ __forceinline__ float max_over(float x) {        // of LANES neighbouring lanes
 #pragma unroll
@@ -22,22 +32,22 @@ template <int LANES> __device__ __forceinline__ float max_over(float x) {       
     return x;
 }
 template <int LANES> __device__ __forceinline__ bool any_over(bool b, uint32_t lane) {
-    return (__ballot_sync(0xffffffffu, b) >> (lane & ~(uint32_t)(LANES - 1)) & ((1u << LANES) - 1u)) != 0;
+    return (__ballot_sync(0xffffffffu, b) >> (lane & ~(uint32_t)(LANES - 1)) & (0xffffffffu >> (32 - LANES))) != 0;
 }
 
 // A row over LANES lanes, eight values each, as 8-bit codes: what all quantised rows of 8 bits share.  `scale` is NaN for a row that is
 // not finite (its codes are 0).
-template <int LANES> __device__ __forceinline__ void quantise8(const float (&v)[8], uint32_t lane, int (&code)[8], float &scale) {
+template <int LANES, int N> __device__ __forceinline__ void quantise8(const float (&v)[N], uint32_t lane, uint32_t (&code)[N], float &scale) {          // codes: the low bytes
     float top = 0.0f;
     bool bad = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { top = fmaxf(top, fabsf(v[i])); bad |= not_finite(v[i]); }
+    for (int i = 0; i < N; ++i) { top = fmaxf(top, fabsf(v[i])); bad |= not_finite(v[i]); }
     bad = any_over<LANES>(bad, lane);
     top = max_over<LANES>(top);
     const bool zero = top <= SMALLEST || bad;
     const float inv = zero ? 0.0f : __fdiv_rn(127.0f, top);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) code[i] = zero ? 0 : __float2int_rn(__fmul_rn(v[i], inv));
+    for (int i = 0; i < N; ++i) code[i] = rounded_byte(bad ? 0.0f : __fmul_rn(v[i], inv));
     scale = bad ? __uint_as_float(0x7FC00000u) : zero ? 0.0f : __fdiv_rn(top, 127.0f);
 }
 
@@ -52,33 +62,26 @@ __device__ __forceinline__ uint8_t *block_of(const PoolView &p, int64_t slot, ui
 }
 
 // ------------------------------------------------------------------------------------------------ rows in, rows out
-// head_dim / 8 lanes hold a row.  A warp takes 32 * 8 values: 2 rows of 128 or 4 of 64; rows are numbered (token, keys | values, head).
-constexpr uint32_t ROW_THREADS = 256;
+// head_dim / 8 lanes hold a row, eight values each; rows are numbered (token, keys | values, head).  A thread has its part of ROW_AHEAD rows on
+// the way at a time.
+constexpr uint32_t ROW_THREADS = 256, ROW_AHEAD = 4;
+struct RowAt { uint32_t t, value, head; };
+__device__ __forceinline__ RowAt row_at(const PoolStoreArgs &a, uint32_t r) {          // r below 2^31: a division by a multiplication (and a shift) that is exact there
+    const uint32_t per = 2 * a.pool.d.kv_heads, t = __umulhi(r, a.rows_mul) >> a.rows_shift, u = r - t * per, value = u >= a.pool.d.kv_heads ? 1u : 0u;
+    return RowAt{t, value, u - value * a.pool.d.kv_heads};
+}
 
-template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_store_kernel(const __grid_constant__ PoolStoreArgs a) {
+// One row, transformed, into its place.
+template <int HD, int BITS> __device__ __forceinline__ void put_row(const PoolStoreArgs &a, uint8_t *block, uint32_t row, uint32_t value, uint32_t l, uint32_t lane, float (&v)[8]) {
     using B = PoolBlock<HD, BITS>;
-    constexpr uint32_t LANES = HD / 8, PER = 32 / LANES;
-    const uint32_t lane = threadIdx.x & 31, l = lane % LANES, kh = a.pool.d.kv_heads;
-    const uint64_t r = ((uint64_t)blockIdx.x * (ROW_THREADS / 32) + (threadIdx.x >> 5)) * PER + lane / LANES;
-    const bool live = r < (uint64_t)a.n_tok * 2 * kh;
-    const uint32_t t = live ? (uint32_t)(r / (2 * kh)) : 0, u = live ? (uint32_t)(r % (2 * kh)) : 0, value = u >= kh ? 1 : 0, head = u - value * kh;
-    pdl_wait();
-    pdl_trigger();
-    uint32_t row = 0;
-    uint8_t *block = live ? block_of(a.pool, __ldcg(a.slots + t), head, B::BYTES, row) : nullptr;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    const RowsArg &src = value ? a.v : a.k;
-    if (block != nullptr) rows_get8(src, t * src.token_stride + head * src.head_stride + l * 8, v);
-    transform8(v, signs8(a.pool, l * 8), lane);
+    constexpr uint32_t LANES = HD / 8;
     if (BITS == 8) {
-        int c[8];
+        uint32_t c[8];
         float scale;
         quantise8<LANES>(v, lane, c, scale);
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i / 4] |= (uint32_t)(c[i] + 128) << (i % 4 * 8);
         if (block == nullptr) return;
-        *reinterpret_cast<uint2 *>(block + value * B::V_AT + row_place<B::RB>(row, l * 8)) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2 *>(block + value * B::V_AT + row_place<B::RB>(row, l * 8)) =
+            make_uint2(four_bytes(c[0], c[1], c[2], c[3]) ^ 0x80808080u, four_bytes(c[4], c[5], c[6], c[7]) ^ 0x80808080u);
         if (l == 0) reinterpret_cast<float *>(block + (value ? B::VS_AT : B::KS_AT))[row] = scale;
     } else {
         float top = 0.0f;
@@ -92,9 +95,9 @@ template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_
         float rc[8], den = 0.0f, num = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float c = CENTROIDS[nearest(__fmul_rn(v[i], inv0))];
+            const float c = nearest_value(__fmul_rn(v[i], inv0));
             rc[i] = __fmul_rn(v[i], c);
-            den += c * c;                    // whole numbers below 2^24: in any order
+            den = __fmaf_rn(c, c, den);                    // whole numbers below 2^24: in any order
         }
 #pragma unroll
         for (int m = 4; m > 0; m >>= 1) den += __shfl_xor_sync(0xffffffffu, den, m);
@@ -118,38 +121,91 @@ template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_
     }
 }
 
-// Eight stored values of a row, element 8 l on, times their scale.
-template <int HD, int BITS> __device__ __forceinline__ void stored8(const uint8_t *block, uint32_t rows_at, uint32_t scales_at, uint32_t row, uint32_t l, float (&v)[8]) {
+template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_store_kernel(const __grid_constant__ PoolStoreArgs a) {
     using B = PoolBlock<HD, BITS>;
-    if (BITS == 8) {
-        const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(block + rows_at + row_place<B::RB>(row, l * 8)));
-        const float s = __ldcg(reinterpret_cast<const float *>(block + scales_at) + row);
+    constexpr uint32_t LANES = HD / 8, STEP = ROW_THREADS / LANES;
+    const uint32_t lane = threadIdx.x & 31, l = lane % LANES, signs = signs8(a.pool, l * 8), rows = a.n_tok * 2 * a.pool.d.kv_heads;
+    const uint32_t r0 = blockIdx.x * (STEP * ROW_AHEAD) + threadIdx.x / LANES;
+    pdl_wait();
+    pdl_trigger();
+    int64_t slot[ROW_AHEAD];
+    Row8 got[ROW_AHEAD];
+    RowAt at[ROW_AHEAD];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn((float)((int)(((i < 4 ? w.x : w.y) >> (i % 4 * 8)) & 255u) - 128), s);
-    } else {
-        const uint32_t w = __ldcg(reinterpret_cast<const uint32_t *>(block + rows_at + row_place<B::RB>(row, l * 4)));
-        const float s = bf16_bits_to_f32(__ldcg(reinterpret_cast<const uint16_t *>(block + scales_at) + row * B::G + l / 8));
+    for (uint32_t u = 0; u < ROW_AHEAD; ++u) {
+        const uint32_t r = r0 + u * STEP;
+        at[u] = row_at(a, min(r, rows - 1));
+        slot[u] = r < rows ? __ldcg(a.slots + at[u].t) : -1;
+        const RowsArg &src = at[u].value ? a.v : a.k;
+        got[u].ask(src, at[u].t * src.token_stride + at[u].head * src.head_stride + l * 8);
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(CENTROIDS[w >> (4 * i) & 15u], s);
+    for (uint32_t u = 0; u < ROW_AHEAD; ++u) {
+        if (r0 - threadIdx.x / LANES + u * STEP >= rows) break;          // all of the CTA
+        uint32_t row = 0;
+        uint8_t *block = block_of(a.pool, slot[u], at[u].head, B::BYTES, row);
+        float v[8];
+        got[u].values(a.k.type, v);
+        transform8(v, signs, lane);
+        put_row<HD, BITS>(a, block, row, at[u].value, l, lane, v);
     }
 }
 
+// N stored values of a row, element N l on, times their scale; l over HD / N lanes.
+template <int HD, int BITS, int N> struct Stored {
+    using B = PoolBlock<HD, BITS>;
+    static constexpr uint32_t BYTES = N * BITS / 8;
+    uint32_t w[BYTES > 4 ? 2 : 1], s;
+    __device__ __forceinline__ void get(const uint8_t *block, uint32_t rows_at, uint32_t scales_at, uint32_t row, uint32_t l) {
+        const uint8_t *p = block + rows_at + row_place<B::RB>(row, l * BYTES);
+        if constexpr (BYTES == 8) { const uint2 x = __ldcg(reinterpret_cast<const uint2 *>(p)); w[0] = x.x; w[1] = x.y; }
+        else if constexpr (BYTES == 4) w[0] = __ldcg(reinterpret_cast<const uint32_t *>(p));
+        else if constexpr (BYTES == 2) w[0] = __ldcg(reinterpret_cast<const uint16_t *>(p));
+        else w[0] = __ldcg(p);
+        if (BITS == 8) s = __ldcg(reinterpret_cast<const uint32_t *>(block + scales_at) + row);
+        else s = (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(block + scales_at) + row * B::G + l * N / 64) << 16;
+    }
+    __device__ __forceinline__ void values(const Expand &ex, float (&v)[N]) const {
+        const float scale = __uint_as_float(s);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __fmul_rn(signed_byte(BITS == 8 ? w[i / 4] : ex.centroids4(w[0] >> (i / 4 * 16)), i % 4), scale);
+    }
+};
+
 template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_load_kernel(const __grid_constant__ PoolStoreArgs a) {
     using B = PoolBlock<HD, BITS>;
-    constexpr uint32_t LANES = HD / 8, PER = 32 / LANES;
-    const uint32_t lane = threadIdx.x & 31, l = lane % LANES, kh = a.pool.d.kv_heads;
-    const uint64_t r = ((uint64_t)blockIdx.x * (ROW_THREADS / 32) + (threadIdx.x >> 5)) * PER + lane / LANES;
-    const bool live = r < (uint64_t)a.n_tok * 2 * kh;
-    const uint32_t t = live ? (uint32_t)(r / (2 * kh)) : 0, u = live ? (uint32_t)(r % (2 * kh)) : 0, value = u >= kh ? 1 : 0, head = u - value * kh;
+    constexpr uint32_t LANES = HD / 8, STEP = ROW_THREADS / LANES;
+    const uint32_t lane = threadIdx.x & 31, l = lane % LANES, signs = signs8(a.pool, l * 8), rows = a.n_tok * 2 * a.pool.d.kv_heads;
+    const uint32_t r0 = blockIdx.x * (STEP * ROW_AHEAD) + threadIdx.x / LANES;
+    const Expand ex;
     pdl_wait();
     pdl_trigger();
-    uint32_t row = 0;
-    const uint8_t *block = live ? block_of(a.pool, __ldcg(a.slots + t), head, B::BYTES, row) : nullptr;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (block != nullptr) stored8<HD, BITS>(block, value ? B::V_AT : 0, value ? B::VS_AT : B::KS_AT, row, l, v);
-    transform8_back(v, signs8(a.pool, l * 8), lane);
-    const RowsArg &dst = value ? a.v : a.k;
-    if (block != nullptr) rows_put8(dst, t * dst.token_stride + head * dst.head_stride + l * 8, v);
+    RowAt at[ROW_AHEAD];
+    int64_t slot[ROW_AHEAD];
+    Stored<HD, BITS, 8> got[ROW_AHEAD];
+    bool live[ROW_AHEAD];
+#pragma unroll
+    for (uint32_t u = 0; u < ROW_AHEAD; ++u) {
+        const uint32_t r = r0 + u * STEP;
+        at[u] = row_at(a, min(r, rows - 1));
+        slot[u] = r < rows ? __ldcg(a.slots + at[u].t) : -1;
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < ROW_AHEAD; ++u) {
+        uint32_t row = 0;
+        const uint8_t *block = block_of(a.pool, slot[u], at[u].head, B::BYTES, row);
+        live[u] = block != nullptr;
+        got[u].get(live[u] ? block : a.pool.rows, at[u].value ? B::V_AT : 0, at[u].value ? B::VS_AT : B::KS_AT, row, l);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < ROW_AHEAD; ++u) {
+        if (r0 - threadIdx.x / LANES + u * STEP >= rows) break;          // all of the CTA
+        float v[8];
+        got[u].values(ex, v);
+        transform8_back(v, signs, lane);
+        const RowsArg &dst = at[u].value ? a.v : a.k;
+        if (live[u]) rows_put8(dst, at[u].t * dst.token_stride + at[u].head * dst.head_stride + l * 8, v);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ block keys
@@ -157,11 +213,12 @@ template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_
 // token that writes a page's last row makes it.  A warp looks over 32 tokens of a head.
 template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_block_key_kernel(const __grid_constant__ PoolStoreArgs a) {
     using B = PoolBlock<HD, BITS>;
-    constexpr uint32_t LANES = HD / 8;
-    const uint32_t lane = threadIdx.x & 31, l = lane % LANES, kh = a.pool.d.kv_heads, pt = 1u << a.pool.d.page_shift;
+    constexpr int N = HD / 32, AHEAD = 16;
+    const uint32_t lane = threadIdx.x & 31, kh = a.pool.d.kv_heads, pt = 1u << a.pool.d.page_shift;
     const uint64_t w = (uint64_t)blockIdx.x * (ROW_THREADS / 32) + (threadIdx.x >> 5);
     const uint32_t head = (uint32_t)(w % kh);
     const uint64_t t = w / kh * 32 + lane;
+    const Expand ex;
     pdl_wait();
     pdl_trigger();
     const int64_t slot = t < a.n_tok ? __ldcg(a.slots + t) : -1;
@@ -169,24 +226,30 @@ template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_
     for (uint32_t todo = __ballot_sync(0xffffffffu, last); todo != 0; todo &= todo - 1) {
         const uint64_t page = (uint64_t)__shfl_sync(0xffffffffu, slot, __ffs(todo) - 1) >> a.pool.d.page_shift;
         const uint8_t *block = a.pool.rows + ((page * kh + head) << (a.pool.d.page_shift - 4)) * B::BYTES;
-        float sum[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 8
-        for (uint32_t i = 0; i < pt; ++i) {
-            float v[8];
-            stored8<HD, BITS>(block + (size_t)(i >> 4) * B::BYTES, 0, B::KS_AT, i & 15u, l, v);
+        float sum[N];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) sum[k] = __fadd_rn(sum[k], v[k]);
+        for (int k = 0; k < N; ++k) sum[k] = 0.0f;
+        for (uint32_t i = 0; i < pt; i += AHEAD, block += B::BYTES) {
+            Stored<HD, BITS, N> got[AHEAD];
+#pragma unroll
+            for (uint32_t j = 0; j < AHEAD; ++j) got[j].get(block, 0, B::KS_AT, j, lane);
+#pragma unroll
+            for (uint32_t j = 0; j < AHEAD; ++j) {
+                float v[N];
+                got[j].values(ex, v);
+#pragma unroll
+                for (int k = 0; k < N; ++k) sum[k] = __fadd_rn(sum[k], v[k]);
+            }
         }
         const float part = 1.0f / (float)pt;             // a power of two
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum[k] = __fmul_rn(sum[k], part);
-        int c[8];
+        for (int k = 0; k < N; ++k) sum[k] = __fmul_rn(sum[k], part);
+        uint32_t c[N];
         float scale;
-        quantise8<LANES>(sum, lane, c, scale);
-        uint32_t word[2] = {0, 0};
-#pragma unroll
-        for (int k = 0; k < 8; ++k) word[k / 4] |= ((uint32_t)c[k] & 255u) << (k % 4 * 8);
-        if (lane < LANES) *reinterpret_cast<uint2 *>(a.pool.block_keys + (page * kh + head) * HD + l * 8) = make_uint2(word[0], word[1]);
+        quantise8<32>(sum, lane, c, scale);
+        int8_t *to = a.pool.block_keys + (page * kh + head) * HD + lane * N;
+        if constexpr (N == 4) *reinterpret_cast<uint32_t *>(to) = four_bytes(c[0], c[1], c[2], c[3]);
+        else *reinterpret_cast<uint16_t *>(to) = (uint16_t)prmt(c[0], c[1], 0x0040u);
         if (lane == 0) a.pool.block_key_scales[page * kh + head] = scale;
     }
 }
@@ -194,7 +257,7 @@ template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_
 // ------------------------------------------------------------------------------------------------ choice of pages
 // CTA = (token, kv head).  The query is the sum of the head's queries, quantised as an 8-bit row; a page scores the whole-number product
 // with its block key times the key's scale (one rounding, so that scores are the same wherever they are computed).  The order of
-// scores is that of their bits as numbers; the highest `want` of them are found by four passes over their bytes, ties by index.
+// scores is that of their bits as numbers; the pages are those at or above a threshold, of its equals the first.
 // Two sizes of CTA: with few (token, kv head) pairs the time is one CTA's chain of loads, and 512 threads have a whole sequence's keys in
 // flight; with many, smaller CTAs have fewer threads idle at their barriers.
 __device__ __forceinline__ uint32_t ordered(float x) {           // NaN behind everything
@@ -207,7 +270,7 @@ template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_TH
     constexpr uint32_t SEL_WARPS = SEL_THREADS / 32;
     extern __shared__ uint32_t s_key[];
     __shared__ __align__(16) int8_t s_q[HD];
-    __shared__ uint32_t s_hist[256], s_warp[SEL_WARPS], s_pick[2];
+    __shared__ uint32_t s_warp[2][SEL_WARPS];
     const PoolShape &d = a.pool.d;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t = blockIdx.x / d.kv_heads, h = blockIdx.x % d.kv_heads, group = a.heads / d.kv_heads;
     pdl_wait();
@@ -261,23 +324,24 @@ template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_TH
         float v[8];
 #pragma unroll 1
         for (uint32_t g0 = 0; g0 < group; g0 += 8) {          // the sum in the order of the heads, eight of them on their way
-            float x[8][8];
+            Row8 x[8];
 #pragma unroll
             for (uint32_t g = 0; g < 8; ++g)
-                if (g0 + g < group) rows_get8(a.q, t * a.q.token_stride + (h * group + g0 + g) * a.q.head_stride + l * 8, x[g]);
+                if (g0 + g < group) x[g].ask(a.q, t * a.q.token_stride + (h * group + g0 + g) * a.q.head_stride + l * 8);
 #pragma unroll
             for (uint32_t g = 0; g < 8; ++g)
-                if (g0 + g < group)
+                if (g0 + g < group) {
+                    float y[8];
+                    x[g].values(a.q.type, y);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = g0 + g == 0 ? x[g][i] : __fadd_rn(v[i], x[g][i]);
+                    for (int i = 0; i < 8; ++i) v[i] = g0 + g == 0 ? y[i] : __fadd_rn(v[i], y[i]);
+                }
         }
         transform8(v, signs8(a.pool, l * 8), lane);
-        int c[8];
+        uint32_t c[8];
         float unused;
         quantise8<LANES>(v, lane, c, unused);
-        if (lane < LANES)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s_q[l * 8 + i] = (int8_t)c[i];
+        if (lane < LANES) *reinterpret_cast<uint2 *>(s_q + l * 8) = make_uint2(four_bytes(c[0], c[1], c[2], c[3]), four_bytes(c[4], c[5], c[6], c[7]));
     }
     __syncthreads();
     int q[W];
@@ -297,102 +361,117 @@ template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_TH
         }
     }
     __syncthreads();
-    const uint32_t m = to - from;
-    uint32_t want = a.top - a.sinks - a.local, prefix = 0;         // keys above `prefix` are in; of its equals the first `want`
-    if (want > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (uint32_t i = tid; i < 256; i += SEL_THREADS) s_hist[i] = 0;
-            __syncthreads();
-            const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-            for (uint32_t i = tid; i < m; i += SEL_THREADS)
-                if (((s_key[i] ^ prefix) & mask) == 0) atomicAdd(s_hist + (s_key[i] >> shift & 255u), 1u);
-            __syncthreads();
-            if (warp == 0) {              // the bin that holds the last one wanted, from the top
-                uint32_t sum = 0, mine[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) { mine[k] = s_hist[255 - (lane * 8 + k)]; sum += mine[k]; }
-                uint32_t upto = sum;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += x; }
-                uint32_t before = upto - sum;
-                if (before < want && want <= upto)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        if (before < want && want <= before + mine[k]) { s_pick[0] = 255 - (lane * 8 + k); s_pick[1] = want - before; }
-                        before += mine[k];
-                    }
-            }
-            __syncthreads();
-            prefix |= s_pick[0] << shift;
-            want = s_pick[1];
-            __syncthreads();
-        }
-    } else {
-        prefix = 0xFFFFFFFFu;             // above every score
-    }
-    // in the order of the pages: sinks, the chosen ones, the last ones
+    const uint32_t m = to - from, want = a.top - a.sinks - a.local;
     for (uint32_t i = tid; i < a.sinks; i += SEL_THREADS) out[i] = (int32_t)i;
     for (uint32_t i = tid; i < a.local; i += SEL_THREADS) out[a.top - a.local + i] = (int32_t)(to + i);
+    if (want == 0) return;
+    // The highest key that at least `want` keys reach, by halving the interval: a CTA-wide count a step, keys in registers where they are few.
+    constexpr uint32_t KEEP = 8;
+    const bool few = m <= KEEP * SEL_THREADS;
+    uint32_t mine[KEEP];
+#pragma unroll
+    for (uint32_t u = 0; u < KEEP; ++u) mine[u] = few && tid + u * SEL_THREADS < m ? s_key[tid + u * SEL_THREADS] : 0;
+    const uint32_t rounds = (m + SEL_THREADS - 1) / SEL_THREADS;
+    auto reach = [&](uint32_t bound, uint32_t step) {          // how many keys are `bound` or above; bound > 0
+        uint32_t c = 0;
+        if (few) {
+#pragma unroll
+            for (uint32_t u = 0; u < KEEP; ++u)
+                if (u < rounds) c += mine[u] >= bound ? 1u : 0u;
+        } else {
+            for (uint32_t i = tid; i < m; i += SEL_THREADS) c += s_key[i] >= bound ? 1u : 0u;
+        }
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (lane == 0) s_warp[step & 1u][warp] = c;
+        __syncthreads();
+        uint32_t all = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < SEL_WARPS; ++k) all += s_warp[step & 1u][k];
+        return all;
+    };
+    uint32_t low = 0, high = 0xFF800001u, above = 0, step = 0;          // low is reached by enough, high (behind +inf) by `above`, which is too few
+    bool exact = false;
+    while (high - low > 1) {
+        const uint32_t mid = low + (high - low) / 2, c = reach(mid, step++);
+        if (c < want) { high = mid; above = c; continue; }
+        low = mid;
+        if (c == want) { exact = true; break; }
+    }
+    // keys from `low` on, where they are too many the first of those that equal it; in the order of the pages
+    const uint32_t equals = exact ? 0xFFFFFFFFu : want - above;
     uint32_t done = a.sinks, equal = 0;
     for (uint32_t i0 = 0; i0 < m; i0 += SEL_THREADS) {
         const uint32_t i = i0 + tid, key = i < m ? s_key[i] : 0;
-        const bool is_equal = i < m && key == prefix;
-        // counts of equals before this one, then of takers: two scans over the CTA by ballots
-        const uint32_t e = __ballot_sync(0xffffffffu, is_equal);
-        if (lane == 0) s_warp[warp] = __popc(e);
-        __syncthreads();
-        uint32_t eq_before = equal, eq_all = 0;
-        for (uint32_t k = 0; k < SEL_WARPS; ++k) {
-            if (k < warp) eq_before += s_warp[k];
-            eq_all += s_warp[k];
+        const bool tie = !exact && i < m && key == low;
+        uint32_t eq_before = equal;
+        if (!exact) {
+            const uint32_t e = __ballot_sync(0xffffffffu, tie);
+            if (lane == 0) s_warp[step & 1u][warp] = __popc(e);
+            __syncthreads();
+            for (uint32_t k = 0; k < SEL_WARPS; ++k) {
+                if (k < warp) eq_before += s_warp[step & 1u][k];
+                equal += s_warp[step & 1u][k];
+            }
+            eq_before += __popc(e & ((1u << lane) - 1u));
+            ++step;
         }
-        eq_before += __popc(e & ((1u << lane) - 1u));
-        __syncthreads();
-        const bool take = i < m && (key > prefix || (is_equal && eq_before < want));
+        const bool take = i < m && key >= low && (!tie || eq_before < equals);
         const uint32_t b = __ballot_sync(0xffffffffu, take);
-        if (lane == 0) s_warp[warp] = __popc(b);
+        if (lane == 0) s_warp[step & 1u][warp] = __popc(b);
         __syncthreads();
-        uint32_t at = done, all = 0;
+        uint32_t at = done;
         for (uint32_t k = 0; k < SEL_WARPS; ++k) {
-            if (k < warp) at += s_warp[k];
-            all += s_warp[k];
+            if (k < warp) at += s_warp[step & 1u][k];
+            done += s_warp[step & 1u][k];
         }
+        ++step;
         at += __popc(b & ((1u << lane) - 1u));
         if (take) out[at] = (int32_t)(from + i);
-        __syncthreads();
-        done += all;
-        equal += eq_all;
     }
 }
 
+uint32_t row_ctas(const PoolStoreArgs &a) {
+    const uint32_t per = ROW_THREADS * 8 / a.pool.d.head_dim * ROW_AHEAD;
+    return (uint32_t)(((uint64_t)a.n_tok * 2 * a.pool.d.kv_heads + per - 1) / per);
+}
+// r / (2 kv heads) for r below 2^31
+PoolStoreArgs divided(PoolStoreArgs a) {
+    const uint32_t per = 2 * a.pool.d.kv_heads;
+    uint32_t bits = 1;
+    while ((1u << bits) < per) ++bits;
+    a.rows_mul = (uint32_t)(((1ull << (31 + bits)) + per - 1) / per);
+    a.rows_shift = bits - 1;
+    return a;
+}
 template <int HD, int BITS> cudaError_t store_rows(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched) {
-    const uint64_t rows = (uint64_t)a.n_tok * 2 * a.pool.d.kv_heads, per = ROW_THREADS * 8 / HD, warps = ((uint64_t)a.n_tok + 31) / 32 * a.pool.d.kv_heads;
     *launched += 1;
-    const cudaError_t e = launch_kernel(pool_store_kernel<HD, BITS>, dim3((unsigned)((rows + per - 1) / per)), dim3(ROW_THREADS), 0, s, true, a);
+    const cudaError_t e = launch_kernel(pool_store_kernel<HD, BITS>, dim3(row_ctas(a)), dim3(ROW_THREADS), 0, s, true, a);
     if (e != cudaSuccess || !a.pool.d.block_keys) return e;
+    const uint64_t warps = ((uint64_t)a.n_tok + 31) / 32 * a.pool.d.kv_heads;
     *launched += 1;
     return launch_kernel(pool_block_key_kernel<HD, BITS>, dim3((unsigned)((warps + ROW_THREADS / 32 - 1) / (ROW_THREADS / 32))), dim3(ROW_THREADS), 0, s, true, a);
 }
 template <int HD, int BITS> cudaError_t load_rows(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched) {
-    const uint64_t rows = (uint64_t)a.n_tok * 2 * a.pool.d.kv_heads, per = ROW_THREADS * 8 / HD;
     *launched += 1;
-    return launch_kernel(pool_load_kernel<HD, BITS>, dim3((unsigned)((rows + per - 1) / per)), dim3(ROW_THREADS), 0, s, true, a);
+    return launch_kernel(pool_load_kernel<HD, BITS>, dim3(row_ctas(a)), dim3(ROW_THREADS), 0, s, true, a);
 }
 
 }  // namespace
 
-cudaError_t launch_pool_store(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched) {
+cudaError_t launch_pool_store(cudaStream_t s, const PoolStoreArgs &args, uint32_t *launched) {
+    const PoolStoreArgs a = divided(args);
     const bool wide = a.pool.d.head_dim == 128, b8 = a.pool.d.bits == 8;
     return wide ? (b8 ? store_rows<128, 8>(s, a, launched) : store_rows<128, 4>(s, a, launched)) : b8 ? store_rows<64, 8>(s, a, launched) : store_rows<64, 4>(s, a, launched);
 }
-cudaError_t launch_pool_load(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched) {
+cudaError_t launch_pool_load(cudaStream_t s, const PoolStoreArgs &args, uint32_t *launched) {
+    const PoolStoreArgs a = divided(args);
     const bool wide = a.pool.d.head_dim == 128, b8 = a.pool.d.bits == 8;
     return wide ? (b8 ? load_rows<128, 8>(s, a, launched) : load_rows<128, 4>(s, a, launched)) : b8 ? load_rows<64, 8>(s, a, launched) : load_rows<64, 4>(s, a, launched);
 }
 cudaError_t launch_pool_select(cudaStream_t s, const PoolAttnArgs &a, uint32_t *launched) {
     const size_t smem = (size_t)a.pages_stride * 4;
     const uint32_t pairs = a.n_tok * a.pool.d.kv_heads;
-    const bool small = pairs >= 4 * a.sm_count && a.pages_stride <= 4096;
+    const bool small = pairs >= 4 * a.sm_count && a.pages_stride <= 1024;
     const auto kernel = a.pool.d.head_dim == 128 ? (small ? pool_select_kernel<128, 128> : pool_select_kernel<128, 512>) : small ? pool_select_kernel<64, 128> : pool_select_kernel<64, 512>;
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;

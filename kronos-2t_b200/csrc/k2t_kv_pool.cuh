@@ -40,34 +40,45 @@ __device__ __forceinline__ uint32_t pack2(uint32_t type, float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-// Eight consecutive elements from / to element `at` of rows.
-__device__ __forceinline__ void rows_get8(const RowsArg &a, size_t at, float (&v)[8]) {
-    if (a.type == TYPE_F32) {
-        const float *p = static_cast<const float *>(a.p) + at;
+// Eight consecutive elements from / to element `at` of rows.  Asking and converting are apart, so that several rows can be on their way: a
+// conversion inside the branches on the type would wait for each.
+struct Row8 {
+    uint32_t w[8];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ void ask(const RowsArg &a, size_t at) {
+        const uint8_t *p = static_cast<const uint8_t *>(a.p) + at * (a.type == TYPE_F32 ? 4 : 2);
         if (a.wide) {
-            const float4 x = __ldcg(reinterpret_cast<const float4 *>(p)), y = __ldcg(reinterpret_cast<const float4 *>(p) + 1);
-            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+            const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(p));
+            w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+            if (a.type == TYPE_F32) {
+                const uint4 y = __ldcg(reinterpret_cast<const uint4 *>(p) + 1);
+                w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+            }
+        } else if (a.type == TYPE_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __ldcg(reinterpret_cast<const uint32_t *>(p) + i);
         } else {
+            const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __ldcg(p + i);
+            for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldcg(q + 2 * i) | ((uint32_t)__ldcg(q + 2 * i + 1) << 16);
         }
-        return;
     }
-    const uint16_t *p = static_cast<const uint16_t *>(a.p) + at;
-    uint32_t w[4];
-    if (a.wide) {
-        const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(p));
-        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-    } else {
+    __device__ __forceinline__ void values(uint32_t type, float (&v)[8]) const {
+        if (type == TYPE_F32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldcg(p + 2 * i) | ((uint32_t)__ldcg(p + 2 * i + 1) << 16);
-    }
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+            return;
+        }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2(a.type, w[i]);
-        v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2(type, w[i]);
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        }
     }
-}
+};
 __device__ __forceinline__ void rows_put8(const RowsArg &a, size_t at, const float (&v)[8]) {
     if (a.type == TYPE_F32) {
         float *p = static_cast<float *>(a.p) + at;
@@ -157,7 +168,7 @@ struct Expand {
     __device__ __forceinline__ uint32_t halves_hi(uint32_t x) const { return hsub2(prmt(x, exponent, 0x4342u), 0x64806480u); }
     // Four 4-bit codes (the low 16 bits of w) as bytes 128 + centroid.  A selector with bit 3 set yields a byte's sign, here 0: of the two
     // tables each index finds its magnitude in one and 0 in the other.
-    __device__ __forceinline__ uint32_t centroids4(uint32_t w) const { return (prmt(hi0, hi1, w ^ 0x8888u) | 0x80808080u) - prmt(lo0, lo1, w); }
+    __device__ __forceinline__ uint32_t centroids4(uint32_t w) const { return 0x80808080u + prmt(hi0, hi1, w ^ 0x8888u) - prmt(lo0, lo1, w); }
 };
 
 constexpr uint32_t POOL_ERR_PAGE = 6;        // a page or slot outside the pool

@@ -43,7 +43,8 @@ struct PoolStoreArgs {
     PoolView pool;
     RowsArg k, v;
     const int64_t *slots;
-    uint32_t n_tok;
+    uint32_t n_tok;              // times 2 kv heads: below 2^31
+    uint32_t rows_mul, rows_shift;
 };
 cudaError_t launch_pool_store(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched);
 cudaError_t launch_pool_load(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched);

@@ -193,8 +193,11 @@ template <int HD, int QT, int NR> __device__ __forceinline__ void put_queries(co
         const uint32_t row = row0 + tid / LANES;
         if (row0 + (tid & ~31u) / LANES >= 8 * NR) break;          // whole warps
         uint32_t t, head;
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, top = 0.0f;
-        if (item_row(p, it, row, t, head)) rows_get8(p.a.q, t * p.a.q.token_stride + head * p.a.q.head_stride + l * 8, v);
+        float v[8], top = 0.0f;
+        Row8 x;
+        x.clear();
+        if (item_row(p, it, row, t, head)) x.ask(p.a.q, t * p.a.q.token_stride + head * p.a.q.head_stride + l * 8);
+        x.values(p.a.q.type, v);
         transform8(v, signs, lane);
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
@@ -206,10 +209,10 @@ template <int HD, int QT, int NR> __device__ __forceinline__ void put_queries(co
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float x = v[2 * i] * up, y = v[2 * i + 1] * up;
-            hi[i] = half2_bits(x, y);
+            const float y = v[2 * i] * up, z = v[2 * i + 1] * up;
+            hi[i] = half2_bits(y, z);
             const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
-            lo[i] = half2_bits(x - f.x, y - f.y);
+            lo[i] = half2_bits(y - f.x, z - f.y);
         }
         uint4 *to = reinterpret_cast<uint4 *>(s_query + row * QT * HD * 2) + (l ^ (row & 7u));
         to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);

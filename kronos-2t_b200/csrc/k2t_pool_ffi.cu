@@ -130,8 +130,8 @@ int32_t move_rows(KronosCudaContext *ctx, KronosCudaKvPool *pool, uint32_t type,
     PoolStoreArgs a{};
     std::string why;
     if (!k || !v) return fail(ctx, "kv_pool: NULL rows"), -1;
-    if (n_tok > (1u << 24)) return fail(ctx, "kv_pool: too many tokens"), -1;
     const PoolShape &d = pool->view.d;
+    if (n_tok > (1u << 24) || n_tok * 2 * d.kv_heads >= 1ull << 31) return fail(ctx, "kv_pool: too many tokens"), -1;
     if (!pool_rows(d, type, d.kv_heads, n_tok, *k, "k", load, a.k, why) || !pool_rows(d, type, d.kv_heads, n_tok, *v, "v", load, a.v, why)) return fail(ctx, why), -1;
     if (n_tok == 0) return 0;
     if (!slots) return fail(ctx, "kv_pool: NULL slots"), -1;

@@ -206,20 +206,20 @@ template <int HD, int BITS, int QT> __device__ __forceinline__ void flash_querie
     constexpr uint32_t AHEAD = 4;              // rows of a lane on their way together
 #pragma unroll 1
     for (uint32_t i0 = 0; i0 < mine; i0 += ROWS * AHEAD) {
-        float ahead[AHEAD][8];
+        Row8 ahead[AHEAD];
 #pragma unroll
         for (uint32_t u = 0; u < AHEAD; ++u) {
             const uint32_t r = r0 + warp * mine + i0 + u * ROWS + lane / LANES;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) ahead[u][k] = 0.0f;
-            if (i0 + u * ROWS < mine && r < all) rows_get8(p.a.q, r / group * p.a.q.token_stride + (h * group + r % group) * p.a.q.head_stride + l * 8, ahead[u]);
+            ahead[u].clear();
+            if (i0 + u * ROWS < mine && r < all) ahead[u].ask(p.a.q, r / group * p.a.q.token_stride + (h * group + r % group) * p.a.q.head_stride + l * 8);
         }
 #pragma unroll
         for (uint32_t u = 0; u < AHEAD; ++u) {
         const uint32_t i = i0 + u * ROWS;
         if (i >= mine) break;
         const uint32_t row = warp * mine + i + lane / LANES;
-        float (&v)[8] = ahead[u], top = 0.0f;
+        float v[8], top = 0.0f;
+        ahead[u].values(p.a.q.type, v);
         transform8(v, signs, lane);
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
