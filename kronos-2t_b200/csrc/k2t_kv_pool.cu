@@ -8,16 +8,25 @@
 namespace k2t {
 namespace {
 
-// The nearest of the 16 centroids: its index, and its value (borders halfway between the magnitudes).
-__device__ __forceinline__ uint32_t nearest(float y) {
-    const float a = fabsf(y);
-    const uint32_t p = a < 37.5f ? (a < 12.0f ? 0u : a < 24.5f ? 1u : 2u) : a < 85.5f ? (a < 51.0f ? 3u : a < 66.5f ? 4u : 5u) : a < 111.5f ? 6u : 7u;
-    return y >= 0.0f ? 8u + p : 7u - p;
-}
+// The nearest of the 16 centroids.  The magnitude is a sum of steps at the borders between magnitudes: a comparison that yields 1.0 or 0.0 and a
+// fused multiply-add each, on two pipes, where a tree of selections keeps one busy twice as long.
+__device__ __forceinline__ float at_least(float a, float border) { float s; asm("set.ge.f32.f32 %0, %1, %2;" : "=f"(s) : "f"(a), "f"(border)); return s; }
+__device__ __forceinline__ float with_sign(float x, float of) { return __uint_as_float(__float_as_uint(x) | (__float_as_uint(of) & 0x80000000u)); }          // x >= 0
 __device__ __forceinline__ float nearest_value(float y) {
     const float a = fabsf(y);
-    const float c = a < 37.5f ? (a < 12.0f ? 6.0f : a < 24.5f ? 18.0f : 31.0f) : a < 85.5f ? (a < 51.0f ? 44.0f : a < 66.5f ? 58.0f : 75.0f) : a < 111.5f ? 96.0f : 127.0f;
-    return y >= 0.0f ? c : -c;
+    float c = __fmaf_rn(at_least(a, 12.0f), 12.0f, 6.0f);
+    c = __fmaf_rn(at_least(a, 24.5f), 13.0f, c);
+    c = __fmaf_rn(at_least(a, 37.5f), 13.0f, c);
+    c = __fmaf_rn(at_least(a, 51.0f), 14.0f, c);
+    c = __fmaf_rn(at_least(a, 66.5f), 17.0f, c);
+    c = __fmaf_rn(at_least(a, 85.5f), 21.0f, c);
+    c = __fmaf_rn(at_least(a, 111.5f), 31.0f, c);
+    return with_sign(c, __fadd_rn(y, 0.0f));          // + 0 takes the sign of -0
+}
+__device__ __forceinline__ float nearest_index(float y) {          // 0 .. 15
+    const float a = fabsf(y);
+    const float low = __fadd_rn(__fadd_rn(at_least(a, 12.0f), at_least(a, 24.5f)), at_least(a, 37.5f)), high = __fadd_rn(__fadd_rn(at_least(a, 51.0f), at_least(a, 66.5f)), __fadd_rn(at_least(a, 85.5f), at_least(a, 111.5f)));
+    return __fadd_rn(7.5f, with_sign(__fadd_rn(__fadd_rn(low, 0.5f), high), __fadd_rn(y, 0.0f)));
 }
 constexpr float SMALLEST = 1.1920929e-07f;       // 8-bit rows up to here are stored as zeros
 // Rounded to the nearest whole number, the even one of two: the low byte of the result.  |x| <= 2^22.
@@ -112,9 +121,15 @@ template <int HD, int BITS> __device__ __forceinline__ void put_row(const PoolSt
         const float fit = den > 1e-12f && num > 0.0f ? __fdiv_rn(num, den) : __fdiv_rn(top, 127.0f);
         const __nv_bfloat16 sb = __float2bfloat16_rn(zero ? 0.0f : fit);
         const float s = __bfloat162float(sb), inv = s > 1e-30f ? __fdiv_rn(1.0f, s) : 0.0f;
-        uint32_t w = 0;
+        uint32_t half[2];                      // four indices each as one whole number below 2^16
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w |= (zero ? 8u : nearest(__fmul_rn(v[i], inv))) << (4 * i);
+        for (int i = 0; i < 2; ++i) {
+            float n = nearest_index(__fmul_rn(v[4 * i + 3], inv));
+#pragma unroll
+            for (int j = 2; j >= 0; --j) n = __fmaf_rn(n, 16.0f, nearest_index(__fmul_rn(v[4 * i + j], inv)));
+            half[i] = __float_as_uint(__fadd_rn(n, 8388608.0f));
+        }
+        const uint32_t w = zero ? 0x88888888u : prmt(half[0], half[1], 0x5410u);
         if (block == nullptr) return;
         *reinterpret_cast<uint32_t *>(block + value * B::V_AT + row_place<B::RB>(row, l * 4)) = w;
         if (l % 8 == 0) reinterpret_cast<uint16_t *>(block + (value ? B::VS_AT : B::KS_AT))[row * B::G + l / 8] = bad ? 0x7FC0u : __bfloat16_as_ushort(sb);
@@ -257,7 +272,7 @@ template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_
 // ------------------------------------------------------------------------------------------------ choice of pages
 // CTA = (token, kv head).  The query is the sum of the head's queries, quantised as an 8-bit row; a page scores the whole-number product
 // with its block key times the key's scale (one rounding, so that scores are the same wherever they are computed).  The order of
-// scores is that of their bits as numbers; the pages are those at or above a threshold, of its equals the first.
+// scores is that of their bits as numbers; the pages are those at or above a threshold (found byte by byte), of its equals the first.
 // Two sizes of CTA: with few (token, kv head) pairs the time is one CTA's chain of loads, and 512 threads have a whole sequence's keys in
 // flight; with many, smaller CTAs have fewer threads idle at their barriers.
 __device__ __forceinline__ uint32_t ordered(float x) {           // NaN behind everything
@@ -266,11 +281,12 @@ __device__ __forceinline__ uint32_t ordered(float x) {           // NaN behind e
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_THREADS) pool_select_kernel(const __grid_constant__ PoolAttnArgs a) {
+template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_THREADS, 2048 / SEL_THREADS / 2) pool_select_kernel(const __grid_constant__ PoolAttnArgs a) {
     constexpr uint32_t SEL_WARPS = SEL_THREADS / 32;
     extern __shared__ uint32_t s_key[];
     __shared__ __align__(16) int8_t s_q[HD];
-    __shared__ uint32_t s_warp[2][SEL_WARPS];
+    __shared__ uint32_t s_warp[2][SEL_WARPS], s_hist[256], s_pick[3];
+    __shared__ float s_rows[SEL_WARPS][HD], s_sum[HD];
     const PoolShape &d = a.pool.d;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t = blockIdx.x / d.kv_heads, h = blockIdx.x % d.kv_heads, group = a.heads / d.kv_heads;
     pdl_wait();
@@ -318,25 +334,31 @@ template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_TH
         }
     };
     ask(from + warp * 4);
-    if (warp == SEL_WARPS - 1) {
+    // the head's queries, a warp each, to shared memory; their sum in the order of the heads
+    for (uint32_t g0 = 0; g0 < group; g0 += SEL_WARPS) {
+        if (g0 > 0) __syncthreads();
+        if (g0 + warp < group && lane < HD / 8) {
+            Row8 x;
+            float y[8];
+            x.ask(a.q, t * a.q.token_stride + (h * group + g0 + warp) * a.q.head_stride + lane * 8);
+            x.values(a.q.type, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s_rows[warp][lane * 8 + i] = y[i];
+        }
+        __syncthreads();
+        if (tid < HD) {
+            float v = g0 == 0 ? s_rows[0][tid] : __fadd_rn(s_sum[tid], s_rows[0][tid]);
+            for (uint32_t g = 1; g < min(SEL_WARPS, group - g0); ++g) v = __fadd_rn(v, s_rows[g][tid]);
+            s_sum[tid] = v;
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {
         constexpr uint32_t LANES = HD / 8;
         const uint32_t l = lane % LANES;
         float v[8];
-#pragma unroll 1
-        for (uint32_t g0 = 0; g0 < group; g0 += 8) {          // the sum in the order of the heads, eight of them on their way
-            Row8 x[8];
 #pragma unroll
-            for (uint32_t g = 0; g < 8; ++g)
-                if (g0 + g < group) x[g].ask(a.q, t * a.q.token_stride + (h * group + g0 + g) * a.q.head_stride + l * 8);
-#pragma unroll
-            for (uint32_t g = 0; g < 8; ++g)
-                if (g0 + g < group) {
-                    float y[8];
-                    x[g].values(a.q.type, y);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = g0 + g == 0 ? y[i] : __fadd_rn(v[i], y[i]);
-                }
-        }
+        for (int i = 0; i < 8; ++i) v[i] = s_sum[l * 8 + i];
         transform8(v, signs8(a.pool, l * 8), lane);
         uint32_t c[8];
         float unused;
@@ -361,50 +383,47 @@ template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_TH
         }
     }
     __syncthreads();
-    const uint32_t m = to - from, want = a.top - a.sinks - a.local;
+    const uint32_t m = to - from;
+    uint32_t want = a.top - a.sinks - a.local, low = 0;          // keys above `low` are in; of its equals the first `want`
     for (uint32_t i = tid; i < a.sinks; i += SEL_THREADS) out[i] = (int32_t)i;
     for (uint32_t i = tid; i < a.local; i += SEL_THREADS) out[a.top - a.local + i] = (int32_t)(to + i);
     if (want == 0) return;
-    // The highest key that at least `want` keys reach, by halving the interval: a CTA-wide count a step, keys in registers where they are few.
-    constexpr uint32_t KEEP = 8;
-    const bool few = m <= KEEP * SEL_THREADS;
-    uint32_t mine[KEEP];
-#pragma unroll
-    for (uint32_t u = 0; u < KEEP; ++u) mine[u] = few && tid + u * SEL_THREADS < m ? s_key[tid + u * SEL_THREADS] : 0;
-    const uint32_t rounds = (m + SEL_THREADS - 1) / SEL_THREADS;
-    auto reach = [&](uint32_t bound, uint32_t step) {          // how many keys are `bound` or above; bound > 0
-        uint32_t c = 0;
-        if (few) {
-#pragma unroll
-            for (uint32_t u = 0; u < KEEP; ++u)
-                if (u < rounds) c += mine[u] >= bound ? 1u : 0u;
-        } else {
-            for (uint32_t i = tid; i < m; i += SEL_THREADS) c += s_key[i] >= bound ? 1u : 0u;
-        }
-        c = __reduce_add_sync(0xffffffffu, c);
-        if (lane == 0) s_warp[step & 1u][warp] = c;
+#pragma unroll 1
+    for (int shift = 24; shift >= 0; shift -= 8) {               // byte by byte the key that is the last one wanted
+        for (uint32_t i = tid; i < 256; i += SEL_THREADS) s_hist[i] = 0;
         __syncthreads();
-        uint32_t all = 0;
+        const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
+        for (uint32_t i = tid; i < m; i += SEL_THREADS)
+            if (((s_key[i] ^ low) & mask) == 0) atomicAdd(s_hist + (s_key[i] >> shift & 255u), 1u);
+        __syncthreads();
+        if (warp == 0) {              // the bin that holds it, from the top
+            uint32_t sum = 0, mine[8];
 #pragma unroll
-        for (uint32_t k = 0; k < SEL_WARPS; ++k) all += s_warp[step & 1u][k];
-        return all;
-    };
-    uint32_t low = 0, high = 0xFF800001u, above = 0, step = 0;          // low is reached by enough, high (behind +inf) by `above`, which is too few
-    bool exact = false;
-    while (high - low > 1) {
-        const uint32_t mid = low + (high - low) / 2, c = reach(mid, step++);
-        if (c < want) { high = mid; above = c; continue; }
-        low = mid;
-        if (c == want) { exact = true; break; }
+            for (int k = 0; k < 8; ++k) { mine[k] = s_hist[255 - (lane * 8 + k)]; sum += mine[k]; }
+            uint32_t upto = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= (uint32_t)o) upto += x; }
+            uint32_t before = upto - sum;
+            if (before < want && want <= upto)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (before < want && want <= before + mine[k]) { s_pick[0] = 255 - (lane * 8 + k); s_pick[1] = want - before; s_pick[2] = mine[k]; }
+                    before += mine[k];
+                }
+        }
+        __syncthreads();
+        low |= s_pick[0] << shift;
+        want = s_pick[1];
+        if (want == s_pick[2]) break;          // the whole bin: everything from its lowest key on
     }
-    // keys from `low` on, where they are too many the first of those that equal it; in the order of the pages
-    const uint32_t equals = exact ? 0xFFFFFFFFu : want - above;
-    uint32_t done = a.sinks, equal = 0;
+    // in the order of the pages: two scans over the CTA by ballots a stretch
+    const bool all_equal = want == s_pick[2];
+    uint32_t done = a.sinks, equal = 0, step = 0;
     for (uint32_t i0 = 0; i0 < m; i0 += SEL_THREADS) {
         const uint32_t i = i0 + tid, key = i < m ? s_key[i] : 0;
-        const bool tie = !exact && i < m && key == low;
+        const bool tie = !all_equal && i < m && key == low;
         uint32_t eq_before = equal;
-        if (!exact) {
+        if (!all_equal) {
             const uint32_t e = __ballot_sync(0xffffffffu, tie);
             if (lane == 0) s_warp[step & 1u][warp] = __popc(e);
             __syncthreads();
@@ -415,7 +434,7 @@ template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_TH
             eq_before += __popc(e & ((1u << lane) - 1u));
             ++step;
         }
-        const bool take = i < m && key >= low && (!tie || eq_before < equals);
+        const bool take = i < m && key >= low && (!tie || eq_before < want);
         const uint32_t b = __ballot_sync(0xffffffffu, take);
         if (lane == 0) s_warp[step & 1u][warp] = __popc(b);
         __syncthreads();
@@ -471,7 +490,7 @@ cudaError_t launch_pool_load(cudaStream_t s, const PoolStoreArgs &args, uint32_t
 cudaError_t launch_pool_select(cudaStream_t s, const PoolAttnArgs &a, uint32_t *launched) {
     const size_t smem = (size_t)a.pages_stride * 4;
     const uint32_t pairs = a.n_tok * a.pool.d.kv_heads;
-    const bool small = pairs >= 4 * a.sm_count && a.pages_stride <= 1024;
+    const bool small = pairs >= 4 * a.sm_count && a.pages_stride <= 4096;
     const auto kernel = a.pool.d.head_dim == 128 ? (small ? pool_select_kernel<128, 128> : pool_select_kernel<128, 512>) : small ? pool_select_kernel<64, 128> : pool_select_kernel<64, 512>;
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;
