@@ -12,6 +12,7 @@
 // long sequence alike keep every CTA busy to the end.  An item that lies in one part is finished there; the others leave partial
 // results, which pool_merge_kernel joins.
 #include <algorithm>
+#include <cstdlib>
 
 #include "k2t_flash_tc.cuh"
 #include "k2t_kv_pool.cuh"
@@ -459,16 +460,21 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, BITS, QT == 2, P
     }
     Item it;
     uint32_t left;                             // blocks of the CTA's part
-    if (p.direct) {             // the part is one item, which may hold no block at all
-        const uint32_t per = d.kv_heads * p.rbo;
+    if (p.pieces != 0) {             // the part is a piece of one item, which may hold no block at all
+        const uint32_t per = d.kv_heads * p.rbo, item = unit / p.pieces, piece = unit % p.pieces;
         it.prefix = false;
-        it.index = unit;
-        it.t = unit / per;
-        it.h = unit % per / p.rbo;
-        it.rb = unit % p.rbo;
-        it.next = 0;
+        it.index = item;
+        it.t = item / per;
+        it.h = item % per / p.rbo;
+        it.rb = item % p.rbo;
         item_fill(p, it);
-        left = it.blocks;
+        const uint32_t part = piece_blocks(p, it.blocks);
+        it.next = min(it.blocks, piece * part);
+        left = min(it.blocks - it.next, part);
+        if (piece > 0 && left == 0) {          // fewer blocks than pieces; the first one stands for an item without any
+            if (behind) pdl_wait();
+            return;
+        }
     } else {
         const uint64_t all = prefix_line(p) + warp_total(p, lane) * d.kv_heads * p.rbo, part = part_blocks(all, p.units), x = (uint64_t)unit * part;
         if (x >= all) {
@@ -632,8 +638,10 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
     uint32_t near_first = 0, near_n = 0, near_item = 0, own_first = 0, own_n = 0;
     const uint32_t own_item = (t * kh + h) * p.rbo + in / p.tile, r = t * group + in;
     const uint64_t mine = item_blocks(p, t);
-    if (p.direct) {
-        own_n = mine > 0 ? 1 : 0;
+    if (p.pieces != 0) {
+        const uint32_t part = piece_blocks(p, (uint32_t)mine);
+        own_first = 0;
+        own_n = mine > 0 ? (uint32_t)((mine + part - 1) / part) : 0;
     } else {
         uint64_t total, before;
         if (p.a.chosen != nullptr) {
@@ -677,7 +685,8 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
         near_first = b / f.part;
         near_n = ((e - 1) / f.part + 1 - near_first) << (f.halved ? 1 : 0);
     }
-    const bool finished = own_n == 1 && p.a.prefix_len == 0;
+    // an item without a block has one piece all the same, which has written its zeros
+    const bool finished = p.a.prefix_len == 0 && (own_n == 1 || (p.pieces != 0 && own_n == 0));
     const uint32_t n = finished ? 0 : near_n + own_n;
     auto slot = [&](uint32_t i, uint32_t &row, uint32_t &rows) -> const float * {
         const bool near = i < near_n;
@@ -689,7 +698,7 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
         }
         row = (near ? r : in) % p.tile;
         rows = p.slot_rows(near);
-        return near ? p.slot(true, near_first + i, near_item) : p.slot(false, own_first + i - near_n, own_item);
+        return near ? p.slot(true, near_first + i, near_item) : p.slot(false, (p.pieces != 0 ? own_item * p.pieces : own_first) + i - near_n, own_item);
     };
     float top = -INFINITY;
     for (uint32_t i = lane; i < n; i += 32) {
@@ -742,15 +751,18 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-// One CTA per item where there are several items for every CTA that the SMs hold: their ends then overlap anyway, and nothing has to
-// be looked up or joined.
+// A line of blocks in equal parts, or items in equal pieces, one a CTA?  Chosen pages: items are of one length, so pieces of them are as equal
+// as parts and begin no second item.  Tables: a line, since lengths are ragged, but one CTA per item (nothing to look up, nothing to join)
+// where no item can be longer than a CTA's start (SHORT blocks), or where there are several for every CTA that the SMs hold.
+constexpr uint32_t SHORT = 32;
 SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     SplitArgs p{};
     p.a = a;
     const PoolShape &d = a.pool.d;
     const uint32_t group = a.heads / d.kv_heads;
     const uint32_t rows = a.n_tok * group;
-    p.flash.on = a.prefix_len > 0 && rows > 16;          // more than one tile of this kernel: k2t_pool_flash.cu
+    static const char *dbg = getenv("POOL_FLASH");
+    p.flash.on = a.prefix_len > 0 && rows > (dbg ? (uint32_t)atoi(dbg) : 16);          // more than one tile of this kernel: k2t_pool_flash.cu
     if (p.flash.on) {
         FlashArgs &f = p.flash;
         f.halved = rows <= FLASH_ROWS;
@@ -764,11 +776,16 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     p.rbo = (group + p.tile - 1) / p.tile;
     p.rbp = near ? (rows + p.tile - 1) / p.tile : 0;
     const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * p.rbo, room = (uint64_t)a.sm_count * split_ctas(d.head_dim, d.bits, type != TYPE_BF16, type == TYPE_F32, p.tile / 8);
-    p.direct = p.rbp == 0 && items >= 3 * room;
-    p.units = (uint32_t)(p.direct ? items : room);
+    if (a.chosen != nullptr) {
+        const uint64_t blocks = (uint64_t)a.top << (d.page_shift - 4);
+        p.pieces = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(room / items, blocks / MIN_PART));
+    } else if (p.rbp == 0 && (items >= 3 * room || (items <= room && ((uint64_t)a.pages_stride << (d.page_shift - 4)) <= SHORT))) {
+        p.pieces = 1;
+    }
+    p.units = (uint32_t)(p.pieces != 0 ? items * p.pieces : room);
     return p;
 }
-size_t own_slots(const SplitArgs &p) { return p.direct ? p.units : p.units + (size_t)p.a.n_tok * p.a.pool.d.kv_heads * p.rbo; }
+size_t own_slots(const SplitArgs &p) { return p.units + (p.pieces != 0 ? 0 : (size_t)p.a.n_tok * p.a.pool.d.kv_heads * p.rbo); }
 size_t near_floats(const SplitArgs &p) {
     if (p.flash.on) return ((size_t)p.a.sm_count + p.flash.items) * flash_slot_floats(p.a.pool.d.head_dim);
     return p.rbp == 0 ? 0 : (p.units + (size_t)p.a.pool.d.kv_heads * p.rbp) * p.slot_floats(true);
@@ -791,6 +808,7 @@ template <int HD, int BITS> cudaError_t split_launch(cudaStream_t s, const Split
 
 }  // namespace
 
+// Room for a call of these sizes whatever its table's width and choice: as many pieces or parts as there can be.
 size_t pool_work_bytes(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint32_t prefix_len, uint32_t sm_count) {
     PoolAttnArgs a{};
     a.pool.d = d;
@@ -798,10 +816,12 @@ size_t pool_work_bytes(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint3
     a.n_tok = n_tok;
     a.prefix_len = prefix_len;
     a.sm_count = sm_count;
+    a.pages_stride = 0x7fffffff;          // a line
     size_t most = 0;
     for (uint32_t type : {TYPE_F32, TYPE_BF16, TYPE_F16}) {
         const SplitArgs p = split_plan(a, type);
-        most = std::max(most, (own_slots(p) * p.slot_floats(false) + near_floats(p)) * 4);
+        const size_t items = (size_t)n_tok * d.kv_heads * p.rbo;
+        most = std::max(most, (std::max(own_slots(p), p.units + items) * p.slot_floats(false) + near_floats(p)) * 4);
     }
     return most;
 }
@@ -809,7 +829,7 @@ size_t pool_work_bytes(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint3
 cudaError_t launch_pool_attend(cudaStream_t s, const PoolAttnArgs &a, uint32_t *launched) {
     SplitArgs p = split_plan(a, a.q.type);
     p.own = reinterpret_cast<float *>(a.work);
-    p.near = p.own + own_slots(p) * p.slot_floats(false);
+    p.near = p.own + own_slots(p) * p.slot_floats(false);          // 16-byte boundaries: see slot_floats
     const PoolShape &d = a.pool.d;
     const bool b8 = d.bits == 8;
     cudaError_t e = cudaSuccess;
@@ -820,7 +840,7 @@ cudaError_t launch_pool_attend(cudaStream_t s, const PoolAttnArgs &a, uint32_t *
     }
     e = d.head_dim == 128 ? (b8 ? split_launch<128, 8>(s, p) : split_launch<128, 4>(s, p)) : b8 ? split_launch<64, 8>(s, p) : split_launch<64, 4>(s, p);
     *launched += 1;
-    if (e != cudaSuccess || (p.direct && a.prefix_len == 0)) return e;
+    if (e != cudaSuccess || (p.pieces == 1 && a.prefix_len == 0)) return e;
     *launched += 1;
     // rows are few where their pieces are many
     const uint32_t rows = a.n_tok * a.heads;

@@ -19,15 +19,15 @@ struct SplitArgs {
     PoolAttnArgs a;
     uint32_t tile, rbo, rbp;     // query rows of a CTA, 8 or 16; tiles of a token and kv head; of the prefix (0: the line holds none)
     uint32_t units;              // CTAs
-    bool direct;                 // every CTA has one item
+    uint32_t pieces;             // CTAs of an item; 0: the line is cut into parts
     float *own, *near;           // partial results of own rows; of the prefix
     FlashArgs flash;
 
     __host__ __device__ uint32_t slot_rows(bool prefix) const { const uint32_t g = a.heads / a.pool.d.kv_heads; return prefix || g > tile ? tile : g; }
     __host__ __device__ uint32_t slot_floats(bool prefix) const { return (slot_rows(prefix) * (a.pool.d.head_dim + 2) + 3u) & ~3u; }       // 16-byte boundaries
-    // CTAs and items both ascend along the line, so their sum numbers the pieces
+    // CTAs and items both ascend along the line, so their sum numbers the parts of items
     __host__ __device__ float *slot(bool prefix, uint32_t unit, uint32_t item) const {
-        return (prefix ? near : own) + (size_t)((direct ? 0u : unit) + item) * slot_floats(prefix);
+        return (prefix ? near : own) + (size_t)(pieces != 0 ? unit : unit + item) * slot_floats(prefix);
     }
 };
 __host__ __device__ inline uint32_t prefix_blocks(const SplitArgs &p) { return (p.a.prefix_len + POOL_ROWS - 1) / POOL_ROWS; }
@@ -35,6 +35,9 @@ __host__ __device__ inline uint64_t prefix_line(const SplitArgs &p) { return (ui
 // blocks of a CTA's part: at least MIN_PART, since a part costs its queries and a partial result
 constexpr uint32_t MIN_PART = 8;
 __host__ __device__ inline uint64_t part_blocks(uint64_t all, uint32_t units) { const uint64_t n = (all + units - 1) / units; return n < MIN_PART ? MIN_PART : n; }
+
+// blocks of a piece
+__host__ __device__ inline uint32_t piece_blocks(const SplitArgs &p, uint32_t blocks) { return blocks == 0 ? 1 : (blocks + p.pieces - 1) / p.pieces; }
 
 cudaError_t launch_pool_flash(cudaStream_t s, const SplitArgs &p);
 

@@ -5,6 +5,7 @@ Host-buffer methods take numpy arrays; `*_dev` methods take raw device addresses
 """
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -371,7 +372,7 @@ class Context:
 
 def _rows(r):
     """Rows of (address, token stride, head stride in elements), or of an address alone (dense)."""
-    return Rows(*r) if isinstance(r, (tuple, list)) else Rows(r, 0, 0)
+    return tuple(r) if isinstance(r, (tuple, list)) else (r or 0, 0, 0)
 
 
 class KvPool:
@@ -383,6 +384,9 @@ class KvPool:
         self.ctx, self.L, self.handle = ctx, ctx.L, None
         self.kv_heads, self.head_dim, self.kv_bits, self.page_tokens, self.num_pages = kv_heads, head_dim, kv_bits, page_tokens, num_pages
         cfg = KvPoolConfig(C.sizeof(KvPoolConfig), kv_heads, head_dim, kv_bits, page_tokens, num_pages, POOL_BLOCK_KEYS if block_keys else 0)
+        # argument structs of the calls, kept and filled in at once: a step makes several calls per layer
+        self._args, self._k, self._v = PoolAttention(), Rows(), Rows()
+        self._at = C.byref(self._args), C.byref(self._k), C.byref(self._v)
         self.handle = self.L.kronos_cuda_kv_pool_create(ctx.handle, C.byref(cfg))
         if not self.handle:
             raise KronosCudaError(self.L.kronos_cuda_last_error(ctx.handle).decode())
@@ -399,35 +403,40 @@ class KvPool:
     def device_bytes(self):
         return self.L.kronos_cuda_kv_pool_bytes(self.handle)
 
+    _ROWS, _ATTENTION = struct.Struct("3Q"), struct.Struct("9If3Q3Q7Q")          # fields of Rows and PoolAttention
+
+    def _move(self, f, dtype, d_k, d_v, d_slots, n_tok):
+        self._ROWS.pack_into(self._k, 0, *_rows(d_k))
+        self._ROWS.pack_into(self._v, 0, *_rows(d_v))
+        self.ctx._check(f(self.ctx.handle, self.handle, TYPES[dtype], self._at[1], self._at[2], d_slots, n_tok))
+
     def store_dev(self, dtype, d_k, d_v, d_slots, n_tok):
         """Rows of n_tok tokens into slots (int64: page * page_tokens + row, below 0: left out)."""
-        self.ctx._check(self.L.kronos_cuda_kv_pool_store_dev(self.ctx.handle, self.handle, TYPES[dtype], C.byref(_rows(d_k)), C.byref(_rows(d_v)), d_slots, n_tok))
+        self._move(self.L.kronos_cuda_kv_pool_store_dev, dtype, d_k, d_v, d_slots, n_tok)
 
     def load_dev(self, dtype, d_slots, n_tok, d_k, d_v):
-        self.ctx._check(self.L.kronos_cuda_kv_pool_load_dev(self.ctx.handle, self.handle, TYPES[dtype], C.byref(_rows(d_k)), C.byref(_rows(d_v)), d_slots, n_tok))
+        self._move(self.L.kronos_cuda_kv_pool_load_dev, dtype, d_k, d_v, d_slots, n_tok)
 
     def workspace_bytes(self, heads, n_tok, prefix_len=0):
         return self.L.kronos_cuda_kv_pool_workspace(self.handle, heads, n_tok, prefix_len)
 
-    def _tokens(self, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq=None, workspace=(None, 0), d_out=None, scale=0.0, **rest):
-        return PoolAttention(struct_size=C.sizeof(PoolAttention), row_type=TYPES[dtype], heads=heads, n_tok=n_tok, pages_stride=pages_stride, scale=scale, q=_rows(d_q),
-                             out=_rows(d_out), lens=d_lens, seq=d_seq, pages=d_pages, workspace=workspace[0], workspace_bytes=workspace[1], **rest)
+    def _attention(self, f, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq, workspace, d_out, scale, prefix=(0, 0), top=0, sinks=0, local=0, d_chosen=0):
+        self._ATTENTION.pack_into(self._args, 0, self._ATTENTION.size, TYPES[dtype], heads, n_tok, pages_stride, prefix[1], top, sinks, local, scale, *_rows(d_q), *_rows(d_out),
+                                  d_lens or 0, d_seq or 0, d_pages or 0, prefix[0] or 0, d_chosen or 0, workspace[0] or 0, workspace[1])
+        self.ctx._check(f(self.ctx.handle, self.handle, self._at[0]))
 
     def attend_dev(self, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_out, workspace, d_seq=None, d_prefix_pages=None, prefix_len=0, scale=0.0):
         """Attention of n_tok query tokens over the shared prefix and the first lens[t] (int32) positions of their sequences; d_pages: int32
         table [rows][pages_stride], d_seq: each token's row of it (None: row t), workspace: (address, workspace_bytes(..))."""
-        a = self._tokens(dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq, workspace, d_out, scale, prefix_pages=d_prefix_pages, prefix_len=prefix_len)
-        self.ctx._check(self.L.kronos_cuda_kv_pool_attend_dev(self.ctx.handle, self.handle, C.byref(a)))
+        self._attention(self.L.kronos_cuda_kv_pool_attend_dev, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq, workspace, d_out, scale, (d_prefix_pages, prefix_len))
 
     def select_dev(self, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, top, d_chosen, sinks=1, local=1, d_seq=None, workspace=(None, 0)):
         """The `top` pages of each token and kv head by block keys, int32 [n_tok][kv_heads][top]: indices into the token's row of the table."""
-        a = self._tokens(dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq, workspace, top=top, sinks=sinks, local=local, chosen=d_chosen)
-        self.ctx._check(self.L.kronos_cuda_kv_pool_select_dev(self.ctx.handle, self.handle, C.byref(a)))
+        self._attention(self.L.kronos_cuda_kv_pool_select_dev, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq, workspace, None, 0.0, (0, 0), top, sinks, local, d_chosen)
 
     def attend_chosen_dev(self, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, top, d_chosen, d_out, workspace, d_seq=None, scale=0.0):
         """Attention over the chosen pages alone."""
-        a = self._tokens(dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq, workspace, d_out, scale, top=top, chosen=d_chosen)
-        self.ctx._check(self.L.kronos_cuda_kv_pool_attend_chosen_dev(self.ctx.handle, self.handle, C.byref(a)))
+        self._attention(self.L.kronos_cuda_kv_pool_attend_chosen_dev, dtype, heads, n_tok, d_q, d_lens, d_pages, pages_stride, d_seq, workspace, d_out, scale, (0, 0), top, 0, 0, d_chosen)
 
 
 def desc_of(m):
