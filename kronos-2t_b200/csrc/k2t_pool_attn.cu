@@ -92,7 +92,6 @@ __device__ __forceinline__ void item_fill(const SplitArgs &p, Item &it) {
 
 // Sums of the tokens' blocks over a warp: the whole, and the place of the token that holds block `x` of them (counted per kv head and tile).
 __device__ __forceinline__ uint64_t warp_total(const SplitArgs &p, uint32_t lane) {
-    if (p.a.chosen != nullptr) return (uint64_t)p.a.n_tok * (p.a.top << (p.a.pool.d.page_shift - 4));
     uint64_t sum = 0;
 #pragma unroll 4
     for (uint32_t t = lane; t < p.a.n_tok; t += 32) sum += item_blocks(p, t);
@@ -101,12 +100,6 @@ __device__ __forceinline__ uint64_t warp_total(const SplitArgs &p, uint32_t lane
     return sum;
 }
 __device__ __forceinline__ void warp_find(const SplitArgs &p, uint64_t x, uint32_t lane, uint32_t &t, uint64_t &before, uint32_t &blocks) {
-    if (p.a.chosen != nullptr) {
-        blocks = p.a.top << (p.a.pool.d.page_shift - 4);
-        t = (uint32_t)(x / blocks);
-        before = (uint64_t)t * blocks;
-        return;
-    }
     uint64_t base = 0;
 #pragma unroll 1
     for (uint32_t t0 = 0; t0 < p.a.n_tok; t0 += 32) {
@@ -127,45 +120,29 @@ __device__ __forceinline__ void warp_find(const SplitArgs &p, uint64_t x, uint32
     t = p.a.n_tok; before = base; blocks = 1;            // not reached: x lies below the total
 }
 
-// The item that holds block x of the line: prefix items first, then tokens in order, of a token its kv heads, of those their tiles.
+// The item that holds block x of the line: tokens in order, of a token its kv heads, of those their tiles.
 __device__ __forceinline__ void item_at(const SplitArgs &p, uint64_t x, uint32_t lane, Item &it) {
-    const uint64_t far = prefix_line(p);
-    it.prefix = x < far;
-    if (it.prefix) {
-        const uint32_t nb = prefix_blocks(p);
-        it.index = (uint32_t)(x / nb);
-        it.h = it.index / p.rbp;
-        it.rb = it.index % p.rbp;
-        it.t = 0;
-        it.next = (uint32_t)(x - (uint64_t)it.index * nb);
-    } else {
-        const uint32_t per = p.a.pool.d.kv_heads * p.rbo;
-        uint32_t blocks;
-        uint64_t before;
-        warp_find(p, (x - far) / per, lane, it.t, before, blocks);
-        const uint64_t in = x - far - before * per;
-        const uint32_t sub = (uint32_t)(in / blocks);
-        it.h = sub / p.rbo;
-        it.rb = sub % p.rbo;
-        it.index = it.t * per + sub;
-        it.next = (uint32_t)(in - (uint64_t)sub * blocks);
-    }
+    const uint32_t per = p.a.pool.d.kv_heads * p.rbo;
+    uint32_t blocks;
+    uint64_t before;
+    warp_find(p, x / per, lane, it.t, before, blocks);
+    const uint64_t in = x - before * per;
+    const uint32_t sub = (uint32_t)(in / blocks);
+    it.prefix = false;
+    it.h = sub / p.rbo;
+    it.rb = sub % p.rbo;
+    it.index = it.t * per + sub;
+    it.next = (uint32_t)(in - (uint64_t)sub * blocks);
     item_fill(p, it);
 }
 // The item behind this one; tokens without a block are passed over (the caller knows that there is one).
-__device__ __forceinline__ bool item_after(const SplitArgs &p, Item &it) {          // whether its list is another one
+__device__ __forceinline__ bool item_after(const SplitArgs &p, Item &it) {          // of a line; whether its list is another one
     it.next = 0;
     it.index += 1;
-    if (++it.rb == (it.prefix ? p.rbp : p.rbo)) { it.rb = 0; it.h += 1; }
-    if (it.h < p.a.pool.d.kv_heads) {
-        if (p.a.chosen == nullptr || it.rb != 0) return false;
-        it.list += p.a.top;
-        return true;
-    }
+    if (++it.rb == p.rbo) { it.rb = 0; it.h += 1; }
+    if (it.h < p.a.pool.d.kv_heads) return false;
     it.h = 0;
-    it.t += it.prefix ? 0 : 1;
-    if (it.prefix) it.index = 0;
-    it.prefix = false;
+    it.t += 1;
     if (it.t < p.a.n_tok) item_fill(p, it);
     while (it.blocks == 0 && it.t + 1 < p.a.n_tok) {
         it.t += 1;
@@ -441,7 +418,7 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, BITS, QT == 2, P
     using S = SplitSmem<HD, BITS, QT, NR>;
     extern __shared__ __align__(128) uint8_t smb[];
     __shared__ __align__(8) uint64_t bars[SP_WARPS][SP_STAGES];
-    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, unit = blockIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t sbase = (uint32_t)__cvta_generic_to_shared(smb), ring = sbase + warp * SP_STAGES * B::BYTES, bar = (uint32_t)__cvta_generic_to_shared(bars[warp]);
     const PoolShape &d = p.a.pool.d;
     const uint32_t bs = d.page_shift - 4, in_page = (1u << bs) - 1u;
@@ -460,15 +437,17 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, BITS, QT == 2, P
     }
     Item it;
     uint32_t left;                             // blocks of the CTA's part
-    if (p.pieces != 0) {             // the part is a piece of one item, which may hold no block at all
-        const uint32_t per = d.kv_heads * p.rbo, item = unit / p.pieces, piece = unit % p.pieces;
-        it.prefix = false;
+    const bool near = blockIdx.x < p.near_units;
+    const uint32_t unit = near ? blockIdx.x : blockIdx.x - p.near_units, pieces = near ? p.near_pieces : p.pieces;
+    if (pieces != 0) {             // the part is a piece of one item, which may hold no block at all
+        const uint32_t tiles = near ? p.rbp : p.rbo, per = d.kv_heads * tiles, item = unit / pieces, piece = unit % pieces;
+        it.prefix = near;
         it.index = item;
         it.t = item / per;
-        it.h = item % per / p.rbo;
-        it.rb = item % p.rbo;
+        it.h = item % per / tiles;
+        it.rb = item % tiles;
         item_fill(p, it);
-        const uint32_t part = piece_blocks(p, it.blocks);
+        const uint32_t part = piece_blocks(pieces, it.blocks);
         it.next = min(it.blocks, piece * part);
         left = min(it.blocks - it.next, part);
         if (piece > 0 && left == 0) {          // fewer blocks than pieces; the first one stands for an item without any
@@ -476,9 +455,9 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, BITS, QT == 2, P
             return;
         }
     } else {
-        const uint64_t all = prefix_line(p) + warp_total(p, lane) * d.kv_heads * p.rbo, part = part_blocks(all, p.units), x = (uint64_t)unit * part;
+        const uint64_t all = warp_total(p, lane) * d.kv_heads * p.rbo, part = part_blocks(all, p.units), x = (uint64_t)unit * part;
         if (x >= all) {
-            pdl_wait();
+            if (behind) pdl_wait();
             return;
         }
         left = (uint32_t)min(part, all - x);
@@ -639,44 +618,37 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
     const uint32_t own_item = (t * kh + h) * p.rbo + in / p.tile, r = t * group + in;
     const uint64_t mine = item_blocks(p, t);
     if (p.pieces != 0) {
-        const uint32_t part = piece_blocks(p, (uint32_t)mine);
-        own_first = 0;
+        const uint32_t part = piece_blocks(p.pieces, (uint32_t)mine);
+        own_first = own_item * p.pieces;
         own_n = mine > 0 ? (uint32_t)((mine + part - 1) / part) : 0;
-    } else {
-        uint64_t total, before;
-        if (p.a.chosen != nullptr) {
-            total = p.a.n_tok * mine;
-            before = t * mine;
-        } else {                               // the CTA sums up to its first token, a warp the few up to its own
-            uint64_t sum[2] = {0, 0};
-            for (uint32_t k = threadIdx.x; k < p.a.n_tok; k += MERGE_WARPS * 32) {
-                const uint32_t n = item_blocks(p, k);
-                sum[0] += n;
-                sum[1] += k < t0 ? n : 0;
-            }
+    } else {                                   // the CTA sums up to its first token, a warp the few up to its own
+        uint64_t sum[2] = {0, 0};
+        for (uint32_t k = threadIdx.x; k < p.a.n_tok; k += MERGE_WARPS * 32) {
+            const uint32_t n = item_blocks(p, k);
+            sum[0] += n;
+            sum[1] += k < t0 ? n : 0;
+        }
 #pragma unroll
-            for (int m = 16; m > 0; m >>= 1) {
-                sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], m);
-                sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], m);
-            }
-            if (lane == 0) { s_sum[warp][0] = sum[0]; s_sum[warp][1] = sum[1]; }
-            __syncthreads();
-            total = before = 0;
-            for (uint32_t k = 0; k < MERGE_WARPS; ++k) { total += s_sum[k][0]; before += s_sum[k][1]; }
-            for (uint32_t k = t0; k < t; ++k) before += item_blocks(p, k);
+        for (int m = 16; m > 0; m >>= 1) {
+            sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], m);
+            sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], m);
         }
-        const uint64_t far = prefix_line(p), per = part_blocks(far + total * kh * p.rbo, p.units);
-        if (far > 0) {
-            near_item = h * p.rbp + r / p.tile;
-            const uint64_t b = (uint64_t)near_item * prefix_blocks(p), e = b + prefix_blocks(p);
-            near_first = (uint32_t)(b / per);
-            near_n = (uint32_t)((e - 1) / per) + 1 - near_first;
-        }
+        if (lane == 0) { s_sum[warp][0] = sum[0]; s_sum[warp][1] = sum[1]; }
+        __syncthreads();
+        uint64_t total = 0, before = 0;
+        for (uint32_t k = 0; k < MERGE_WARPS; ++k) { total += s_sum[k][0]; before += s_sum[k][1]; }
+        for (uint32_t k = t0; k < t; ++k) before += item_blocks(p, k);
         if (mine > 0) {
-            const uint64_t b = far + before * kh * p.rbo + (uint64_t)(h * p.rbo + in / p.tile) * mine, e = b + mine;
+            const uint64_t per = part_blocks(total * kh * p.rbo, p.units), b = before * kh * p.rbo + (uint64_t)(h * p.rbo + in / p.tile) * mine, e = b + mine;
             own_first = (uint32_t)(b / per);
             own_n = (uint32_t)((e - 1) / per) + 1 - own_first;
         }
+    }
+    if (p.near_units > 0) {
+        near_item = h * p.rbp + r / p.tile;
+        const uint32_t part = piece_blocks(p.near_pieces, prefix_blocks(p));
+        near_first = near_item * p.near_pieces;
+        near_n = (prefix_blocks(p) + part - 1) / part;
     }
     if (p.flash.on) {
         const FlashArgs &f = p.flash;
@@ -698,7 +670,7 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
         }
         row = (near ? r : in) % p.tile;
         rows = p.slot_rows(near);
-        return near ? p.slot(true, near_first + i, near_item) : p.slot(false, (p.pieces != 0 ? own_item * p.pieces : own_first) + i - near_n, own_item);
+        return near ? p.slot(true, near_first + i, near_item) : p.slot(false, own_first + i - near_n, own_item);
     };
     float top = -INFINITY;
     for (uint32_t i = lane; i < n; i += 32) {
@@ -751,10 +723,16 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
 }
 
 // ------------------------------------------------------------------------------------------------ launches
-// A line of blocks in equal parts, or items in equal pieces, one a CTA?  Chosen pages: items are of one length, so pieces of them are as equal
-// as parts and begin no second item.  Tables: a line, since lengths are ragged, but one CTA per item (nothing to look up, nothing to join)
-// where no item can be longer than a CTA's start (SHORT blocks), or where there are several for every CTA that the SMs hold.
-constexpr uint32_t SHORT = 32;
+// A line of blocks in equal parts, or items in equal pieces, one a CTA?  A piece begins no second item, and nothing has to be looked up for it, but
+// pieces are as equal as the items are long.  The prefix and chosen pages: items of one length, pieces.  Tables: pieces of as many blocks
+// as the widest row of the table gives CTAs that the SMs hold at once (an item that is shorter has fewer: the others leave at once), or of
+// whole items of up to LONGEST blocks where there are a few for every such CTA, or of any length where there are many; else a line.
+constexpr uint32_t LONGEST = 64;
+uint32_t own_pieces(uint64_t items, uint64_t widest, uint64_t room) {
+    for (uint64_t part = MIN_PART; part <= LONGEST; part *= 2)
+        if (items * ((widest + part - 1) / part) <= room) return (uint32_t)((widest + part - 1) / part);
+    return (widest <= LONGEST && items <= 4 * room) || items >= 16 * room ? 1 : 0;
+}
 SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     SplitArgs p{};
     p.a = a;
@@ -776,19 +754,19 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     p.rbo = (group + p.tile - 1) / p.tile;
     p.rbp = near ? (rows + p.tile - 1) / p.tile : 0;
     const uint64_t items = (uint64_t)a.n_tok * d.kv_heads * p.rbo, room = (uint64_t)a.sm_count * split_ctas(d.head_dim, d.bits, type != TYPE_BF16, type == TYPE_F32, p.tile / 8);
-    if (a.chosen != nullptr) {
-        const uint64_t blocks = (uint64_t)a.top << (d.page_shift - 4);
-        p.pieces = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(room / items, blocks / MIN_PART));
-    } else if (p.rbp == 0 && (items >= 3 * room || (items <= room && ((uint64_t)a.pages_stride << (d.page_shift - 4)) <= SHORT))) {
-        p.pieces = 1;
+    const auto pieces_of = [&](uint64_t n, uint64_t blocks) { return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(room / n, blocks / MIN_PART)); };
+    if (near) {
+        p.near_pieces = pieces_of((uint64_t)d.kv_heads * p.rbp, prefix_blocks(p));
+        p.near_units = d.kv_heads * p.rbp * p.near_pieces;
     }
+    p.pieces = a.chosen != nullptr ? pieces_of(items, (uint64_t)a.top << (d.page_shift - 4)) : own_pieces(items, std::max<uint64_t>(1, (uint64_t)a.pages_stride << (d.page_shift - 4)), room);
     p.units = (uint32_t)(p.pieces != 0 ? items * p.pieces : room);
     return p;
 }
 size_t own_slots(const SplitArgs &p) { return p.units + (p.pieces != 0 ? 0 : (size_t)p.a.n_tok * p.a.pool.d.kv_heads * p.rbo); }
 size_t near_floats(const SplitArgs &p) {
     if (p.flash.on) return ((size_t)p.a.sm_count + p.flash.items) * flash_slot_floats(p.a.pool.d.head_dim);
-    return p.rbp == 0 ? 0 : (p.units + (size_t)p.a.pool.d.kv_heads * p.rbp) * p.slot_floats(true);
+    return p.near_units * (size_t)p.slot_floats(true);
 }
 
 // Halves of an operand: bf16 queries and weights are rounded to one each (11 bits where bf16 has 8); fp16 queries keep two, since a score is a
@@ -798,7 +776,7 @@ template <int HD, int BITS, int QT, int PT, int NR> cudaError_t split_go(cudaStr
     static_assert((smem + 1024) * split_ctas(HD, BITS, QT == 2, PT == 2, NR) <= 233472, "shared memory of an SM");
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(pool_split_kernel<HD, BITS, QT, PT, NR>), smem);
     if (e != cudaSuccess) return e;
-    return launch_kernel(pool_split_kernel<HD, BITS, QT, PT, NR>, dim3(p.units), dim3(SP_WARPS * 32), smem, s, true, p);
+    return launch_kernel(pool_split_kernel<HD, BITS, QT, PT, NR>, dim3(p.near_units + p.units), dim3(SP_WARPS * 32), smem, s, true, p);
 }
 template <int HD, int BITS, int NR> cudaError_t split_type(cudaStream_t s, const SplitArgs &p) {
     const uint32_t type = p.a.q.type;
@@ -808,21 +786,21 @@ template <int HD, int BITS> cudaError_t split_launch(cudaStream_t s, const Split
 
 }  // namespace
 
-// Room for a call of these sizes whatever its table's width and choice: as many pieces or parts as there can be.
+// Room for a call of these sizes whatever its table's width and choice (a line has the most partial results), and for one without a prefix.
 size_t pool_work_bytes(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint32_t prefix_len, uint32_t sm_count) {
-    PoolAttnArgs a{};
-    a.pool.d = d;
-    a.heads = heads;
-    a.n_tok = n_tok;
-    a.prefix_len = prefix_len;
-    a.sm_count = sm_count;
-    a.pages_stride = 0x7fffffff;          // a line
     size_t most = 0;
-    for (uint32_t type : {TYPE_F32, TYPE_BF16, TYPE_F16}) {
-        const SplitArgs p = split_plan(a, type);
-        const size_t items = (size_t)n_tok * d.kv_heads * p.rbo;
-        most = std::max(most, (std::max(own_slots(p), p.units + items) * p.slot_floats(false) + near_floats(p)) * 4);
-    }
+    for (uint32_t type : {TYPE_F32, TYPE_BF16, TYPE_F16})
+        for (uint32_t prefix : {0u, prefix_len}) {
+            PoolAttnArgs a{};
+            a.pool.d = d;
+            a.heads = heads;
+            a.n_tok = n_tok;
+            a.prefix_len = prefix;
+            a.sm_count = sm_count;
+            a.pages_stride = 0x7fffffff;
+            const SplitArgs p = split_plan(a, type);
+            most = std::max(most, ((p.units + (size_t)n_tok * d.kv_heads * p.rbo) * p.slot_floats(false) + near_floats(p)) * 4);
+        }
     return most;
 }
 

@@ -18,8 +18,8 @@ __host__ __device__ constexpr uint32_t flash_slot_floats(uint32_t head_dim) { re
 struct SplitArgs {
     PoolAttnArgs a;
     uint32_t tile, rbo, rbp;     // query rows of a CTA, 8 or 16; tiles of a token and kv head; of the prefix (0: the line holds none)
-    uint32_t units;              // CTAs
-    uint32_t pieces;             // CTAs of an item; 0: the line is cut into parts
+    uint32_t units, pieces;      // CTAs for own rows; of an item, or 0: the line of all items' blocks is cut into parts
+    uint32_t near_units, near_pieces;          // CTAs for the prefix, before them; of an item
     float *own, *near;           // partial results of own rows; of the prefix
     FlashArgs flash;
 
@@ -27,17 +27,16 @@ struct SplitArgs {
     __host__ __device__ uint32_t slot_floats(bool prefix) const { return (slot_rows(prefix) * (a.pool.d.head_dim + 2) + 3u) & ~3u; }       // 16-byte boundaries
     // CTAs and items both ascend along the line, so their sum numbers the parts of items
     __host__ __device__ float *slot(bool prefix, uint32_t unit, uint32_t item) const {
-        return (prefix ? near : own) + (size_t)(pieces != 0 ? unit : unit + item) * slot_floats(prefix);
+        return (prefix ? near : own) + (size_t)(prefix || pieces != 0 ? unit : unit + item) * slot_floats(prefix);
     }
 };
 __host__ __device__ inline uint32_t prefix_blocks(const SplitArgs &p) { return (p.a.prefix_len + POOL_ROWS - 1) / POOL_ROWS; }
-__host__ __device__ inline uint64_t prefix_line(const SplitArgs &p) { return (uint64_t)p.a.pool.d.kv_heads * p.rbp * prefix_blocks(p); }
 // blocks of a CTA's part: at least MIN_PART, since a part costs its queries and a partial result
 constexpr uint32_t MIN_PART = 8;
 __host__ __device__ inline uint64_t part_blocks(uint64_t all, uint32_t units) { const uint64_t n = (all + units - 1) / units; return n < MIN_PART ? MIN_PART : n; }
 
 // blocks of a piece
-__host__ __device__ inline uint32_t piece_blocks(const SplitArgs &p, uint32_t blocks) { return blocks == 0 ? 1 : (blocks + p.pieces - 1) / p.pieces; }
+__host__ __device__ inline uint32_t piece_blocks(uint32_t pieces, uint32_t blocks) { return blocks == 0 ? 1 : (blocks + pieces - 1) / pieces; }
 
 cudaError_t launch_pool_flash(cudaStream_t s, const SplitArgs &p);
 
