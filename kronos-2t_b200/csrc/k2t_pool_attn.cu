@@ -765,7 +765,7 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
 }
 size_t own_slots(const SplitArgs &p) { return p.units + (p.pieces != 0 ? 0 : (size_t)p.a.n_tok * p.a.pool.d.kv_heads * p.rbo); }
 size_t near_floats(const SplitArgs &p) {
-    if (p.flash.on) return ((size_t)p.a.sm_count + p.flash.items) * flash_slot_floats(p.a.pool.d.head_dim);
+    if (p.flash.on) return ((size_t)p.a.sm_count + p.flash.items) * flash_slot_floats(p.a.pool.d.head_dim) + p.flash.items * flash_query_bytes(p.a.pool.d.head_dim, true) / 4;
     return p.near_units * (size_t)p.slot_floats(true);
 }
 
@@ -812,9 +812,11 @@ cudaError_t launch_pool_attend(cudaStream_t s, const PoolAttnArgs &a, uint32_t *
     const bool b8 = d.bits == 8;
     cudaError_t e = cudaSuccess;
     if (p.flash.on) {
+        p.flash.queries = reinterpret_cast<uint8_t *>(p.near + ((size_t)a.sm_count + p.flash.items) * flash_slot_floats(d.head_dim));
+        p.flash.factors = reinterpret_cast<float *>(p.flash.queries + p.flash.items * (flash_query_bytes(d.head_dim, a.q.type != TYPE_BF16) - 2 * FLASH_ROWS * 4));
         e = launch_pool_flash(s, p);
         if (e != cudaSuccess) return e;
-        *launched += 1;
+        *launched += 2;
     }
     e = d.head_dim == 128 ? (b8 ? split_launch<128, 8>(s, p) : split_launch<128, 4>(s, p)) : b8 ? split_launch<64, 8>(s, p) : split_launch<64, 4>(s, p);
     *launched += 1;

@@ -10,7 +10,11 @@ constexpr uint32_t FLASH_ROWS = 128, FLASH_MIN_PART = 2;
 struct FlashArgs {
     bool on, halved;
     uint32_t items, row_tiles, tiles, part;
+    uint8_t *queries;            // operand tiles of all items, two of FLASH_ROWS rows each
+    float *factors;              // of their rows
 };
+// bytes of an item's queries and factors
+__host__ __device__ constexpr size_t flash_query_bytes(uint32_t head_dim, bool two_terms) { return 2 * FLASH_ROWS * (head_dim * (two_terms ? 4 : 2) + 4); }
 // partial results of a CTA and item: two of FLASH_ROWS rows
 __host__ __device__ constexpr uint32_t flash_slot_floats(uint32_t head_dim) { return 2 * FLASH_ROWS * (head_dim + 2); }
 

@@ -20,7 +20,7 @@ constexpr uint32_t FL_KT = 64, FL_SOFT = 8, FL_CONV = 4, FL_WARPS = FL_SOFT + FL
 template <int HD, int BITS, int QT> struct Flash {
     static constexpr uint32_t PD = HD / 64, G = PoolBlock<HD, BITS>::G, STAGES = HD == 128 && QT == 2 ? 2 : 4;
     static constexpr uint32_t Q_TILE = PD * FLASH_ROWS * 128, K_TILE = PD * FL_KT * 128, CONST = G == 1 ? 24 : 48;        // bytes; CONST per pair of columns
-    static constexpr uint32_t CONSTS = 1024, FACTORS = CONSTS + STAGES * (FL_KT / 2) * CONST, HEAD = (FACTORS + 2 * FLASH_ROWS * 4 + 1023) / 1024 * 1024;
+    static constexpr uint32_t CONSTS = 1024, HEAD = (CONSTS + STAGES * (FL_KT / 2) * CONST + 1023) / 1024 * 1024;
     static constexpr uint32_t Q_AT = HEAD, K_AT = Q_AT + 2 * QT * Q_TILE, SMEM = K_AT + STAGES * 2 * K_TILE + 1024;
 };
 
@@ -196,51 +196,42 @@ template <int HD, int BITS, int QT> struct Converter {
 };
 
 // ------------------------------------------------------------------------------------------------ queries
-// Eight warps write the item's rows: transformed, scaled by a power of two, one or two halves; their factors to s_c.
-template <int HD, int BITS, int QT> __device__ __forceinline__ void flash_queries(const SplitArgs &p, const FlashArgs &f, uint32_t item, uint32_t warp, uint32_t lane, uint32_t s_q, float *s_c) {
-    using F = Flash<HD, BITS, QT>;
-    constexpr uint32_t LANES = HD / 8, ROWS = 32 / LANES;
-    const uint32_t group = p.a.heads / p.a.pool.d.kv_heads, all = p.a.n_tok * group, h = item / f.row_tiles, r0 = item % f.row_tiles * 2 * FLASH_ROWS;
-    const uint32_t mine = (f.halved ? FLASH_ROWS : 2 * FLASH_ROWS) / FL_SOFT, l = lane % LANES;
-    const uint32_t signs = p.a.pool.signs[l / 4] >> (l % 4 * 8);
-    constexpr uint32_t AHEAD = 4;              // rows of a lane on their way together
-#pragma unroll 1
-    for (uint32_t i0 = 0; i0 < mine; i0 += ROWS * AHEAD) {
-        Row8 ahead[AHEAD];
+// The rows of all items as the kernel's first operand, made once for all parts of the line: transformed, scaled by a power of two, one or two
+// halves, in the layout of shared memory ([item][tile of 128 rows][term][panel][row]: a bulk copy brings a tile); their factors behind them.
+constexpr uint32_t QK_THREADS = 256;
+template <int HD, int QT> __global__ void __launch_bounds__(QK_THREADS) pool_query_kernel(const __grid_constant__ SplitArgs p) {
+    constexpr uint32_t LANES = HD / 8, TILE = HD / 64 * FLASH_ROWS * 128;
+    const FlashArgs &f = p.flash;
+    const uint32_t lane = threadIdx.x & 31u, l = lane % LANES, group = p.a.heads / p.a.pool.d.kv_heads, all = p.a.n_tok * group;
+    const uint32_t at = (blockIdx.x * QK_THREADS + threadIdx.x) / LANES, item = at / (2 * FLASH_ROWS), row = at % (2 * FLASH_ROWS);          // whole warps below the last item
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t h = item / f.row_tiles, r = item % f.row_tiles * 2 * FLASH_ROWS + row;
+    if (item >= f.items) return;
+    float v[8], top = 0.0f;
+    Row8 x;
+    x.clear();
+    if (r < all) x.ask(p.a.q, r / group * p.a.q.token_stride + (h * group + r % group) * p.a.q.head_stride + l * 8);
+    x.values(p.a.q.type, v);
+    transform8(v, p.a.pool.signs[l / 4] >> (l % 4 * 8), lane);
 #pragma unroll
-        for (uint32_t u = 0; u < AHEAD; ++u) {
-            const uint32_t r = r0 + warp * mine + i0 + u * ROWS + lane / LANES;
-            ahead[u].clear();
-            if (i0 + u * ROWS < mine && r < all) ahead[u].ask(p.a.q, r / group * p.a.q.token_stride + (h * group + r % group) * p.a.q.head_stride + l * 8);
-        }
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
 #pragma unroll
-        for (uint32_t u = 0; u < AHEAD; ++u) {
-        const uint32_t i = i0 + u * ROWS;
-        if (i >= mine) break;
-        const uint32_t row = warp * mine + i + lane / LANES;
-        float v[8], top = 0.0f;
-        ahead[u].values(p.a.q.type, v);
-        transform8(v, signs, lane);
+    for (uint32_t m = LANES / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+    const int e = query_exponent(top);
+    const float up = power_of_two(e);
+    if (l == 0) f.factors[item * 2 * FLASH_ROWS + row] = p.a.scale * LOG2E * power_of_two(-e);
+    uint32_t hi[4], lo[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
-#pragma unroll
-        for (uint32_t m = LANES / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-        const int e = query_exponent(top);
-        const float up = power_of_two(e);
-        if (l == 0) s_c[row] = p.a.scale * LOG2E * power_of_two(-e);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float x = v[2 * k] * up, y = v[2 * k + 1] * up;
-            hi[k] = half2_bits(x, y);
-            const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&hi[k]));
-            lo[k] = half2_bits(x - g.x, y - g.y);
-        }
-        const uint32_t at = s_q + row / FLASH_ROWS * QT * F::Q_TILE + (l / 8) * (FLASH_ROWS * 128) + row % FLASH_ROWS * 128 + (((l % 8) ^ (row & 7u)) << 4);
-        sts4(at, hi[0], hi[1], hi[2], hi[3]);
-        if (QT == 2) sts4(at + F::Q_TILE, lo[0], lo[1], lo[2], lo[3]);
-        }
+    for (int k = 0; k < 4; ++k) {
+        const float y = v[2 * k] * up, z = v[2 * k + 1] * up;
+        hi[k] = half2_bits(y, z);
+        const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&hi[k]));
+        lo[k] = half2_bits(y - g.x, z - g.y);
     }
+    uint8_t *to = f.queries + ((size_t)item * 2 + row / FLASH_ROWS) * QT * TILE + (l / 8) * (FLASH_ROWS * 128) + row % FLASH_ROWS * 128 + (((l % 8) ^ (row & 7u)) << 4);
+    *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (QT == 2) *reinterpret_cast<uint4 *>(to + TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
 
 template <int HD, int BITS, int QT, int PT>
@@ -255,13 +246,12 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
     // barriers: tiles landed / free; of each stream: S ready (two buffers), weights ready (two), O updated; queries; end of a segment; end
     const uint32_t b_full = sbase, b_free = b_full + 8 * STAGES, b_s = b_free + 8 * STAGES, b_p = b_s + 32, b_o = b_p + 32, b_q = b_o + 16, b_end = b_q + 8, b_last = b_end + 8;
     volatile uint32_t *s_tmem = reinterpret_cast<volatile uint32_t *>(smem + 512), *s_abort = reinterpret_cast<volatile uint32_t *>(smem + 516);
-    float *s_c = reinterpret_cast<float *>(smem + F::FACTORS);
     const uint32_t s_q = sbase + F::Q_AT, s_k = sbase + F::K_AT;
     if (tid == 0) {
         for (uint32_t i = 0; i < STAGES; ++i) { mbar_init(b_full + 8 * i, FL_CONV); mbar_init(b_free + 8 * i, 1); }
         for (uint32_t i = 0; i < 4; ++i) { mbar_init(b_s + 8 * i, 1); mbar_init(b_p + 8 * i, 128); }
         for (uint32_t i = 0; i < 2; ++i) mbar_init(b_o + 8 * i, 1);
-        mbar_init(b_q, FL_SOFT);
+        mbar_init(b_q, 1);
         mbar_init(b_end, 1);
         mbar_init(b_last, 1);
         *s_abort = 0;
@@ -285,8 +275,8 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
     if (warp >= FL_SOFT && warp < FL_SOFT + FL_CONV) {
         const Converter<HD, BITS, QT> cv(p, tid - FL_SOFT * 32);
         uint32_t n = 0;                            // tiles of the CTA so far
-        typename Converter<HD, BITS, QT>::Raw now, next;
-        // tiles two ahead, over the ends of segments
+        // two tiles on their way, each in registers of its own: a copy from one to the other would wait for the younger one's loads
+        typename Converter<HD, BITS, QT>::Raw even, odd;
         Segment ahead;
         uint32_t as = 0, at = 0;
         bool more = segment_of(f, 0, ahead);
@@ -299,20 +289,25 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
                 if (more) at = ahead.first;
             }
         };
-        fetch(now);
-        fetch(next);
-        const uint32_t total = min(f.part, f.items * f.tiles - blockIdx.x * f.part);
-#pragma unroll 1
-        for (; n < total; ++n) {
+        auto tile = [&](typename Converter<HD, BITS, QT>::Raw &r) {          // one tile, and the one two behind it asked for
             const uint32_t stage = n % STAGES;
             if (n >= STAGES) ok = mbar_wait_warp(b_free + 8 * stage, (n / STAGES - 1) & 1u, FL_WAIT, s_abort);
-            if (!ok) break;
-            cv.put(s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST, now);
+            if (!ok) return;
+            cv.put(s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST, r);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(b_full + 8 * stage);
-            now = next;
-            fetch(next);
+            fetch(r);
+            ++n;
+        };
+        fetch(even);
+        fetch(odd);
+        const uint32_t total = min(f.part, f.items * f.tiles - blockIdx.x * f.part);
+#pragma unroll 1
+        while (ok && n < total) {
+            tile(even);
+            if (!ok || n >= total) break;
+            tile(odd);
         }
     } else if (warp == FL_WARPS - 1) {
         if (lane == 0) {
@@ -386,19 +381,18 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
         const uint32_t t_s0 = tmem + st * t_stream + ((quarter * 32u) << 16), t_o = t_s0 + 128;
         uint32_t n0 = 0, done = 0;
         for (uint32_t s = 0; ok && segment_of(f, s, g); ++s) {
-            flash_queries<HD, BITS, QT>(p, f, g.item, warp, lane, s_q, s_c);
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(b_q);
-            ok = mbar_wait_warp(b_q, s & 1u, FL_WAIT, s_abort);          // the factors of all rows
-            if (!ok) break;
+            if (tid == 0) {                            // the products that read the last segment's queries have ended (b_end)
+                const uint32_t bytes = (f.halved ? 1 : 2) * QT * F::Q_TILE;
+                mbar_expect_tx(b_q, bytes);
+                for (uint32_t i = 0; i < bytes; i += F::Q_TILE) bulk_g2s(s_q + i, f.queries + (size_t)g.item * 2 * QT * F::Q_TILE + i, F::Q_TILE, b_q);
+            }
             const uint32_t n = g.last - g.first, count = f.halved ? (n + 1 - st) / 2 : n;
             const uint32_t r0 = g.item % f.row_tiles * 2 * FLASH_ROWS + (f.halved ? 0u : st * FLASH_ROWS), left = all > r0 ? all - r0 : 0;          // rows of the stream's tile
             const bool idle = quarter * 32 >= left;
             float c[4], m[4], l[4];                // rows quarter * 32 + lr + 8 k
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                c[k] = s_c[(f.halved ? 0u : st * FLASH_ROWS) + quarter * 32 + lr + 8 * k];
+                c[k] = __ldcg(f.factors + g.item * 2 * FLASH_ROWS + (f.halved ? 0u : st * FLASH_ROWS) + quarter * 32 + lr + 8 * k);
                 m[k] = -INFINITY;
                 l[k] = 0.0f;
             }
@@ -569,7 +563,9 @@ template <int HD, int BITS, int QT, int PT> cudaError_t flash_go(cudaStream_t s,
     static_assert(smem <= 232448, "shared memory of an SM");
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(pool_flash_kernel<HD, BITS, QT, PT>), smem);
     if (e != cudaSuccess) return e;
-    const uint32_t line = p.flash.items * p.flash.tiles;
+    const uint32_t line = p.flash.items * p.flash.tiles, rows = p.flash.items * 2 * FLASH_ROWS;
+    const cudaError_t q = launch_kernel(pool_query_kernel<HD, QT>, dim3(rows * (HD / 8) / QK_THREADS), dim3(QK_THREADS), 0, s, true, p);
+    if (q != cudaSuccess) return q;
     return launch_kernel(pool_flash_kernel<HD, BITS, QT, PT>, dim3((line + p.flash.part - 1) / p.flash.part), dim3(FL_THREADS), smem, s, true, p);
 }
 template <int HD, int BITS> cudaError_t flash_type(cudaStream_t s, const SplitArgs &p) {
