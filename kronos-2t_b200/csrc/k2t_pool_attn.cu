@@ -652,7 +652,7 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
     }
     if (p.flash.on) {
         const FlashArgs &f = p.flash;
-        near_item = h * f.row_tiles + (f.halved ? 0u : r / (2 * FLASH_ROWS));
+        near_item = h * f.row_tiles + r / (f.halved ? FLASH_ROWS : 2 * FLASH_ROWS);
         const uint32_t b = near_item * f.tiles, e = b + f.tiles;
         near_first = b / f.part;
         near_n = ((e - 1) / f.part + 1 - near_first) << (f.halved ? 1 : 0);
@@ -743,8 +743,8 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     p.flash.on = a.prefix_len > 0 && rows > (dbg ? (uint32_t)atoi(dbg) : 16);          // more than one tile of this kernel: k2t_pool_flash.cu
     if (p.flash.on) {
         FlashArgs &f = p.flash;
-        f.halved = rows <= FLASH_ROWS;
-        f.row_tiles = (rows + 2 * FLASH_ROWS - 1) / (2 * FLASH_ROWS);
+        f.halved = rows <= FLASH_ROWS || type != TYPE_BF16;
+        f.row_tiles = f.halved ? (rows + FLASH_ROWS - 1) / FLASH_ROWS : (rows + 2 * FLASH_ROWS - 1) / (2 * FLASH_ROWS);
         f.items = d.kv_heads * f.row_tiles;
         f.tiles = (a.prefix_len + 63) / 64;
         f.part = (uint32_t)std::max<uint64_t>(FLASH_MIN_PART, ((uint64_t)f.items * f.tiles + a.sm_count - 1) / a.sm_count);
@@ -765,7 +765,7 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
 }
 size_t own_slots(const SplitArgs &p) { return p.units + (p.pieces != 0 ? 0 : (size_t)p.a.n_tok * p.a.pool.d.kv_heads * p.rbo); }
 size_t near_floats(const SplitArgs &p) {
-    if (p.flash.on) return ((size_t)p.a.sm_count + p.flash.items) * flash_slot_floats(p.a.pool.d.head_dim) + p.flash.items * flash_query_bytes(p.a.pool.d.head_dim, true) / 4;
+    if (p.flash.on) return ((size_t)p.a.sm_count + p.flash.items) * flash_slot_floats(p.a.pool.d.head_dim) + p.flash.items * flash_query_bytes(p.a.pool.d.head_dim) / 4;
     return p.near_units * (size_t)p.slot_floats(true);
 }
 
@@ -813,7 +813,7 @@ cudaError_t launch_pool_attend(cudaStream_t s, const PoolAttnArgs &a, uint32_t *
     cudaError_t e = cudaSuccess;
     if (p.flash.on) {
         p.flash.queries = reinterpret_cast<uint8_t *>(p.near + ((size_t)a.sm_count + p.flash.items) * flash_slot_floats(d.head_dim));
-        p.flash.factors = reinterpret_cast<float *>(p.flash.queries + p.flash.items * (flash_query_bytes(d.head_dim, a.q.type != TYPE_BF16) - 2 * FLASH_ROWS * 4));
+        p.flash.factors = reinterpret_cast<float *>(p.flash.queries + p.flash.items * (flash_query_bytes(d.head_dim) - 2 * FLASH_ROWS * 4));
         e = launch_pool_flash(s, p);
         if (e != cudaSuccess) return e;
         *launched += 2;

@@ -5,7 +5,7 @@
 namespace k2t {
 
 // The prefix over many rows (k2t_pool_flash.cu): items are (kv head, 2 FLASH_ROWS rows), tiles of 64 positions; a line of items * tiles, `part` of it
-// a CTA.  halved: an item has at most FLASH_ROWS rows, and its tiles are dealt out to two streams over the same rows.
+// a CTA.  halved: an item has FLASH_ROWS rows, and its tiles are dealt out to two streams over the same rows.
 constexpr uint32_t FLASH_ROWS = 128, FLASH_MIN_PART = 2;
 struct FlashArgs {
     bool on, halved;
@@ -13,8 +13,8 @@ struct FlashArgs {
     uint8_t *queries;            // operand tiles of all items, two of FLASH_ROWS rows each
     float *factors;              // of their rows
 };
-// bytes of an item's queries and factors
-__host__ __device__ constexpr size_t flash_query_bytes(uint32_t head_dim, bool two_terms) { return 2 * FLASH_ROWS * (head_dim * (two_terms ? 4 : 2) + 4); }
+// bytes of an item's queries (at most two tiles: of rows, or of terms) and factors
+__host__ __device__ constexpr size_t flash_query_bytes(uint32_t head_dim) { return 2 * FLASH_ROWS * (head_dim * 2 + 4); }
 // partial results of a CTA and item: two of FLASH_ROWS rows
 __host__ __device__ constexpr uint32_t flash_slot_floats(uint32_t head_dim) { return 2 * FLASH_ROWS * (head_dim + 2); }
 

@@ -1,10 +1,13 @@
 // Attention of many query rows over the pages of a shared prefix: the rows of all tokens against the same keys and values, on the
 // tensor-memory cores.  The mathematics is that of k2t_pool_attn.cu (weights that carry the values' scales, codes as exact halves).
-//   * A CTA takes a stretch of an item (kv head, 256 rows) of the prefix in tiles of 64 positions, as two STREAMS of 128 rows, or, where an
-//     item has no more than 128 rows, of even and odd tiles.  While the softmax warps of one stream work, the products of the other run.
-//   * Four warps bring tiles in: 16 bytes of codes a load, two tiles ahead in registers, expanded to halves in the operand layout (panels
-//     of 64 columns, 128-byte rows, 128-byte swizzle), and the tile's scales as column constants.
-//   * One thread issues S = Q K^T (queries from shared memory) and O += P V (weights from tensor memory, where they overwrite S).
+//   * A CTA takes a stretch of an item of the prefix in tiles of 64 positions, as two STREAMS of 128 rows: an item is a kv head and 256 rows,
+//     or, where there are no more than 128 or a row has two terms (their operands would not fit), 128 rows, whose even and odd tiles are
+//     the streams.  While the softmax warps of one stream work, the products of the other run.
+//   * One warp asks for the blocks of a tile (bulk copies into a ring of raw tiles; as loads into registers, two tiles in flight, they were
+//     throttled by the little L1 that the operands leave: 2200 cycles a tile).  Four warps expand the codes to halves in the operand layout
+//     (panels of 64 columns, 128-byte rows, 128-byte swizzle) and the tile's scales to column constants.
+//   * One warp issues S = Q K^T (queries from shared memory) and O += P V (weights from tensor memory, where they overwrite S).  All its lanes
+//     run along, so that descriptors stay in uniform registers, and lane 0 issues: alone in its branch it took 100 cycles a product.
 //   * Eight warps of softmax read S in fragments of 16x256b: a lane then has 4 rows and a quarter of the columns, so that it reads a quarter
 //     of the column constants; O is rescaled only where a row's maximum has grown by more than 2^8.
 // The tiles of all items form one line that is cut into equal parts, one per CTA; partial results are joined by pool_merge_kernel.
@@ -15,13 +18,14 @@
 namespace k2t {
 namespace {
 
-constexpr uint32_t FL_KT = 64, FL_SOFT = 8, FL_CONV = 4, FL_WARPS = FL_SOFT + FL_CONV + 1, FL_THREADS = FL_WARPS * 32, FL_WAIT = 1u << 22, FL_COLS = 512;
+constexpr uint32_t FL_KT = 64, FL_SOFT = 8, FL_CONV = 4, FL_ISSUE = FL_SOFT + FL_CONV, FL_LOAD = FL_ISSUE + 1, FL_THREADS = (FL_LOAD + 1) * 32, FL_WAIT = 1u << 22, FL_COLS = 512;
 
 template <int HD, int BITS, int QT> struct Flash {
-    static constexpr uint32_t PD = HD / 64, G = PoolBlock<HD, BITS>::G, STAGES = HD == 128 && QT == 2 ? 2 : 4;
-    static constexpr uint32_t Q_TILE = PD * FLASH_ROWS * 128, K_TILE = PD * FL_KT * 128, CONST = G == 1 ? 24 : 48;        // bytes; CONST per pair of columns
+    using B = PoolBlock<HD, BITS>;
+    static constexpr uint32_t PD = HD / 64, G = B::G, STAGES = 3, RAWS = 3, BLOCKS = FL_KT / POOL_ROWS;
+    static constexpr uint32_t Q_TILE = PD * FLASH_ROWS * 128, K_TILE = PD * FL_KT * 128, RAW = (BLOCKS * B::BYTES + 127) / 128 * 128, CONST = G == 1 ? 24 : 48;        // bytes; CONST per pair of columns
     static constexpr uint32_t CONSTS = 1024, HEAD = (CONSTS + STAGES * (FL_KT / 2) * CONST + 1023) / 1024 * 1024;
-    static constexpr uint32_t Q_AT = HEAD, K_AT = Q_AT + 2 * QT * Q_TILE, SMEM = K_AT + STAGES * 2 * K_TILE + 1024;
+    static constexpr uint32_t Q_AT = HEAD, K_AT = Q_AT + 2 * Q_TILE, RAW_AT = K_AT + STAGES * 2 * K_TILE, SMEM = RAW_AT + RAWS * RAW + 1024;          // two tiles of queries: of rows, or of terms
 };
 
 using u64 = unsigned long long;
@@ -55,6 +59,25 @@ __device__ __forceinline__ void sts4(uint32_t at, uint32_t x, uint32_t y, uint32
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
+// As mma_ss, mma_ts and tc_commit, by the lane that `on` is 1 in: all lanes of the warp run along, without a branch.
+__device__ __forceinline__ void mma_ss_on(uint32_t on, uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n"
+        ::"r"(d_tmem), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(on) : "memory");
+}
+__device__ __forceinline__ void mma_ts_on(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(on) : "memory");
+}
+__device__ __forceinline__ void tc_commit_on(uint32_t on, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar), "r"(on) : "memory");
+}
+__device__ __forceinline__ uint4 lds4(uint32_t at) { uint4 v; asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at)); return v; }
+__device__ __forceinline__ uint32_t lds1(uint32_t at) { uint32_t v; asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at)); return v; }
+
 struct Segment { uint32_t item, first, last; };          // tiles [first, last) of an item
 // Segment s of a CTA's part of the line; false behind the last.
 __device__ __forceinline__ bool segment_of(const FlashArgs &f, uint32_t s, Segment &g) {
@@ -80,18 +103,12 @@ template <uint32_t RB> __device__ __forceinline__ void unit_place(uint32_t r, ui
 template <int HD, int BITS, int QT> struct Converter {
     using B = PoolBlock<HD, BITS>;
     using F = Flash<HD, BITS, QT>;
-    static constexpr uint32_t BLOCKS = FL_KT / POOL_ROWS, STEP = 128 / B::RB, PER = BLOCKS / STEP;          // blocks of a tile; between two of a thread; of a thread
+    static constexpr uint32_t STEP = 128 / B::RB, PER = F::BLOCKS / STEP;          // blocks between two of a thread; of a thread
     static_assert(FL_CONV == 4, "128 threads");
-    struct Raw {
-        uint4 k[PER], v[PER];
-        uint32_t ks[2], vs[2];        // threads below 64: scales of position `thread` (fp32, or of each group)
-        bool seen;
-    };
-    const SplitArgs &p;
-    uint32_t ct, lane, first, load_at, store_at, store_x;
+    uint32_t ct, first, load_at, store_at, store_x;
     Expand ex;
 
-    __device__ __forceinline__ Converter(const SplitArgs &args, uint32_t thread) : p(args), ct(thread), lane(thread & 31u) {
+    __device__ __forceinline__ explicit Converter(uint32_t thread) : ct(thread) {
         // eight neighbouring threads: four chunks of two neighbouring rows, whose stores meet in no bank (rows differ in the last bit of the swizzle)
         const uint32_t u = ct % B::RB;
         first = ct / B::RB;
@@ -104,41 +121,6 @@ template <int HD, int BITS, int QT> struct Converter {
         const uint32_t c0 = BITS == 8 ? chunk * 2 : chunk * 4;          // first 16-byte chunk of halves
         store_at = (c0 >> 3) * (FL_KT * 128) + row * 128;
         store_x = (c0 & 7u) ^ (row & 7u);
-    }
-    // Lane b < BLOCKS: the place of block b of a tile in the pool, ~0 where nothing of it is in sight.
-    __device__ __forceinline__ uint32_t place(uint32_t head, uint32_t tile) const {
-        const PoolShape &d = p.a.pool.d;
-        const uint32_t pos = tile * FL_KT + lane * POOL_ROWS;
-        if (lane >= BLOCKS || pos >= p.a.prefix_len) return ~0u;
-        const int32_t page = __ldg(p.a.prefix_pages + (pos >> d.page_shift));
-        if (page < 0 || (uint32_t)page >= d.num_pages) { pool_bad_page(p.a.pool); return ~0u; }
-        return (((uint32_t)page * d.kv_heads + head) << (d.page_shift - 4)) + ((pos & ((1u << d.page_shift) - 1u)) >> 4);
-    }
-    __device__ __forceinline__ const uint8_t *block(uint32_t at) const { return p.a.pool.rows + (size_t)(at == ~0u ? 0u : at) * B::BYTES; }          // any, where none is in sight
-    __device__ __forceinline__ void fetch(uint32_t head, uint32_t tile, Raw &r) const {
-        const uint32_t mine = place(head, tile);
-#pragma unroll
-        for (uint32_t i = 0; i < PER; ++i) {
-            const uint8_t *at = block(__shfl_sync(0xffffffffu, mine, first + i * STEP)) + load_at;
-            r.k[i] = __ldcg(reinterpret_cast<const uint4 *>(at));
-            r.v[i] = __ldcg(reinterpret_cast<const uint4 *>(at + B::V_AT));
-        }
-        const uint32_t own = __shfl_sync(0xffffffffu, mine, ct / POOL_ROWS % BLOCKS);
-        if (ct < FL_KT) {
-            const uint32_t row = ct % POOL_ROWS;
-            const uint8_t *at = block(own);
-            r.seen = own != ~0u && tile * FL_KT + ct < p.a.prefix_len;
-            if (BITS == 8) {
-                r.ks[0] = __ldcg(reinterpret_cast<const uint32_t *>(at + B::KS_AT) + row);
-                r.vs[0] = __ldcg(reinterpret_cast<const uint32_t *>(at + B::VS_AT) + row);
-            } else {
-#pragma unroll
-                for (uint32_t g = 0; g < B::G; ++g) {
-                    r.ks[g] = (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(at + B::KS_AT) + row * B::G + g) << 16;
-                    r.vs[g] = (uint32_t)__ldcg(reinterpret_cast<const uint16_t *>(at + B::VS_AT) + row * B::G + g) << 16;
-                }
-            }
-        }
     }
     __device__ __forceinline__ void expand(uint32_t at, const uint4 &w) const {          // `at`: the thread's row and panel
         if (BITS == 8) {
@@ -153,29 +135,40 @@ template <int HD, int BITS, int QT> struct Converter {
             }
         }
     }
-    __device__ __forceinline__ void put(uint32_t s_tile, uint8_t *consts, const Raw &r) const {
+    // A raw tile at shared address `raw` becomes an operand tile; `seen`: whether position ct of it is in sight.
+    __device__ __forceinline__ void put(uint32_t raw, uint32_t s_tile, uint8_t *consts, bool seen) const {
+        uint4 k[PER], v[PER];
 #pragma unroll
-        for (uint32_t i = 0; i < PER; ++i) {
-            const uint32_t at = s_tile + store_at + (first + i * STEP) * (POOL_ROWS * 128);
-            expand(at, r.k[i]);
-            expand(at + F::K_TILE, r.v[i]);
-        }
+        for (uint32_t i = 0; i < PER; ++i) k[i] = lds4(raw + (first + i * STEP) * B::BYTES + load_at);
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) v[i] = lds4(raw + (first + i * STEP) * B::BYTES + B::V_AT + load_at);
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) expand(s_tile + store_at + (first + i * STEP) * (POOL_ROWS * 128), k[i]);
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) expand(s_tile + F::K_TILE + store_at + (first + i * STEP) * (POOL_ROWS * 128), v[i]);
         if (ct < FL_KT) {
             constexpr uint32_t G = B::G;
-            float ks[2], v[2], lv = -INFINITY, iv = 0.0f, part[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (uint32_t g = 0; g < G; ++g) {
-                ks[g] = r.seen ? __uint_as_float(r.ks[g]) : 0.0f;
-                v[g] = __uint_as_float(r.vs[g]);
+            const uint32_t at = raw + ct / POOL_ROWS * B::BYTES, row = ct % POOL_ROWS;
+            float ks[2], vs[2], lv = -INFINITY, iv = 0.0f, part[2] = {0.0f, 0.0f};
+            if (BITS == 8) {
+                ks[0] = __uint_as_float(lds1(at + B::KS_AT + row * 4));
+                vs[0] = __uint_as_float(lds1(at + B::VS_AT + row * 4));
+            } else {
+                const uint32_t a = lds1(at + B::KS_AT + (row * G & ~1u) * 2), b = lds1(at + B::VS_AT + (row * G & ~1u) * 2);          // one row's two groups, or two rows
+                const bool high = G == 1 && (row & 1u);
+                ks[0] = __uint_as_float(high ? a & 0xFFFF0000u : a << 16); ks[1] = __uint_as_float(a & 0xFFFF0000u);
+                vs[0] = __uint_as_float(high ? b & 0xFFFF0000u : b << 16); vs[1] = __uint_as_float(b & 0xFFFF0000u);
             }
-            if (r.seen) {
+            if (seen) {
                 // a row of zeros: 8-bit codes are 0, and two groups have a factor each; a single group of 4-bit codes, which has neither, is
                 // given a scale below everything that counts
-                const float top = G == 1 ? v[0] : fmaxf(v[0], v[G - 1]), u = v[0] != v[0] ? v[0] : top == 0.0f ? (BITS == 4 && G == 1 ? 0x1p-100f : 1.0f) : top;
+                const float top = G == 1 ? vs[0] : fmaxf(vs[0], vs[1]), u = vs[0] != vs[0] ? vs[0] : top == 0.0f ? (BITS == 4 && G == 1 ? 0x1p-100f : 1.0f) : top;
                 lv = log2_approx(u);
                 iv = rcp_approx(u);
 #pragma unroll
-                for (uint32_t g = 0; g < G; ++g) part[g] = v[g] * iv;
+                for (uint32_t g = 0; g < G; ++g) part[g] = vs[g] * iv;
+            } else {
+                ks[0] = ks[1] = 0.0f;
             }
             float *c = reinterpret_cast<float *>(consts);
             const uint32_t i = ct >> 1, e = ct & 1u;
@@ -203,10 +196,10 @@ template <int HD, int QT> __global__ void __launch_bounds__(QK_THREADS) pool_que
     constexpr uint32_t LANES = HD / 8, TILE = HD / 64 * FLASH_ROWS * 128;
     const FlashArgs &f = p.flash;
     const uint32_t lane = threadIdx.x & 31u, l = lane % LANES, group = p.a.heads / p.a.pool.d.kv_heads, all = p.a.n_tok * group;
-    const uint32_t at = (blockIdx.x * QK_THREADS + threadIdx.x) / LANES, item = at / (2 * FLASH_ROWS), row = at % (2 * FLASH_ROWS);          // whole warps below the last item
+    const uint32_t per = (f.halved ? 1 : 2) * FLASH_ROWS, at = (blockIdx.x * QK_THREADS + threadIdx.x) / LANES, item = at / per, row = at % per;          // whole warps below the last item
     pdl_wait();
     pdl_trigger();
-    const uint32_t h = item / f.row_tiles, r = item % f.row_tiles * 2 * FLASH_ROWS + row;
+    const uint32_t h = item / f.row_tiles, r = item % f.row_tiles * per + row;
     if (item >= f.items) return;
     float v[8], top = 0.0f;
     Row8 x;
@@ -220,7 +213,7 @@ template <int HD, int QT> __global__ void __launch_bounds__(QK_THREADS) pool_que
     for (uint32_t m = LANES / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
     const int e = query_exponent(top);
     const float up = power_of_two(e);
-    if (l == 0) f.factors[item * 2 * FLASH_ROWS + row] = p.a.scale * LOG2E * power_of_two(-e);
+    if (l == 0) f.factors[item * per + row] = p.a.scale * LOG2E * power_of_two(-e);
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -229,7 +222,7 @@ template <int HD, int QT> __global__ void __launch_bounds__(QK_THREADS) pool_que
         const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&hi[k]));
         lo[k] = half2_bits(y - g.x, z - g.y);
     }
-    uint8_t *to = f.queries + ((size_t)item * 2 + row / FLASH_ROWS) * QT * TILE + (l / 8) * (FLASH_ROWS * 128) + row % FLASH_ROWS * 128 + (((l % 8) ^ (row & 7u)) << 4);
+    uint8_t *to = f.queries + ((size_t)item * (per / FLASH_ROWS) + row / FLASH_ROWS) * QT * TILE + (l / 8) * (FLASH_ROWS * 128) + row % FLASH_ROWS * 128 + (((l % 8) ^ (row & 7u)) << 4);
     *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     if (QT == 2) *reinterpret_cast<uint4 *>(to + TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
@@ -239,14 +232,15 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
     using F = Flash<HD, BITS, QT>;
     constexpr uint32_t G = F::G, STAGES = F::STAGES;
     extern __shared__ uint8_t smem_raw[];
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw), sbase = (raw + 1023u) & ~1023u;
     uint8_t *smem = smem_raw + (sbase - raw);
     const FlashArgs &f = p.flash;
-    // barriers: tiles landed / free; of each stream: S ready (two buffers), weights ready (two), O updated; queries; end of a segment; end
-    const uint32_t b_full = sbase, b_free = b_full + 8 * STAGES, b_s = b_free + 8 * STAGES, b_p = b_s + 32, b_o = b_p + 32, b_q = b_o + 16, b_end = b_q + 8, b_last = b_end + 8;
+    // barriers: tiles ready / free; of each stream: S ready (two buffers), weights ready (two), O updated; queries; end of a segment; end; raw
+    // tiles landed / free
+    const uint32_t b_full = sbase, b_free = b_full + 8 * STAGES, b_s = b_free + 8 * STAGES, b_p = b_s + 32, b_o = b_p + 32, b_q = b_o + 16, b_end = b_q + 8, b_last = b_end + 8, b_rfull = b_last + 8, b_rfree = b_rfull + 8 * F::RAWS;
     volatile uint32_t *s_tmem = reinterpret_cast<volatile uint32_t *>(smem + 512), *s_abort = reinterpret_cast<volatile uint32_t *>(smem + 516);
-    const uint32_t s_q = sbase + F::Q_AT, s_k = sbase + F::K_AT;
+    const uint32_t s_q = sbase + F::Q_AT, s_k = sbase + F::K_AT, s_raw = sbase + F::RAW_AT;
     if (tid == 0) {
         for (uint32_t i = 0; i < STAGES; ++i) { mbar_init(b_full + 8 * i, FL_CONV); mbar_init(b_free + 8 * i, 1); }
         for (uint32_t i = 0; i < 4; ++i) { mbar_init(b_s + 8 * i, 1); mbar_init(b_p + 8 * i, 128); }
@@ -254,10 +248,11 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
         mbar_init(b_q, 1);
         mbar_init(b_end, 1);
         mbar_init(b_last, 1);
+        for (uint32_t i = 0; i < F::RAWS; ++i) { mbar_init(b_rfull + 8 * i, 1); mbar_init(b_rfree + 8 * i, FL_CONV); }
         *s_abort = 0;
         fence_mbar_init();
     }
-    if (warp == FL_WARPS - 1) {
+    if (warp == FL_ISSUE) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sbase + 512), "r"(FL_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -272,109 +267,129 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
     Segment g;
     bool ok = true;
 
-    if (warp >= FL_SOFT && warp < FL_SOFT + FL_CONV) {
-        const Converter<HD, BITS, QT> cv(p, tid - FL_SOFT * 32);
-        uint32_t n = 0;                            // tiles of the CTA so far
-        // two tiles on their way, each in registers of its own: a copy from one to the other would wait for the younger one's loads
-        typename Converter<HD, BITS, QT>::Raw even, odd;
-        Segment ahead;
-        uint32_t as = 0, at = 0;
-        bool more = segment_of(f, 0, ahead);
-        if (more) at = ahead.first;
-        auto fetch = [&](typename Converter<HD, BITS, QT>::Raw &r) {
-            if (!more) return;
-            cv.fetch(ahead.item / f.row_tiles, at, r);
-            if (++at == ahead.last) {
-                more = segment_of(f, ++as, ahead);
-                if (more) at = ahead.first;
-            }
-        };
-        auto tile = [&](typename Converter<HD, BITS, QT>::Raw &r) {          // one tile, and the one two behind it asked for
-            const uint32_t stage = n % STAGES;
-            if (n >= STAGES) ok = mbar_wait_warp(b_free + 8 * stage, (n / STAGES - 1) & 1u, FL_WAIT, s_abort);
-            if (!ok) return;
-            cv.put(s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST, r);
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(b_full + 8 * stage);
-            fetch(r);
-            ++n;
-        };
-        fetch(even);
-        fetch(odd);
-        const uint32_t total = min(f.part, f.items * f.tiles - blockIdx.x * f.part);
-#pragma unroll 1
-        while (ok && n < total) {
-            tile(even);
-            if (!ok || n >= total) break;
-            tile(odd);
-        }
-    } else if (warp == FL_WARPS - 1) {
-        if (lane == 0) {
-            // fp32 accumulators, fp16 operands; A and B K-major for S, B with its columns consecutive for O
-            constexpr uint32_t id_s = (1u << 4) | ((FL_KT >> 3) << 17) | ((FLASH_ROWS >> 4) << 24);
-            constexpr uint32_t id_o = (1u << 4) | (1u << 16) | (((G == 1 ? HD : 64) >> 3) << 17) | ((FLASH_ROWS >> 4) << 24);
-            uint32_t n0 = 0, done[2] = {0, 0};             // tiles of the CTA before the segment; tiles of the streams before it
-            for (uint32_t s = 0; ok && segment_of(f, s, g); ++s) {
-                const uint32_t n = g.last - g.first, count[2] = {f.halved ? (n + 1) / 2 : n, f.halved ? n / 2 : n};
-                auto tile_of = [&](uint32_t st, uint32_t i) { return n0 + (f.halved ? 2 * i + st : i); };
-                auto scores = [&](uint32_t st, uint32_t i) {
-                    const uint32_t tile = tile_of(st, i), stage = tile % STAGES, use = done[st] + i, buf = G == 1 ? use & 1u : 0u;
-                    if (!mbar_wait_thread(b_full + 8 * stage, (tile / STAGES) & 1u, FL_WAIT, s_abort)) return false;
-                    tc_fence_after();
-                    const uint32_t q = s_q + (f.halved ? 0u : st) * QT * F::Q_TILE, k = s_k + stage * 2 * F::K_TILE, t_s = tmem + st * t_stream + buf * FL_KT;
-#pragma unroll
-                    for (uint32_t c = 0; c < HD / 16; ++c)
-#pragma unroll
-                        for (uint32_t x = 0; x < QT; ++x)
-                            mma_ss(t_s + (G == 2 ? c / 4 * FL_KT : 0u), desc_k(q + x * F::Q_TILE + (c / 4) * FLASH_ROWS * 128 + (c % 4) * 32), desc_k(k + (c / 4) * FL_KT * 128 + (c % 4) * 32), id_s,
-                                   (x == 0 && (G == 2 ? c % 4 : c) == 0) ? 0u : 1u);
-                    tc_commit(b_s + 8 * (2 * st + buf));
-                    return true;
-                };
-                ok = mbar_wait_thread(b_q, s & 1u, FL_WAIT, s_abort);
-                for (uint32_t st = 0; ok && st < 2; ++st)
-                    if (count[st] > 0) ok = scores(st, 0);
-                for (uint32_t i = 0; ok && i < count[0]; ++i) {
-                    for (uint32_t st = 0; ok && st < 2; ++st) {
-                        if (i >= count[st]) continue;
-                        const uint32_t use = done[st] + i, buf = G == 1 ? use & 1u : 0u, tile = tile_of(st, i), stage = tile % STAGES;
-                        if (G == 1 && i + 1 < count[st]) {
-                            // the weights of tile i - 1 lie where S of tile i + 1 goes
-                            if (i >= 1) ok = mbar_wait_thread(b_o + 8 * st, (use - 1) & 1u, FL_WAIT, s_abort);
-                            ok = ok && scores(st, i + 1);
-                            if (!ok) break;
-                        }
-                        ok = mbar_wait_thread(b_p + 8 * (2 * st + buf), (G == 1 ? use >> 1 : use) & 1u, FL_WAIT, s_abort);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t t_p = tmem + st * t_stream + buf * FL_KT, t_o = tmem + st * t_stream + 128, v = s_k + stage * 2 * F::K_TILE + F::K_TILE;
-#pragma unroll
-                        for (uint32_t x = 0; x < G; ++x)
-#pragma unroll
-                            for (uint32_t y = 0; y < PT; ++y)
-#pragma unroll
-                                for (uint32_t k = 0; k < FL_KT / 16; ++k)
-                                    mma_ts(t_o + x * 64, t_p + (x * PT + y) * 32 + k * 8, desc_mn(v + x * FL_KT * 128 + k * 16 * 128, FL_KT * 128), id_o, (i | y | k) != 0 ? 1u : 0u);
-                        if (f.halved || st == 1) tc_commit(b_free + 8 * stage);
-                        tc_commit(b_o + 8 * st);
-                    }
-                    if (G == 2)
-                        for (uint32_t st = 0; ok && st < 2; ++st)
-                            if (i + 1 < count[st]) {
-                                ok = mbar_wait_thread(b_o + 8 * st, (done[st] + i) & 1u, FL_WAIT, s_abort);
-                                ok = ok && scores(st, i + 1);
-                            }
+    if (warp == FL_LOAD) {
+        // lane b asks for block b of a tile; a raw tile holds the blocks as they lie
+        const PoolShape &d = p.a.pool.d;
+        uint32_t n = 0;
+        for (uint32_t s = 0; ok && segment_of(f, s, g); ++s) {
+            const uint32_t head = g.item / f.row_tiles;
+            auto page_of = [&](uint32_t tile) {
+                const uint32_t pos = tile * FL_KT + lane * POOL_ROWS;
+                return lane < F::BLOCKS && tile < g.last && pos < p.a.prefix_len ? __ldg(p.a.prefix_pages + (pos >> d.page_shift)) : 0;
+            };
+            int32_t page = page_of(g.first);
+            for (uint32_t t = g.first; t < g.last; ++t, ++n) {
+                const uint32_t slot = n % F::RAWS, pos = t * FL_KT + lane * POOL_ROWS;
+                const int32_t next = page_of(t + 1);
+                if (n >= F::RAWS) ok = mbar_wait_warp(b_rfree + 8 * slot, (n / F::RAWS - 1) & 1u, FL_WAIT, s_abort);
+                if (!ok) break;
+                const bool there = lane < F::BLOCKS && pos < p.a.prefix_len, good = there && page >= 0 && (uint32_t)page < d.num_pages;
+                if (there && !good) pool_bad_page(p.a.pool);
+                const uint32_t blocks = __ballot_sync(0xffffffffu, good);
+                if (lane == 0) {
+                    reinterpret_cast<volatile uint32_t *>(smem + 528)[slot] = blocks;          // which of the tile's blocks are in sight
+                    mbar_expect_tx(b_rfull + 8 * slot, __popc(blocks) * F::B::BYTES);
                 }
-                tc_commit(b_end);
-                n0 += n;
-                done[0] += count[0];
-                done[1] += count[1];
+                __syncwarp();
+                if (good)
+                    bulk_g2s(s_raw + slot * F::RAW + lane * F::B::BYTES,
+                             p.a.pool.rows + ((((size_t)page * d.kv_heads + head) << (d.page_shift - 4)) + ((pos & ((1u << d.page_shift) - 1u)) >> 4)) * F::B::BYTES, F::B::BYTES, b_rfull + 8 * slot);
+                page = next;
             }
-            tc_commit(b_last);               // also after a wait that gave up: the products in flight end before the CTA leaves
-            for (uint32_t spin = 0; spin < FL_WAIT && !mbar_try_wait(b_last, 0); ++spin) {}
-            if (!ok) atomicCAS(p.a.pool.err, 0u, 1u);
         }
+        // the copies in flight land before the CTA leaves, also after a wait that gave up
+        for (uint32_t i = n > F::RAWS ? n - F::RAWS : 0; i < n; ++i)
+            for (uint32_t spin = 0; spin < FL_WAIT && !mbar_try_wait(b_rfull + 8 * (i % F::RAWS), (i / F::RAWS) & 1u); ++spin) {}
+    } else if (warp >= FL_SOFT && warp < FL_ISSUE) {
+        const Converter<HD, BITS, QT> cv(tid - FL_SOFT * 32);
+        uint32_t n = 0;
+        for (uint32_t s = 0; ok && segment_of(f, s, g); ++s)
+#pragma unroll 1
+            for (uint32_t t = g.first; t < g.last; ++t, ++n) {
+                const uint32_t stage = n % STAGES, slot = n % F::RAWS;
+                ok = mbar_wait_warp(b_rfull + 8 * slot, (n / F::RAWS) & 1u, FL_WAIT, s_abort);
+                if (!ok) break;
+                if (n >= STAGES) ok = mbar_wait_warp(b_free + 8 * stage, (n / STAGES - 1) & 1u, FL_WAIT, s_abort);
+                if (!ok) break;
+                const uint32_t blocks = reinterpret_cast<volatile uint32_t *>(smem + 528)[slot];
+                cv.put(s_raw + slot * F::RAW, s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST,
+                       (blocks >> (cv.ct / POOL_ROWS % F::BLOCKS) & 1u) != 0 && t * FL_KT + cv.ct < p.a.prefix_len);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(b_full + 8 * stage);
+                    mbar_arrive(b_rfree + 8 * slot);
+                }
+            }
+    } else if (warp == FL_ISSUE) {
+        // fp32 accumulators, fp16 operands; A and B K-major for S, B with its columns consecutive for O
+        constexpr uint32_t id_s = (1u << 4) | ((FL_KT >> 3) << 17) | ((FLASH_ROWS >> 4) << 24);
+        constexpr uint32_t id_o = (1u << 4) | (1u << 16) | (((G == 1 ? HD : 64) >> 3) << 17) | ((FLASH_ROWS >> 4) << 24);
+        const uint32_t on = lane == 0 ? 1u : 0u;
+        uint32_t n0 = 0, done[2] = {0, 0};             // tiles of the CTA before the segment; tiles of the streams before it
+        for (uint32_t s = 0; ok && segment_of(f, s, g); ++s) {
+            const uint32_t n = g.last - g.first, count[2] = {f.halved ? (n + 1) / 2 : n, f.halved ? n / 2 : n};
+            auto tile_of = [&](uint32_t st, uint32_t i) { return n0 + (f.halved ? 2 * i + st : i); };
+            auto scores = [&](uint32_t st, uint32_t i) {
+                const uint32_t tile = tile_of(st, i), stage = tile % STAGES, use = done[st] + i, buf = G == 1 ? use & 1u : 0u;
+                if (!mbar_wait_warp(b_full + 8 * stage, (tile / STAGES) & 1u, FL_WAIT, s_abort)) return false;
+                tc_fence_after();
+                const uint32_t t_s = tmem + st * t_stream + buf * FL_KT;
+                const uint64_t q = desc_k(s_q + (f.halved ? 0u : st) * F::Q_TILE), k = desc_k(s_k + stage * 2 * F::K_TILE);          // further operands: addresses in units of 16 bytes
+#pragma unroll
+                for (uint32_t c = 0; c < HD / 16; ++c)
+#pragma unroll
+                    for (uint32_t x = 0; x < QT; ++x)
+                        mma_ss_on(on, t_s + (G == 2 ? c / 4 * FL_KT : 0u), q + ((x * F::Q_TILE + (c / 4) * FLASH_ROWS * 128 + (c % 4) * 32) >> 4), k + (((c / 4) * FL_KT * 128 + (c % 4) * 32) >> 4), id_s,
+                                  (x == 0 && (G == 2 ? c % 4 : c) == 0) ? 0u : 1u);
+                tc_commit_on(on, b_s + 8 * (2 * st + buf));
+                return true;
+            };
+            ok = mbar_wait_warp(b_q, s & 1u, FL_WAIT, s_abort);
+            for (uint32_t st = 0; ok && st < 2; ++st)
+                if (count[st] > 0) ok = scores(st, 0);
+            for (uint32_t i = 0; ok && i < count[0]; ++i) {
+                for (uint32_t st = 0; ok && st < 2; ++st) {
+                    if (i >= count[st]) continue;
+                    const uint32_t use = done[st] + i, buf = G == 1 ? use & 1u : 0u, tile = tile_of(st, i), stage = tile % STAGES;
+                    if (G == 1 && i + 1 < count[st]) {
+                        // the weights of tile i - 1 lie where S of tile i + 1 goes
+                        if (i >= 1) ok = mbar_wait_warp(b_o + 8 * st, (use - 1) & 1u, FL_WAIT, s_abort);
+                        if (!ok) break;
+                        ok = scores(st, i + 1);
+                        if (!ok) break;
+                    }
+                    ok = mbar_wait_warp(b_p + 8 * (2 * st + buf), (G == 1 ? use >> 1 : use) & 1u, FL_WAIT, s_abort);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t t_p = tmem + st * t_stream + buf * FL_KT, t_o = tmem + st * t_stream + 128;
+                    const uint64_t v = desc_mn(s_k + stage * 2 * F::K_TILE + F::K_TILE, FL_KT * 128);
+#pragma unroll
+                    for (uint32_t x = 0; x < G; ++x)
+#pragma unroll
+                        for (uint32_t y = 0; y < PT; ++y)
+#pragma unroll
+                            for (uint32_t k = 0; k < FL_KT / 16; ++k)
+                                mma_ts_on(on, t_o + x * 64, t_p + (x * PT + y) * 32 + k * 8, v + ((x * FL_KT * 128 + k * 16 * 128) >> 4), id_o, (i | y | k) != 0 ? 1u : 0u);
+                    if (f.halved || st == 1) tc_commit_on(on, b_free + 8 * stage);
+                    tc_commit_on(on, b_o + 8 * st);
+                }
+                if (G == 2)
+                    for (uint32_t st = 0; ok && st < 2; ++st)
+                        if (i + 1 < count[st]) {
+                            ok = mbar_wait_warp(b_o + 8 * st, (done[st] + i) & 1u, FL_WAIT, s_abort);
+                            if (!ok) break;
+                            ok = scores(st, i + 1);
+                        }
+            }
+            tc_commit_on(on, b_end);
+            n0 += n;
+            done[0] += count[0];
+            done[1] += count[1];
+        }
+        tc_commit_on(on, b_last);               // also after a wait that gave up: the products in flight end before the CTA leaves
+        for (uint32_t spin = 0; spin < FL_WAIT && !mbar_try_wait(b_last, 0); ++spin) {}
+        if (!ok && lane == 0) atomicCAS(p.a.pool.err, 0u, 1u);
     } else {
         const uint32_t st = warp / 4, quarter = warp % 4, lr = lane >> 2, lc = lane & 3u;
         const uint32_t group = p.a.heads / p.a.pool.d.kv_heads, all = p.a.n_tok * group;
@@ -382,17 +397,17 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
         uint32_t n0 = 0, done = 0;
         for (uint32_t s = 0; ok && segment_of(f, s, g); ++s) {
             if (tid == 0) {                            // the products that read the last segment's queries have ended (b_end)
-                const uint32_t bytes = (f.halved ? 1 : 2) * QT * F::Q_TILE;
+                const uint32_t bytes = (f.halved ? QT : 2) * F::Q_TILE;
                 mbar_expect_tx(b_q, bytes);
-                for (uint32_t i = 0; i < bytes; i += F::Q_TILE) bulk_g2s(s_q + i, f.queries + (size_t)g.item * 2 * QT * F::Q_TILE + i, F::Q_TILE, b_q);
+                for (uint32_t i = 0; i < bytes; i += F::Q_TILE) bulk_g2s(s_q + i, f.queries + (size_t)g.item * bytes + i, F::Q_TILE, b_q);
             }
             const uint32_t n = g.last - g.first, count = f.halved ? (n + 1 - st) / 2 : n;
-            const uint32_t r0 = g.item % f.row_tiles * 2 * FLASH_ROWS + (f.halved ? 0u : st * FLASH_ROWS), left = all > r0 ? all - r0 : 0;          // rows of the stream's tile
+            const uint32_t r0 = g.item % f.row_tiles * (f.halved ? 1 : 2) * FLASH_ROWS + (f.halved ? 0u : st * FLASH_ROWS), left = all > r0 ? all - r0 : 0;          // rows of the stream's tile
             const bool idle = quarter * 32 >= left;
             float c[4], m[4], l[4];                // rows quarter * 32 + lr + 8 k
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                c[k] = __ldcg(f.factors + g.item * 2 * FLASH_ROWS + (f.halved ? 0u : st * FLASH_ROWS) + quarter * 32 + lr + 8 * k);
+                c[k] = __ldcg(f.factors + g.item * (f.halved ? 1 : 2) * FLASH_ROWS + (f.halved ? 0u : st * FLASH_ROWS) + quarter * 32 + lr + 8 * k);
                 m[k] = -INFINITY;
                 l[k] = 0.0f;
             }
@@ -552,7 +567,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == FL_WARPS - 1) {
+    if (warp == FL_ISSUE) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(FL_COLS) : "memory");
     }
@@ -563,7 +578,7 @@ template <int HD, int BITS, int QT, int PT> cudaError_t flash_go(cudaStream_t s,
     static_assert(smem <= 232448, "shared memory of an SM");
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(pool_flash_kernel<HD, BITS, QT, PT>), smem);
     if (e != cudaSuccess) return e;
-    const uint32_t line = p.flash.items * p.flash.tiles, rows = p.flash.items * 2 * FLASH_ROWS;
+    const uint32_t line = p.flash.items * p.flash.tiles, rows = p.flash.items * (p.flash.halved ? 1 : 2) * FLASH_ROWS;
     const cudaError_t q = launch_kernel(pool_query_kernel<HD, QT>, dim3(rows * (HD / 8) / QK_THREADS), dim3(QK_THREADS), 0, s, true, p);
     if (q != cudaSuccess) return q;
     return launch_kernel(pool_flash_kernel<HD, BITS, QT, PT>, dim3((line + p.flash.part - 1) / p.flash.part), dim3(FL_THREADS), smem, s, true, p);
