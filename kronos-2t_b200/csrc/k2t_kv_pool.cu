@@ -72,8 +72,9 @@ __device__ __forceinline__ uint8_t *block_of(const PoolView &p, int64_t slot, ui
 
 // ------------------------------------------------------------------------------------------------ rows in, rows out
 // head_dim / 8 lanes hold a row, eight values each; rows are numbered (token, keys | values, head).  A thread has its part of ROW_AHEAD rows on
-// the way at a time.
-constexpr uint32_t ROW_THREADS = 256, ROW_AHEAD = 4;
+// the way at a time: four, or one where the rows are too few to fill the SMs even so (a decode batch: the rows of a thread would only follow
+// one another).
+constexpr uint32_t ROW_THREADS = 256;
 struct RowAt { uint32_t t, value, head; };
 __device__ __forceinline__ RowAt row_at(const PoolStoreArgs &a, uint32_t r) {          // r below 2^31: a division by a multiplication (and a shift) that is exact there
     const uint32_t per = 2 * a.pool.d.kv_heads, t = __umulhi(r, a.rows_mul) >> a.rows_shift, u = r - t * per, value = u >= a.pool.d.kv_heads ? 1u : 0u;
@@ -136,7 +137,7 @@ template <int HD, int BITS> __device__ __forceinline__ void put_row(const PoolSt
     }
 }
 
-template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_store_kernel(const __grid_constant__ PoolStoreArgs a) {
+template <int HD, int BITS, uint32_t ROW_AHEAD> __global__ void __launch_bounds__(ROW_THREADS) pool_store_kernel(const __grid_constant__ PoolStoreArgs a) {
     using B = PoolBlock<HD, BITS>;
     constexpr uint32_t LANES = HD / 8, STEP = ROW_THREADS / LANES;
     const uint32_t lane = threadIdx.x & 31, l = lane % LANES, signs = signs8(a.pool, l * 8), rows = a.n_tok * 2 * a.pool.d.kv_heads;
@@ -187,7 +188,7 @@ template <int HD, int BITS, int N> struct Stored {
     }
 };
 
-template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_load_kernel(const __grid_constant__ PoolStoreArgs a) {
+template <int HD, int BITS, uint32_t ROW_AHEAD> __global__ void __launch_bounds__(ROW_THREADS) pool_load_kernel(const __grid_constant__ PoolStoreArgs a) {
     using B = PoolBlock<HD, BITS>;
     constexpr uint32_t LANES = HD / 8, STEP = ROW_THREADS / LANES;
     const uint32_t lane = threadIdx.x & 31, l = lane % LANES, signs = signs8(a.pool, l * 8), rows = a.n_tok * 2 * a.pool.d.kv_heads;
@@ -449,10 +450,11 @@ template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_TH
     }
 }
 
-uint32_t row_ctas(const PoolStoreArgs &a) {
-    const uint32_t per = ROW_THREADS * 8 / a.pool.d.head_dim * ROW_AHEAD;
+uint32_t row_ctas(const PoolStoreArgs &a, uint32_t ahead) {
+    const uint32_t per = ROW_THREADS * 8 / a.pool.d.head_dim * ahead;
     return (uint32_t)(((uint64_t)a.n_tok * 2 * a.pool.d.kv_heads + per - 1) / per);
 }
+bool few_rows(const PoolStoreArgs &a) { return row_ctas(a, 1) <= 4 * a.sm_count; }
 // r / (2 kv heads) for r below 2^31
 PoolStoreArgs divided(PoolStoreArgs a) {
     const uint32_t per = 2 * a.pool.d.kv_heads;
@@ -464,7 +466,8 @@ PoolStoreArgs divided(PoolStoreArgs a) {
 }
 template <int HD, int BITS> cudaError_t store_rows(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched) {
     *launched += 1;
-    const cudaError_t e = launch_kernel(pool_store_kernel<HD, BITS>, dim3(row_ctas(a)), dim3(ROW_THREADS), 0, s, true, a);
+    const cudaError_t e = few_rows(a) ? launch_kernel(pool_store_kernel<HD, BITS, 1>, dim3(row_ctas(a, 1)), dim3(ROW_THREADS), 0, s, true, a)
+                                      : launch_kernel(pool_store_kernel<HD, BITS, 4>, dim3(row_ctas(a, 4)), dim3(ROW_THREADS), 0, s, true, a);
     if (e != cudaSuccess || !a.pool.d.block_keys) return e;
     const uint64_t warps = ((uint64_t)a.n_tok + 31) / 32 * a.pool.d.kv_heads;
     *launched += 1;
@@ -472,7 +475,8 @@ template <int HD, int BITS> cudaError_t store_rows(cudaStream_t s, const PoolSto
 }
 template <int HD, int BITS> cudaError_t load_rows(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched) {
     *launched += 1;
-    return launch_kernel(pool_load_kernel<HD, BITS>, dim3(row_ctas(a)), dim3(ROW_THREADS), 0, s, true, a);
+    return few_rows(a) ? launch_kernel(pool_load_kernel<HD, BITS, 1>, dim3(row_ctas(a, 1)), dim3(ROW_THREADS), 0, s, true, a)
+                       : launch_kernel(pool_load_kernel<HD, BITS, 4>, dim3(row_ctas(a, 4)), dim3(ROW_THREADS), 0, s, true, a);
 }
 
 }  // namespace

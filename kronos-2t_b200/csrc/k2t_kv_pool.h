@@ -44,7 +44,7 @@ struct PoolStoreArgs {
     RowsArg k, v;
     const int64_t *slots;
     uint32_t n_tok;              // times 2 kv heads: below 2^31
-    uint32_t rows_mul, rows_shift;
+    uint32_t rows_mul, rows_shift, sm_count;
 };
 cudaError_t launch_pool_store(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched);
 cudaError_t launch_pool_load(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched);

@@ -12,7 +12,6 @@
 // long sequence alike keep every CTA busy to the end.  An item that lies in one part is finished there; the others leave partial
 // results, which pool_merge_kernel joins.
 #include <algorithm>
-#include <cstdlib>
 
 #include "k2t_flash_tc.cuh"
 #include "k2t_kv_pool.cuh"
@@ -739,8 +738,9 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     const PoolShape &d = a.pool.d;
     const uint32_t group = a.heads / d.kv_heads;
     const uint32_t rows = a.n_tok * group;
-    static const char *dbg = getenv("POOL_FLASH");
-    p.flash.on = a.prefix_len > 0 && rows > (dbg ? (uint32_t)atoi(dbg) : 16);          // more than one tile of this kernel: k2t_pool_flash.cu
+    // More rows than a tile of this kernel: k2t_pool_flash.cu.  Its start costs more, but it expands a cached row once for 128 or 256 query rows
+    // where this one does for 16 (24 sequences x 7 heads behind 500 / 4000 / 16000 positions, the whole call: 19 / 31 / 53 us here, 24 / 28 / 39 there).
+    p.flash.on = a.prefix_len > 0 && rows > 16;
     if (p.flash.on) {
         FlashArgs &f = p.flash;
         f.halved = rows <= FLASH_ROWS || type != TYPE_BF16;

@@ -139,6 +139,7 @@ int32_t move_rows(KronosCudaContext *ctx, KronosCudaKvPool *pool, uint32_t type,
     a.pool.err = ctx->d_err;
     a.slots = slots;
     a.n_tok = (uint32_t)n_tok;
+    a.sm_count = pool->sm_count;
     uint32_t launched = 0;
     const cudaError_t e = load ? launch_pool_load(ctx->stream, a, &launched) : launch_pool_store(ctx->stream, a, &launched);
     ctx->launches += launched;

@@ -7,7 +7,8 @@
 //     throttled by the little L1 that the operands leave: 2200 cycles a tile).  Four warps expand the codes to halves in the operand layout
 //     (panels of 64 columns, 128-byte rows, 128-byte swizzle) and the tile's scales to column constants.
 //   * One warp issues S = Q K^T (queries from shared memory) and O += P V (weights from tensor memory, where they overwrite S).  All its lanes
-//     run along, so that descriptors stay in uniform registers, and lane 0 issues: alone in its branch it took 100 cycles a product.
+//     run along and an elected one issues, which keeps descriptors in uniform registers: as a branch of lane 0, or with a predicate of lanes,
+//     a product took 75 (scores) and 97 cycles to issue and was the bound (160 sequences behind 32768 positions 323 us, 286 elected).
 //   * Eight warps of softmax read S in fragments of 16x256b: a lane then has 4 rows and a quarter of the columns, so that it reads a quarter
 //     of the column constants; O is rescaled only where a row's maximum has grown by more than 2^8.
 // The tiles of all items form one line that is cut into equal parts, one per CTA; partial results are joined by pool_merge_kernel.
@@ -59,21 +60,11 @@ __device__ __forceinline__ void sts4(uint32_t at, uint32_t x, uint32_t y, uint32
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
 
-// As mma_ss, mma_ts and tc_commit, by the lane that `on` is 1 in: all lanes of the warp run along, without a branch.
-__device__ __forceinline__ void mma_ss_on(uint32_t on, uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n"
-        ::"r"(d_tmem), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(on) : "memory");
-}
-__device__ __forceinline__ void mma_ts_on(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(on) : "memory");
-}
-__device__ __forceinline__ void tc_commit_on(uint32_t on, uint32_t bar) {
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar), "r"(on) : "memory");
+// One lane of a warp that is together, always the same one.
+__device__ __forceinline__ bool elected() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
 }
 __device__ __forceinline__ uint4 lds4(uint32_t at) { uint4 v; asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at)); return v; }
 __device__ __forceinline__ uint32_t lds1(uint32_t at) { uint32_t v; asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at)); return v; }
@@ -231,6 +222,7 @@ template <int HD, int BITS, int QT, int PT>
 __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_constant__ SplitArgs p) {
     using F = Flash<HD, BITS, QT>;
     constexpr uint32_t G = F::G, STAGES = F::STAGES;
+    static_assert(STAGES >= 3, "tiles in use at a time, see the order of the products");
     extern __shared__ uint8_t smem_raw[];
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw), sbase = (raw + 1023u) & ~1023u;
@@ -325,7 +317,6 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
         // fp32 accumulators, fp16 operands; A and B K-major for S, B with its columns consecutive for O
         constexpr uint32_t id_s = (1u << 4) | ((FL_KT >> 3) << 17) | ((FLASH_ROWS >> 4) << 24);
         constexpr uint32_t id_o = (1u << 4) | (1u << 16) | (((G == 1 ? HD : 64) >> 3) << 17) | ((FLASH_ROWS >> 4) << 24);
-        const uint32_t on = lane == 0 ? 1u : 0u;
         uint32_t n0 = 0, done[2] = {0, 0};             // tiles of the CTA before the segment; tiles of the streams before it
         for (uint32_t s = 0; ok && segment_of(f, s, g); ++s) {
             const uint32_t n = g.last - g.first, count[2] = {f.halved ? (n + 1) / 2 : n, f.halved ? n / 2 : n};
@@ -336,43 +327,54 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
                 tc_fence_after();
                 const uint32_t t_s = tmem + st * t_stream + buf * FL_KT;
                 const uint64_t q = desc_k(s_q + (f.halved ? 0u : st) * F::Q_TILE), k = desc_k(s_k + stage * 2 * F::K_TILE);          // further operands: addresses in units of 16 bytes
+                if (elected()) {
 #pragma unroll
-                for (uint32_t c = 0; c < HD / 16; ++c)
+                    for (uint32_t c = 0; c < HD / 16; ++c)
 #pragma unroll
-                    for (uint32_t x = 0; x < QT; ++x)
-                        mma_ss_on(on, t_s + (G == 2 ? c / 4 * FL_KT : 0u), q + ((x * F::Q_TILE + (c / 4) * FLASH_ROWS * 128 + (c % 4) * 32) >> 4), k + (((c / 4) * FL_KT * 128 + (c % 4) * 32) >> 4), id_s,
-                                  (x == 0 && (G == 2 ? c % 4 : c) == 0) ? 0u : 1u);
-                tc_commit_on(on, b_s + 8 * (2 * st + buf));
+                        for (uint32_t x = 0; x < QT; ++x)
+                            mma_ss(t_s + (G == 2 ? c / 4 * FL_KT : 0u), q + ((x * F::Q_TILE + (c / 4) * FLASH_ROWS * 128 + (c % 4) * 32) >> 4), k + (((c / 4) * FL_KT * 128 + (c % 4) * 32) >> 4), id_s,
+                                   (x == 0 && (G == 2 ? c % 4 : c) == 0) ? 0u : 1u);
+                    tc_commit(b_s + 8 * (2 * st + buf));
+                }
+                __syncwarp();
                 return true;
             };
             ok = mbar_wait_warp(b_q, s & 1u, FL_WAIT, s_abort);
             for (uint32_t st = 0; ok && st < 2; ++st)
                 if (count[st] > 0) ok = scores(st, 0);
             for (uint32_t i = 0; ok && i < count[0]; ++i) {
+                auto next_scores = [&](uint32_t st) {
+                    if (G != 1 || i + 1 >= count[st]) return true;
+                    // the weights of tile i - 1 lie where S of tile i + 1 goes
+                    if (i >= 1 && !mbar_wait_warp(b_o + 8 * st, (done[st] + i - 1) & 1u, FL_WAIT, s_abort)) return false;
+                    return scores(st, i + 1);
+                };
+                // Streams over the same tiles: both next scores ahead of either's values, since a stream that waits for the other's weights
+                // here holds both back; tiles i and i + 1 are in use.  Streams of even and odd tiles: one after the other, which needs
+                // three tiles, 2 i .. 2 i + 2 (both ahead would need four, and wait for ever for the fourth).
+                for (uint32_t st = 0; ok && !f.halved && st < 2; ++st) ok = next_scores(st);
                 for (uint32_t st = 0; ok && st < 2; ++st) {
                     if (i >= count[st]) continue;
+                    if (f.halved) ok = next_scores(st);
+                    if (!ok) break;
                     const uint32_t use = done[st] + i, buf = G == 1 ? use & 1u : 0u, tile = tile_of(st, i), stage = tile % STAGES;
-                    if (G == 1 && i + 1 < count[st]) {
-                        // the weights of tile i - 1 lie where S of tile i + 1 goes
-                        if (i >= 1) ok = mbar_wait_warp(b_o + 8 * st, (use - 1) & 1u, FL_WAIT, s_abort);
-                        if (!ok) break;
-                        ok = scores(st, i + 1);
-                        if (!ok) break;
-                    }
                     ok = mbar_wait_warp(b_p + 8 * (2 * st + buf), (G == 1 ? use >> 1 : use) & 1u, FL_WAIT, s_abort);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t t_p = tmem + st * t_stream + buf * FL_KT, t_o = tmem + st * t_stream + 128;
                     const uint64_t v = desc_mn(s_k + stage * 2 * F::K_TILE + F::K_TILE, FL_KT * 128);
+                    if (elected()) {
 #pragma unroll
-                    for (uint32_t x = 0; x < G; ++x)
+                        for (uint32_t x = 0; x < G; ++x)
 #pragma unroll
-                        for (uint32_t y = 0; y < PT; ++y)
+                            for (uint32_t y = 0; y < PT; ++y)
 #pragma unroll
-                            for (uint32_t k = 0; k < FL_KT / 16; ++k)
-                                mma_ts_on(on, t_o + x * 64, t_p + (x * PT + y) * 32 + k * 8, v + ((x * FL_KT * 128 + k * 16 * 128) >> 4), id_o, (i | y | k) != 0 ? 1u : 0u);
-                    if (f.halved || st == 1) tc_commit_on(on, b_free + 8 * stage);
-                    tc_commit_on(on, b_o + 8 * st);
+                                for (uint32_t k = 0; k < FL_KT / 16; ++k)
+                                    mma_ts(t_o + x * 64, t_p + (x * PT + y) * 32 + k * 8, v + ((x * FL_KT * 128 + k * 16 * 128) >> 4), id_o, (i | y | k) != 0 ? 1u : 0u);
+                        if (f.halved || st == 1) tc_commit(b_free + 8 * stage);
+                        tc_commit(b_o + 8 * st);
+                    }
+                    __syncwarp();
                 }
                 if (G == 2)
                     for (uint32_t st = 0; ok && st < 2; ++st)
@@ -382,12 +384,13 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
                             ok = scores(st, i + 1);
                         }
             }
-            tc_commit_on(on, b_end);
+            if (elected()) tc_commit(b_end);
+            __syncwarp();
             n0 += n;
             done[0] += count[0];
             done[1] += count[1];
         }
-        tc_commit_on(on, b_last);               // also after a wait that gave up: the products in flight end before the CTA leaves
+        if (elected()) tc_commit(b_last);               // also after a wait that gave up: the products in flight end before the CTA leaves
         for (uint32_t spin = 0; spin < FL_WAIT && !mbar_try_wait(b_last, 0); ++spin) {}
         if (!ok && lane == 0) atomicCAS(p.a.pool.err, 0u, 1u);
     } else {
