@@ -222,7 +222,8 @@ template <int HD, int QT, int NR> __device__ __forceinline__ void get_queries(ui
     }
 }
 
-// o[r][j]: elements n HD / 8 + 2 j and the next, of query rows 8 r + 2 t and the next; m, l of those rows (l of the lane's positions)
+// o[r][j]: elements n HD / 8 + 2 j and the next (two groups of 64: n 8 + 2 j of the first, for j >= 4 of the second), of query rows 8 r + 2 t and
+// the next; m, l of those rows (l of the lane's positions)
 template <int HD, int NR> struct State {
     float o[NR][HD / 16][4], m[NR][2], l[NR][2];
 };
@@ -237,10 +238,12 @@ template <int HD, int BITS> struct LanePlaces {
         const uint32_t n = lane >> 2, t = lane & 3u, p0 = 4 * (n >> 1) + (n & 1u);
         k[0] = row_place<RB>(p0, t * (BITS == 8 ? 16 : 8));
         k[1] = RB == 32 || HD == 64 ? row_place<RB>(p0 + 2, t * (BITS == 8 ? 16 : 8)) : row_place<RB>(p0, RB / 2 + t * (BITS == 8 ? 16 : 8));
-        v[0] = B::V_AT + row_place<RB>(4 * t, n * (RB / 8));
-        v[1] = B::V_AT + row_place<RB>(4 * t + 1, n * (RB / 8));
+        v[0] = B::V_AT + row_place<RB>(4 * t, n * (RB / 8 / B::G));
+        v[1] = B::V_AT + row_place<RB>(4 * t + 1, n * (RB / 8 / B::G));
     }
     __device__ __forceinline__ uint32_t key(uint32_t at, int j, int g) const { return HD == 64 ? at + k[j] : at + k[g] + j * 2 * RB; }          // row p0 + 2 j, group g
+    // row 4 t + i; the second group of 64 elements of a 4-bit row lies 32 bytes on, where no exclusive-or of the first reaches but its own
+    __device__ __forceinline__ uint32_t value2(uint32_t at, int i) const { return at + (v[i & 1] ^ 32u) + (i >> 1) * 2 * RB; }
     __device__ __forceinline__ uint32_t value(uint32_t at, int i) const { return RB == 32 ? at + (v[0] ^ (i * 32)) : at + v[i & 1] + (i >> 1) * 2 * RB; }          // row 4 t + i
 };
 
@@ -295,7 +298,10 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
     constexpr int W = HD / 32, VW = BITS == 8 ? W : W / 2;          // words of four elements; as they lie
     uint32_t vw[4][VW];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lds_words<VW>(place.value(at, i), vw[i]);
+    for (int i = 0; i < 4; ++i) {
+        lds_words<VW / G>(place.value(at, i), vw[i]);
+        if (G == 2) lds_words<VW / G>(place.value2(at, i), vw[i] + VW / 2);
+    }
     // constants of positions p0 and p0 + 2
     float ks[G][2], lv[2], iv[2], part[G][2];
 #pragma unroll
@@ -378,7 +384,7 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
                 }
             }
     }
-    // values: columns of the first operand are positions, two of them a word; rows n and n + 8 of tile j are elements n HD / 8 + 2 j, + 1
+    // values: columns of the first operand are positions, two of them a word; rows n and n + 8 of tile j are the elements of o[.][j]
     uint32_t v[4][W];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -398,16 +404,9 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-                // the elements of lanes n < 4 are the first group's: each group's weights meet the other group's rows as zeros
-                uint32_t a[4];
+            for (int r = 0; r < NR; ++r)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = G == 1 || (n >> 2) == (uint32_t)g ? (e == 0 ? first[i] : second[i]) : 0u;
-#pragma unroll
-                for (int r = 0; r < NR; ++r)
-#pragma unroll
-                    for (int y = 0; y < PT; ++y) mma_f16(st.o[r][2 * k + e], a, b[r][g][y][0], b[r][g][y][1]);
-            }
+                for (int y = 0; y < PT; ++y) mma_f16(st.o[r][2 * k + e], e == 0 ? first : second, b[r][G == 1 ? 0 : k / (W / 2)][y][0], b[r][G == 1 ? 0 : k / (W / 2)][y][1]);
     }
 }
 
@@ -552,9 +551,9 @@ __global__ void __launch_bounds__(SP_WARPS * 32, split_ctas(HD, BITS, QT == 2, P
             for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) st.l[r][e] += __shfl_xor_sync(0xffffffffu, st.l[r][e], o);
-                float *to = s_join + (warp * 8 + 2 * t4 + e) * S::PITCH + n * (HD / 8);
+                float *to = s_join + (warp * 8 + 2 * t4 + e) * S::PITCH + n * (HD / 8 / B::G);
 #pragma unroll
-                for (int j = 0; j < HD / 16; j += 2) *reinterpret_cast<float4 *>(to + 2 * j) = make_float4(st.o[r][j][e], st.o[r][j][2 + e], st.o[r][j + 1][e], st.o[r][j + 1][2 + e]);
+                for (int j = 0; j < HD / 16; j += 2) *reinterpret_cast<float4 *>(to + (B::G == 2 && j >= 4 ? 64 + 2 * (j - 4) : 2 * j)) = make_float4(st.o[r][j][e], st.o[r][j][2 + e], st.o[r][j + 1][e], st.o[r][j + 1][2 + e]);
                 if (n == 0) s_ml[warp * 8 + 2 * t4 + e] = make_float2(st.m[r][e], st.l[r][e]);
             }
             __syncthreads();

@@ -23,7 +23,10 @@ constexpr uint32_t FL_KT = 64, FL_SOFT = 8, FL_CONV = 4, FL_ISSUE = FL_SOFT + FL
 
 template <int HD, int BITS, int QT> struct Flash {
     using B = PoolBlock<HD, BITS>;
-    static constexpr uint32_t PD = HD / 64, G = B::G, STAGES = 3, RAWS = 3, BLOCKS = FL_KT / POOL_ROWS;
+    // two groups of 64 elements a row: with queries and weights of one half the groups' scales go into the codes, relative to the larger one (a
+    // rounding to 11 bits, like that of the queries); with two, each group has scores, weights and products of its own
+    static constexpr bool FOLD = B::G == 2 && QT == 1;
+    static constexpr uint32_t PD = HD / 64, G = FOLD ? 1 : B::G, STAGES = HD == 128 && BITS == 8 ? 3 : 4, RAWS = 3, BLOCKS = FL_KT / POOL_ROWS;          // what shared memory holds
     static constexpr uint32_t Q_TILE = PD * FLASH_ROWS * 128, K_TILE = PD * FL_KT * 128, RAW = (BLOCKS * B::BYTES + 127) / 128 * 128, CONST = G == 1 ? 24 : 48;        // bytes; CONST per pair of columns
     static constexpr uint32_t CONSTS = 1024, HEAD = (CONSTS + STAGES * (FL_KT / 2) * CONST + 1023) / 1024 * 1024;
     static constexpr uint32_t Q_AT = HEAD, K_AT = Q_AT + 2 * Q_TILE, RAW_AT = K_AT + STAGES * 2 * K_TILE, SMEM = RAW_AT + RAWS * RAW + 1024;          // two tiles of queries: of rows, or of terms
@@ -96,7 +99,8 @@ template <int HD, int BITS, int QT> struct Converter {
     using F = Flash<HD, BITS, QT>;
     static constexpr uint32_t STEP = 128 / B::RB, PER = F::BLOCKS / STEP;          // blocks between two of a thread; of a thread
     static_assert(FL_CONV == 4, "128 threads");
-    uint32_t ct, first, load_at, store_at, store_x;
+    uint32_t ct, first, load_at, store_at, store_x, row_in;
+    bool second;                 // of the row's two groups
     Expand ex;
 
     __device__ __forceinline__ explicit Converter(uint32_t thread) : ct(thread) {
@@ -112,48 +116,78 @@ template <int HD, int BITS, int QT> struct Converter {
         const uint32_t c0 = BITS == 8 ? chunk * 2 : chunk * 4;          // first 16-byte chunk of halves
         store_at = (c0 >> 3) * (FL_KT * 128) + row * 128;
         store_x = (c0 & 7u) ^ (row & 7u);
+        row_in = row;
+        second = c0 >= 8;
     }
-    __device__ __forceinline__ void expand(uint32_t at, const uint4 &w) const {          // `at`: the thread's row and panel
+    __device__ __forceinline__ void expand(uint32_t at, const uint4 &w, uint32_t factor) const {          // `at`: the thread's row and panel
         if (BITS == 8) {
             sts4(at + (store_x << 4), ex.halves_lo(w.x), ex.halves_hi(w.x), ex.halves_lo(w.y), ex.halves_hi(w.y));
             sts4(at + ((store_x ^ 1u) << 4), ex.halves_lo(w.z), ex.halves_hi(w.z), ex.halves_lo(w.w), ex.halves_hi(w.w));
         } else {
             const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+            auto scaled = [&](uint32_t h) {
+                if (!F::FOLD) return h;
+                const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&h), *reinterpret_cast<const __half2 *>(&factor));
+                return *reinterpret_cast<const uint32_t *>(&y);
+            };
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 const uint32_t lo = ex.centroids4(x[i]), hi = ex.centroids4(x[i] >> 16);
-                sts4(at + ((store_x ^ i) << 4), ex.halves_lo(lo), ex.halves_hi(lo), ex.halves_lo(hi), ex.halves_hi(hi));
+                sts4(at + ((store_x ^ i) << 4), scaled(ex.halves_lo(lo)), scaled(ex.halves_hi(lo)), scaled(ex.halves_lo(hi)), scaled(ex.halves_hi(hi)));
             }
         }
     }
-    // A raw tile at shared address `raw` becomes an operand tile; `seen`: whether position ct of it is in sight.
-    __device__ __forceinline__ void put(uint32_t raw, uint32_t s_tile, uint8_t *consts, bool seen) const {
+    // The thread's group's scale over the row's larger one, in both halves; 0 for a row of zeros and one that is out of sight or not finite.
+    __device__ __forceinline__ uint32_t factor_of(uint32_t scales, bool seen) const {
+        if (!F::FOLD) return 0;
+        const float a = __uint_as_float(scales << 16), b = __uint_as_float(scales & 0xFFFF0000u), top = fmaxf(a, b);
+        const float x = seen && top > 0.0f ? (second ? b : a) * rcp_approx(top) : 0.0f;
+        return half2_bits(x, x);
+    }
+    // A raw tile at shared address `raw` becomes an operand tile; in sight are the first `end` positions of blocks with their bit set.
+    __device__ __forceinline__ void put(uint32_t raw, uint32_t s_tile, uint8_t *consts, uint32_t blocks, uint32_t end) const {
+        const bool seen = (blocks >> (ct / POOL_ROWS % F::BLOCKS) & 1u) != 0 && ct < end;
         uint4 k[PER], v[PER];
 #pragma unroll
         for (uint32_t i = 0; i < PER; ++i) k[i] = lds4(raw + (first + i * STEP) * B::BYTES + load_at);
 #pragma unroll
         for (uint32_t i = 0; i < PER; ++i) v[i] = lds4(raw + (first + i * STEP) * B::BYTES + B::V_AT + load_at);
+        uint32_t kf[PER], vf[PER];
 #pragma unroll
-        for (uint32_t i = 0; i < PER; ++i) expand(s_tile + store_at + (first + i * STEP) * (POOL_ROWS * 128), k[i]);
+        for (uint32_t i = 0; i < PER; ++i) {
+            kf[i] = vf[i] = 0;
+            if (F::FOLD) {
+                const uint32_t b = first + i * STEP, at = raw + b * B::BYTES + row_in * 4;
+                const bool there = (blocks >> b & 1u) != 0 && b * POOL_ROWS + row_in < end;
+                kf[i] = factor_of(lds1(at + B::KS_AT), there);
+                vf[i] = factor_of(lds1(at + B::VS_AT), there);
+            }
+        }
 #pragma unroll
-        for (uint32_t i = 0; i < PER; ++i) expand(s_tile + F::K_TILE + store_at + (first + i * STEP) * (POOL_ROWS * 128), v[i]);
+        for (uint32_t i = 0; i < PER; ++i) expand(s_tile + store_at + (first + i * STEP) * (POOL_ROWS * 128), k[i], kf[i]);
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) expand(s_tile + F::K_TILE + store_at + (first + i * STEP) * (POOL_ROWS * 128), v[i], vf[i]);
         if (ct < FL_KT) {
-            constexpr uint32_t G = B::G;
+            constexpr uint32_t G = F::G;
             const uint32_t at = raw + ct / POOL_ROWS * B::BYTES, row = ct % POOL_ROWS;
             float ks[2], vs[2], lv = -INFINITY, iv = 0.0f, part[2] = {0.0f, 0.0f};
             if (BITS == 8) {
                 ks[0] = __uint_as_float(lds1(at + B::KS_AT + row * 4));
                 vs[0] = __uint_as_float(lds1(at + B::VS_AT + row * 4));
             } else {
-                const uint32_t a = lds1(at + B::KS_AT + (row * G & ~1u) * 2), b = lds1(at + B::VS_AT + (row * G & ~1u) * 2);          // one row's two groups, or two rows
-                const bool high = G == 1 && (row & 1u);
+                const uint32_t a = lds1(at + B::KS_AT + (row * B::G & ~1u) * 2), b = lds1(at + B::VS_AT + (row * B::G & ~1u) * 2);          // one row's two groups, or two rows
+                const bool high = B::G == 1 && (row & 1u);
                 ks[0] = __uint_as_float(high ? a & 0xFFFF0000u : a << 16); ks[1] = __uint_as_float(a & 0xFFFF0000u);
                 vs[0] = __uint_as_float(high ? b & 0xFFFF0000u : b << 16); vs[1] = __uint_as_float(b & 0xFFFF0000u);
+                if (F::FOLD) {                 // the larger one; all groups of a row are NaN or none
+                    ks[0] = fmaxf(ks[0], ks[1]);
+                    vs[0] = fmaxf(vs[0], vs[1]);
+                }
             }
             if (seen) {
-                // a row of zeros: 8-bit codes are 0, and two groups have a factor each; a single group of 4-bit codes, which has neither, is
+                // a row of zeros: 8-bit codes are 0, and two groups have factors; a single group of 4-bit codes, which has neither, is
                 // given a scale below everything that counts
-                const float top = G == 1 ? vs[0] : fmaxf(vs[0], vs[1]), u = vs[0] != vs[0] ? vs[0] : top == 0.0f ? (BITS == 4 && G == 1 ? 0x1p-100f : 1.0f) : top;
+                const float top = G == 1 ? vs[0] : fmaxf(vs[0], vs[1]), u = vs[0] != vs[0] ? vs[0] : top == 0.0f ? (BITS == 4 && B::G == 1 ? 0x1p-100f : 1.0f) : top;
                 lv = log2_approx(u);
                 iv = rcp_approx(u);
 #pragma unroll
@@ -304,8 +338,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
                 if (n >= STAGES) ok = mbar_wait_warp(b_free + 8 * stage, (n / STAGES - 1) & 1u, FL_WAIT, s_abort);
                 if (!ok) break;
                 const uint32_t blocks = reinterpret_cast<volatile uint32_t *>(smem + 528)[slot];
-                cv.put(s_raw + slot * F::RAW, s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST,
-                       (blocks >> (cv.ct / POOL_ROWS % F::BLOCKS) & 1u) != 0 && t * FL_KT + cv.ct < p.a.prefix_len);
+                cv.put(s_raw + slot * F::RAW, s_k + stage * 2 * F::K_TILE, smem + F::CONSTS + stage * (FL_KT / 2) * F::CONST, blocks, p.a.prefix_len - t * FL_KT);
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) {
@@ -349,13 +382,14 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
                     if (i >= 1 && !mbar_wait_warp(b_o + 8 * st, (done[st] + i - 1) & 1u, FL_WAIT, s_abort)) return false;
                     return scores(st, i + 1);
                 };
-                // Streams over the same tiles: both next scores ahead of either's values, since a stream that waits for the other's weights
-                // here holds both back; tiles i and i + 1 are in use.  Streams of even and odd tiles: one after the other, which needs
-                // three tiles, 2 i .. 2 i + 2 (both ahead would need four, and wait for ever for the fourth).
-                for (uint32_t st = 0; ok && !f.halved && st < 2; ++st) ok = next_scores(st);
+                // Both next scores ahead of either's values, since a stream that waits for the other's weights here holds both back.  Streams over
+                // the same tiles use tiles i and i + 1 then, streams of even and odd tiles 2 i .. 2 i + 3: with three stages these go one after
+                // the other (2 i .. 2 i + 2), or they would wait for ever for the fourth.
+                const bool both = !f.halved || STAGES >= 4;
+                for (uint32_t st = 0; ok && both && st < 2; ++st) ok = next_scores(st);
                 for (uint32_t st = 0; ok && st < 2; ++st) {
                     if (i >= count[st]) continue;
-                    if (f.halved) ok = next_scores(st);
+                    if (!both) ok = next_scores(st);
                     if (!ok) break;
                     const uint32_t use = done[st] + i, buf = G == 1 ? use & 1u : 0u, tile = tile_of(st, i), stage = tile % STAGES;
                     ok = mbar_wait_warp(b_p + 8 * (2 * st + buf), (G == 1 ? use >> 1 : use) & 1u, FL_WAIT, s_abort);
