@@ -533,8 +533,8 @@ typedef struct KronosCudaPoolAttention {
     size_t workspace_bytes;
 } KronosCudaPoolAttention;
 
-/* Bytes of workspace of an attention call of these sizes (select needs none); 0 for sizes that are refused.  Nothing in it has to be
- * cleared, and nothing is kept there from call to call. */
+/* Bytes of workspace of an attention call of these sizes (select needs none), with this prefix or without; 0 for sizes that are refused.
+ * Nothing in it has to be cleared, and nothing is kept there from call to call. */
 size_t kronos_cuda_kv_pool_workspace(const KronosCudaKvPool *pool, uint32_t heads, uint32_t n_tok, uint32_t prefix_len);
 
 /* out = softmax(scale q k^T) v over the prefix and the first lens[t] positions of the token's sequence.  A token that sees nothing gets

@@ -788,6 +788,7 @@ template <int HD, int BITS> cudaError_t split_launch(cudaStream_t s, const Split
 // Room for a call of these sizes whatever its table's width and choice (a line has the most partial results), and for one without a prefix.
 size_t pool_work_bytes(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint32_t prefix_len, uint32_t sm_count) {
     size_t most = 0;
+    if (n_tok == 0) return 0;
     for (uint32_t type : {TYPE_F32, TYPE_BF16, TYPE_F16})
         for (uint32_t prefix : {0u, prefix_len}) {
             PoolAttnArgs a{};

@@ -61,6 +61,7 @@ bool pool_attention(const PoolShape &d, const KronosCudaPoolAttention &c, int wh
     if (!c.lens || !c.pages) return no("NULL table or lengths");
     if (c.pages_stride < 1 || c.pages_stride > (1u << 27)) return no("pages_stride must be 1..2^27");
     if (c.prefix_len > 0x7fffffffu) return no("prefix too long");
+    if (((uint64_t)c.n_tok * c.heads / 64 + d.kv_heads) * (c.prefix_len / 64 + 1) >= 1ull << 32) return no("prefix too long for so many tokens");
     if (c.prefix_len > 0 && (chosen || !c.prefix_pages)) return no(chosen ? "chosen pages do not go with a prefix" : "prefix without its pages");
     if (!(c.scale >= 0.0f) || c.scale > 1e30f) return no("scale must be a number from 0 on (0: 1 / sqrt(head_dim))");
     if (chosen) {
@@ -223,7 +224,7 @@ int32_t kronos_cuda_kv_pool_load_dev(KronosCudaContext *ctx, KronosCudaKvPool *p
 }
 
 size_t kronos_cuda_kv_pool_workspace(const KronosCudaKvPool *pool, uint32_t heads, uint32_t n_tok, uint32_t prefix_len) {
-    if (!pool || heads < pool->view.d.kv_heads || heads % pool->view.d.kv_heads != 0 || n_tok > (1u << 20)) return 0;
+    if (!pool || heads < pool->view.d.kv_heads || heads % pool->view.d.kv_heads != 0 || heads / pool->view.d.kv_heads > 256 || n_tok > (1u << 20)) return 0;
     return pool_work_bytes(pool->view.d, heads, n_tok, prefix_len, pool->sm_count);
 }
 

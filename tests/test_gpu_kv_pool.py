@@ -370,6 +370,20 @@ def test_choice_among_equals_and_pages_that_are_not_finite(ctx):
     assert 3 not in c.select(q, [n], 19, 0, 1)[0, 0] and 3 not in c.select(-q, [n], 19, 0, 1)[0, 0]
 
 
+@pytest.mark.parametrize("tokens,pages", [(700, 30), (3, 6000), (1, 2000)])
+def test_choice_of_many_tokens_and_among_many_pages(ctx, tokens, pages):
+    """More (token, kv head) pairs than the SMs hold, and more pages than threads."""
+    page, n = 16, pages * 16 - 5
+    c = Cache(ctx, [n], 1, 64, 8, page, "f32", block_keys=True)
+    q, rng = c.queries(tokens, 2), np.random.default_rng(tokens)
+    lens = np.maximum(1, n - rng.integers(0, n // 2, tokens))
+    lens[0] = n
+    keys, scales = keys_of(c, 0)
+    got = c.select(q, lens, 24, 1, 2, seq=np.zeros(tokens, int))
+    for t in range(0, tokens, max(1, tokens // 12)):
+        assert np.array_equal(got[t], ref.select(q[t], keys, scales, -(-int(lens[t]) // page), 24, 1, 2)), t
+
+
 def test_block_key_of_a_page_that_is_used_again(ctx):
     """The last row of a page makes its key from the rows that lie there then, also when they came in several calls."""
     page = 32
@@ -428,6 +442,24 @@ def test_pages_and_slots_outside_the_pool_are_reported(ctx):
     with pytest.raises(KronosCudaError, match="outside the pool"):
         c.store(np.array([1 << 40]), np.ones((1, 1, 64), np.float32), np.ones((1, 1, 64), np.float32))
     assert np.array_equal(c.attend(q, lens), good)
+    ctx.synchronize()
+
+
+@pytest.mark.parametrize("seqs,heads", [(1, 4), (40, 4), (90, 4)])
+@pytest.mark.parametrize("d,bits", SHAPES)
+def test_bad_pages_of_a_prefix_are_out_of_sight(ctx, seqs, heads, d, bits):
+    """Few rows, one tile of them, two tiles; what is in sight stays right, and the call is reported."""
+    from kronos_2t_b200 import KronosCudaError
+    c = Cache(ctx, [5] * seqs, 1, d, bits, 16, "bf16", prefix=400)
+    q = c.queries(seqs, heads)
+    c.prefix_pages[[3, 11, 24]] = [-1, 1 << 20, 1 << 30]
+    got = c.attend(q, [5] * seqs)
+    with pytest.raises(KronosCudaError, match="outside the pool"):
+        ctx.synchronize()
+    keep = np.array([i for i in range(400) if i // 16 not in (3, 11, 24)])
+    c.far = tuple(x[keep] for x in c.far)
+    pick = np.arange(0, seqs, max(1, seqs // 3))
+    c.check(got[pick], q[pick], [5] * len(pick), pick)
     ctx.synchronize()
 
 

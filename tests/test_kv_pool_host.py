@@ -76,6 +76,30 @@ def test_choice_needs_block_keys():
     assert "block keys" in refusal(config(flags=0), arguments(chosen=4096, top=4, sinks=1, local=1), 2)
 
 
+def test_calls_without_a_token_need_nothing():
+    assert refusal(config(), arguments(n_tok=0, workspace=None, workspace_bytes=0)) is None
+    assert refusal(config(), arguments(n_tok=0, workspace=None, workspace_bytes=0, prefix_len=1000, prefix_pages=4096)) is None
+    assert refusal(config(), arguments(n_tok=0, workspace=None, workspace_bytes=0, chosen=4096, top=3), 1) is None
+    assert "prefix too long" in refusal(config(), arguments(n_tok=1 << 20, prefix_len=(1 << 31) - 1, prefix_pages=4096))
+
+
+@pytest.mark.parametrize("kv_heads,head_dim,bits,heads", [(4, 128, 8, 28), (1, 64, 4, 20), (8, 128, 4, 64), (3, 64, 8, 3)])
+def test_workspaces_cover_what_calls_need(kv_heads, head_dim, bits, heads):
+    """A call is refused one byte below the size that is asked for some type, never at it; with a prefix it is enough without one."""
+    f = internal("pool_work_bytes", C.c_size_t, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32)
+    shape = (C.c_uint32 * 6)(kv_heads, head_dim, bits, 6, 10, 1)
+    cfg = config(kv_heads=kv_heads, head_dim=head_dim, kv_bits=bits)
+    for n_tok in (1, 2, 3, 7, 40, 160, 2000):
+        for prefix in (0, 1, 500, 100000):
+            need = f(shape, heads, n_tok, prefix, 148)
+            assert need >= f(shape, heads, n_tok, 0, 148) > 0
+            for stride in (1, 3, 40, 5000):
+                for row_type in (0, 1, 2):
+                    a = dict(heads=heads, n_tok=n_tok, prefix_len=prefix, prefix_pages=4096, pages_stride=stride, row_type=row_type)
+                    assert refusal(cfg, arguments(**a, workspace_bytes=need)) is None
+                    assert "workspace too small" in refusal(cfg, arguments(**a, workspace_bytes=need - 1))
+
+
 def test_null_handles_are_tolerated():
     import kronos_2t_b200 as k2
     L = k2.load_library()
