@@ -35,25 +35,22 @@ __device__ __forceinline__ uint32_t four_bytes(uint32_t a, uint32_t b, uint32_t 
 // Byte i of w, which holds 128 + c, as c: 0x4B0000xx is 2^23 + xx.
 __device__ __forceinline__ float signed_byte(uint32_t w, uint32_t i) { return __fsub_rn(__uint_as_float(prmt(w, 0x4B000000u, 0x7540u + i)), 8388736.0f); }
 
-template <int LANES> __device__ __forceinline__ float max_over(float x) {        // of LANES neighbouring lanes
+// The largest magnitude of a row over LANES lanes, as bits: these are ordered as the magnitudes are, with infinities and NaN above all others.
+constexpr uint32_t INFINITE = 0x7F800000u;
+template <int LANES, int N> __device__ __forceinline__ uint32_t top_bits(const float (&v)[N]) {
+    uint32_t top = 0;
 #pragma unroll
-    for (int m = LANES / 2; m > 0; m >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
-    return x;
+    for (int i = 0; i < N; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+#pragma unroll
+    for (int m = LANES / 2; m > 0; m >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
+    return top;
 }
-template <int LANES> __device__ __forceinline__ bool any_over(bool b, uint32_t lane) {
-    return (__ballot_sync(0xffffffffu, b) >> (lane & ~(uint32_t)(LANES - 1)) & (0xffffffffu >> (32 - LANES))) != 0;
-}
-
 // A row over LANES lanes, eight values each, as 8-bit codes: what all quantised rows of 8 bits share.  `scale` is NaN for a row that is
 // not finite (its codes are 0).
-template <int LANES, int N> __device__ __forceinline__ void quantise8(const float (&v)[N], uint32_t lane, uint32_t (&code)[N], float &scale) {          // codes: the low bytes
-    float top = 0.0f;
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < N; ++i) { top = fmaxf(top, fabsf(v[i])); bad |= not_finite(v[i]); }
-    bad = any_over<LANES>(bad, lane);
-    top = max_over<LANES>(top);
-    const bool zero = top <= SMALLEST || bad;
+template <int LANES, int N> __device__ __forceinline__ void quantise8(const float (&v)[N], uint32_t (&code)[N], float &scale) {          // codes: the low bytes
+    const uint32_t bits = top_bits<LANES>(v);
+    const float top = __uint_as_float(bits);
+    const bool bad = bits >= INFINITE, zero = bad || top <= SMALLEST;
     const float inv = zero ? 0.0f : __fdiv_rn(127.0f, top);
 #pragma unroll
     for (int i = 0; i < N; ++i) code[i] = rounded_byte(bad ? 0.0f : __fmul_rn(v[i], inv));
@@ -88,18 +85,15 @@ template <int HD, int BITS> __device__ __forceinline__ void put_row(const PoolSt
     if (BITS == 8) {
         uint32_t c[8];
         float scale;
-        quantise8<LANES>(v, lane, c, scale);
+        quantise8<LANES>(v, c, scale);
         if (block == nullptr) return;
         *reinterpret_cast<uint2 *>(block + value * B::V_AT + row_place<B::RB>(row, l * 8)) =
             make_uint2(four_bytes(c[0], c[1], c[2], c[3]) ^ 0x80808080u, four_bytes(c[4], c[5], c[6], c[7]) ^ 0x80808080u);
         if (l == 0) reinterpret_cast<float *>(block + (value ? B::VS_AT : B::KS_AT))[row] = scale;
     } else {
-        float top = 0.0f;
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { top = fmaxf(top, fabsf(v[i])); bad |= not_finite(v[i]); }
-        bad = any_over<LANES>(bad, lane);            // of the whole row: its groups stand or fall together
-        top = max_over<8>(top);
+        const uint32_t bits = top_bits<8>(v), row_bits = LANES == 8 ? bits : max(bits, __shfl_xor_sync(0xffffffffu, bits, 8));
+        const float top = __uint_as_float(bits);
+        const bool bad = row_bits >= INFINITE;            // of the whole row: its groups stand or fall together
         const bool zero = top < 1e-30f || bad;
         const float inv0 = zero ? 0.0f : __fdiv_rn(127.0f, top);
         float rc[8], den = 0.0f, num = 0.0f;
@@ -140,7 +134,8 @@ template <int HD, int BITS> __device__ __forceinline__ void put_row(const PoolSt
 template <int HD, int BITS, uint32_t ROW_AHEAD> __global__ void __launch_bounds__(ROW_THREADS) pool_store_kernel(const __grid_constant__ PoolStoreArgs a) {
     using B = PoolBlock<HD, BITS>;
     constexpr uint32_t LANES = HD / 8, STEP = ROW_THREADS / LANES;
-    const uint32_t lane = threadIdx.x & 31, l = lane % LANES, signs = signs8(a.pool, l * 8), rows = a.n_tok * 2 * a.pool.d.kv_heads;
+    const uint32_t lane = threadIdx.x & 31, l = lane % LANES, rows = a.n_tok * 2 * a.pool.d.kv_heads;
+    const Eighths signs(signs8(a.pool, l * 8));
     const uint32_t r0 = blockIdx.x * (STEP * ROW_AHEAD) + threadIdx.x / LANES;
     pdl_wait();
     pdl_trigger();
@@ -191,7 +186,8 @@ template <int HD, int BITS, int N> struct Stored {
 template <int HD, int BITS, uint32_t ROW_AHEAD> __global__ void __launch_bounds__(ROW_THREADS) pool_load_kernel(const __grid_constant__ PoolStoreArgs a) {
     using B = PoolBlock<HD, BITS>;
     constexpr uint32_t LANES = HD / 8, STEP = ROW_THREADS / LANES;
-    const uint32_t lane = threadIdx.x & 31, l = lane % LANES, signs = signs8(a.pool, l * 8), rows = a.n_tok * 2 * a.pool.d.kv_heads;
+    const uint32_t lane = threadIdx.x & 31, l = lane % LANES, rows = a.n_tok * 2 * a.pool.d.kv_heads;
+    const Eighths signs(signs8(a.pool, l * 8));
     const uint32_t r0 = blockIdx.x * (STEP * ROW_AHEAD) + threadIdx.x / LANES;
     const Expand ex;
     pdl_wait();
@@ -262,7 +258,7 @@ template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_
         for (int k = 0; k < N; ++k) sum[k] = __fmul_rn(sum[k], part);
         uint32_t c[N];
         float scale;
-        quantise8<32>(sum, lane, c, scale);
+        quantise8<32>(sum, c, scale);
         int8_t *to = a.pool.block_keys + (page * kh + head) * HD + lane * N;
         if constexpr (N == 4) *reinterpret_cast<uint32_t *>(to) = four_bytes(c[0], c[1], c[2], c[3]);
         else *reinterpret_cast<uint16_t *>(to) = (uint16_t)prmt(c[0], c[1], 0x0040u);
@@ -363,7 +359,7 @@ template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_TH
         transform8(v, signs8(a.pool, l * 8), lane);
         uint32_t c[8];
         float unused;
-        quantise8<LANES>(v, lane, c, unused);
+        quantise8<LANES>(v, c, unused);
         if (lane < LANES) *reinterpret_cast<uint2 *>(s_q + l * 8) = make_uint2(four_bytes(c[0], c[1], c[2], c[3]), four_bytes(c[4], c[5], c[6], c[7]));
     }
     __syncthreads();

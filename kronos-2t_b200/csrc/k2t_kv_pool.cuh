@@ -123,7 +123,29 @@ template <int N> __device__ __forceinline__ void butterflies_across(float (&v)[N
 }
 __device__ __forceinline__ float flip(float x, uint32_t signs, int i) { return __uint_as_float(__float_as_uint(x) ^ (signs << (31 - i) & 0x80000000u)); }         // by bit i
 
+// The signs of eight elements times 1/8: one product instead of a shift, an exclusive-or and a product, for kernels that transform several rows.
+struct Eighths {
+    float f[8];
+    __device__ __forceinline__ explicit Eighths(uint32_t signs) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = flip(0.125f, signs, i);
+    }
+};
 // Eight lanes hold 64 values, eight each; (1/8) H64 D x, butterflies in the order 1, 2, .. 32.
+__device__ __forceinline__ void transform8(float (&v)[8], const Eighths &e, uint32_t lane) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], e.f[i]);
+    butterflies_in(v);
+#pragma unroll
+    for (uint32_t m = 1; m < 8; m <<= 1) butterflies_across(v, m, lane);
+}
+__device__ __forceinline__ void transform8_back(float (&v)[8], const Eighths &e, uint32_t lane) {
+    butterflies_in(v);
+#pragma unroll
+    for (uint32_t m = 1; m < 8; m <<= 1) butterflies_across(v, m, lane);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], e.f[i]);
+}
 __device__ __forceinline__ void transform8(float (&v)[8], uint32_t signs, uint32_t lane) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(flip(v[i], signs, i), 0.125f);
@@ -139,8 +161,6 @@ __device__ __forceinline__ void transform8_back(float (&v)[8], uint32_t signs, u
     for (int i = 0; i < 8; ++i) v[i] = flip(__fmul_rn(v[i], 0.125f), signs, i);
 }
 __device__ __forceinline__ uint32_t signs8(const PoolView &p, uint32_t at) { return p.signs[at >> 5] >> (at & 31u) & 0xFFu; }
-
-__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) == 0x7F800000u; }
 
 __device__ __forceinline__ uint32_t half2_bits(float x, float y) { const __half2 h = __floats2half2_rn(x, y); return *reinterpret_cast<const uint32_t *>(&h); }
 __device__ __forceinline__ uint32_t hsub2(uint32_t x, uint32_t y) {
