@@ -737,9 +737,11 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     const PoolShape &d = a.pool.d;
     const uint32_t group = a.heads / d.kv_heads;
     const uint32_t rows = a.n_tok * group;
-    // More rows than a tile of this kernel: k2t_pool_flash.cu.  Its start costs more, but it expands a cached row once for 128 or 256 query rows
-    // where this one does for 16 (24 sequences x 7 heads behind 500 / 4000 / 16000 positions, the whole call: 19 / 31 / 53 us here, 24 / 28 / 39 there).
-    p.flash.on = a.prefix_len > 0 && rows > 16;
+    // More rows than a tile of this kernel: k2t_pool_flash.cu, which expands a cached row once for 128 or 256 query rows where this one does for
+    // 16.  Its start costs more, so it takes FLASH_WORK tiles of 16 rows x 16 positions and up (24 sequences x 28 heads over 4 kv heads behind
+    // 500 / 1000 / 4000 / 16000 positions, the whole call: 19 / 24 / 31 / 53 us here, 24 / 25 / 28 / 39 there).
+    constexpr uint64_t FLASH_WORK = 2048;
+    p.flash.on = a.prefix_len > 0 && rows > 16 && (uint64_t)((rows + 15) / 16) * d.kv_heads * prefix_blocks(p) >= FLASH_WORK;
     if (p.flash.on) {
         FlashArgs &f = p.flash;
         f.halved = rows <= FLASH_ROWS || type != TYPE_BF16;

@@ -6,7 +6,7 @@ namespace k2t {
 
 // The prefix over many rows (k2t_pool_flash.cu): items are (kv head, 2 FLASH_ROWS rows), tiles of 64 positions; a line of items * tiles, `part` of it
 // a CTA.  halved: an item has FLASH_ROWS rows, and its tiles are dealt out to two streams over the same rows.
-constexpr uint32_t FLASH_ROWS = 128, FLASH_MIN_PART = 2;
+constexpr uint32_t FLASH_ROWS = 128, FLASH_MIN_PART = 2;          // tiles of a CTA at least (2 against 4: 24 against 25 us behind 2000 positions)
 struct FlashArgs {
     bool on, halved;
     uint32_t items, row_tiles, tiles, part;

@@ -230,8 +230,8 @@ def test_attention_behind_a_shared_prefix(ctx, d, bits, dtype, prefix, kh, heads
 
 
 @pytest.mark.parametrize("d,bits", SHAPES)
-@pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("prefix,kh,heads,seqs", [(3001, 8, 64, 40), (2500, 5, 5, 100), (9000, 1, 6, 45)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("prefix,kh,heads,seqs", [(3001, 8, 64, 40), (2500, 5, 5, 100), (9000, 1, 6, 45), (20000, 2, 2, 17)])
 def test_a_prefix_over_many_rows(ctx, d, bits, dtype, prefix, kh, heads, seqs):
     """Rows of several tiles, parts that begin and end inside an item, and items of one tile of rows."""
     rng = np.random.default_rng(seqs)
@@ -445,40 +445,41 @@ def test_pages_and_slots_outside_the_pool_are_reported(ctx):
     ctx.synchronize()
 
 
-@pytest.mark.parametrize("seqs,heads", [(1, 4), (40, 4), (90, 4)])
+@pytest.mark.parametrize("seqs,heads,prefix", [(1, 4, 400), (40, 4, 400), (25, 4, 5000), (90, 4, 1600)])
 @pytest.mark.parametrize("d,bits", SHAPES)
-def test_bad_pages_of_a_prefix_are_out_of_sight(ctx, seqs, heads, d, bits):
+def test_bad_pages_of_a_prefix_are_out_of_sight(ctx, seqs, heads, prefix, d, bits):
     """Few rows, one tile of them, two tiles; what is in sight stays right, and the call is reported."""
     from kronos_2t_b200 import KronosCudaError
-    c = Cache(ctx, [5] * seqs, 1, d, bits, 16, "bf16", prefix=400)
+    c = Cache(ctx, [5] * seqs, 1, d, bits, 16, "bf16", prefix=prefix)
     q = c.queries(seqs, heads)
     c.prefix_pages[[3, 11, 24]] = [-1, 1 << 20, 1 << 30]
     got = c.attend(q, [5] * seqs)
     with pytest.raises(KronosCudaError, match="outside the pool"):
         ctx.synchronize()
-    keep = np.array([i for i in range(400) if i // 16 not in (3, 11, 24)])
+    keep = np.array([i for i in range(prefix) if i // 16 not in (3, 11, 24)])
     c.far = tuple(x[keep] for x in c.far)
     pick = np.arange(0, seqs, max(1, seqs // 3))
     c.check(got[pick], q[pick], [5] * len(pick), pick)
     ctx.synchronize()
 
 
-def test_the_same_call_gives_the_same_bits_also_captured_and_on_another_stream(ctx):
+@pytest.mark.parametrize("prefix", [600, 20000])
+def test_the_same_call_gives_the_same_bits_also_captured_and_on_another_stream(ctx, prefix):
     """Two graphs with a workspace each, replayed in turn with new lengths and queries in place."""
     import torch
     lens = [900, 17, 300, 0]
-    c = Cache(ctx, lens, 2, 128, 8, 64, "bf16", prefix=600)
+    c = Cache(ctx, lens, 2, 128, 8, 64, "bf16", prefix=prefix)
     q = [c.queries(4, 16) for _ in range(2)]
     want = [c.attend(x, lens) for x in q]
     assert np.array_equal(want[0], c.attend(q[0], lens))
     stream = torch.cuda.Stream()
     dl, dt, far = device(np.array(lens, np.int32)), device(c.table), device(c.prefix_pages)
     dq, out = [device(x, "bf16") for x in q], [torch.zeros(4, 16, 128, dtype=torch.bfloat16, device="cuda") for _ in q]
-    work = [torch.empty(c.pool.workspace_bytes(16, 4, 600), dtype=torch.uint8, device="cuda") for _ in q]
+    work = [torch.empty(c.pool.workspace_bytes(16, 4, prefix), dtype=torch.uint8, device="cuda") for _ in q]
 
     def call(i):
         c.pool.attend_dev("bf16", 16, 4, dq[i].data_ptr(), dl.data_ptr(), dt.data_ptr(), dt.shape[1], out[i].data_ptr(), (work[i].data_ptr(), work[i].numel()),
-                          d_prefix_pages=far.data_ptr(), prefix_len=600)
+                          d_prefix_pages=far.data_ptr(), prefix_len=prefix)
     torch.cuda.synchronize()
     ctx.set_stream(stream.cuda_stream)
     try:
