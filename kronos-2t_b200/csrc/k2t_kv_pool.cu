@@ -69,8 +69,8 @@ __device__ __forceinline__ uint8_t *block_of(const PoolView &p, int64_t slot, ui
 
 // ------------------------------------------------------------------------------------------------ rows in, rows out
 // head_dim / 8 lanes hold a row, eight values each; rows are numbered (token, keys | values, head).  A thread has its part of ROW_AHEAD rows on
-// the way at a time: four, or one where the rows are too few to fill the SMs even so (a decode batch: the rows of a thread would only follow
-// one another).
+// the way at a time: two (16384 tokens x 8 heads of 128 written and read: one 98, two 95.6, four 96.9 us; 4001 x 32 of 64, 4 bits: 65, 63, 67), or one
+// where the rows are too few to fill the SMs even so (a decode batch of 96 tokens: two kernels 4.4 us, 9.8 with four, which only follow one another).
 constexpr uint32_t ROW_THREADS = 256;
 struct RowAt { uint32_t t, value, head; };
 __device__ __forceinline__ RowAt row_at(const PoolStoreArgs &a, uint32_t r) {          // r below 2^31: a division by a multiplication (and a shift) that is exact there
@@ -463,7 +463,7 @@ PoolStoreArgs divided(PoolStoreArgs a) {
 template <int HD, int BITS> cudaError_t store_rows(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched) {
     *launched += 1;
     const cudaError_t e = few_rows(a) ? launch_kernel(pool_store_kernel<HD, BITS, 1>, dim3(row_ctas(a, 1)), dim3(ROW_THREADS), 0, s, true, a)
-                                      : launch_kernel(pool_store_kernel<HD, BITS, 4>, dim3(row_ctas(a, 4)), dim3(ROW_THREADS), 0, s, true, a);
+                                      : launch_kernel(pool_store_kernel<HD, BITS, 2>, dim3(row_ctas(a, 2)), dim3(ROW_THREADS), 0, s, true, a);
     if (e != cudaSuccess || !a.pool.d.block_keys) return e;
     const uint64_t warps = ((uint64_t)a.n_tok + 31) / 32 * a.pool.d.kv_heads;
     *launched += 1;
@@ -472,7 +472,7 @@ template <int HD, int BITS> cudaError_t store_rows(cudaStream_t s, const PoolSto
 template <int HD, int BITS> cudaError_t load_rows(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched) {
     *launched += 1;
     return few_rows(a) ? launch_kernel(pool_load_kernel<HD, BITS, 1>, dim3(row_ctas(a, 1)), dim3(ROW_THREADS), 0, s, true, a)
-                       : launch_kernel(pool_load_kernel<HD, BITS, 4>, dim3(row_ctas(a, 4)), dim3(ROW_THREADS), 0, s, true, a);
+                       : launch_kernel(pool_load_kernel<HD, BITS, 2>, dim3(row_ctas(a, 2)), dim3(ROW_THREADS), 0, s, true, a);
 }
 
 }  // namespace
