@@ -252,7 +252,7 @@ template <int HD, int BITS, int QT, int PT, int NR>
 __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t lane, const LanePlaces<HD, BITS> &place, const Expand &ex, const Query<HD, QT, NR> &q, State<HD, NR> &st) {
     using B = PoolBlock<HD, BITS>;
     constexpr int G = B::G;
-    const uint32_t n = lane >> 2, t = lane & 3u;
+    const uint32_t n = lane >> 2;
     // Row i of the products is position 4 (i / 2) + i % 2 for the first eight, two further for the others: the lane has rows n and n + 8.
     const uint32_t p0 = 4 * (n >> 1) + (n & 1u);
     float s[NR][G][4];                     // rows n, n + 8 of queries 2 t, 2 t + 1, of each group of 64 elements that has a scale

@@ -21,7 +21,7 @@ __host__ __device__ constexpr uint32_t flash_slot_floats(uint32_t head_dim) { re
 // A partial result: rows x head_dim numerators, then (maximum, denominator) of each row.
 struct SplitArgs {
     PoolAttnArgs a;
-    uint32_t tile, rbo, rbp;     // query rows of a CTA, 8 or 16; tiles of a token and kv head; of the prefix (0: the line holds none)
+    uint32_t tile, rbo, rbp;     // query rows of a CTA, 8 or 16; tiles of a token and kv head; of the prefix (0: not in this kernel)
     uint32_t units, pieces;      // CTAs for own rows; of an item, or 0: the line of all items' blocks is cut into parts
     uint32_t near_units, near_pieces;          // CTAs for the prefix, before them; of an item
     float *own, *near;           // partial results of own rows; of the prefix
