@@ -89,9 +89,10 @@ inline cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block
 
 // Raises a kernel's dynamic shared-memory limit once per (kernel, device) instead of on every launch: the value set so
 // far is remembered per device, and cudaFuncSetAttribute is called only for a larger request.  (The attribute belongs
-// to the function on the current device, so a process that drives several GPUs sets it on each.)
+// to the function on the current device, so a process that drives several GPUs sets it on each.)  Without it a launch may have
+// 48 KB of static and dynamic shared memory TOGETHER; kernels have less than 32 KB of static (the largest 18 KB), so up to 16 KB need nothing.
 inline cudaError_t allow_dynamic_smem(const void *kernel, size_t bytes) {
-    if (bytes <= 48 * 1024) return cudaSuccess;
+    if (bytes <= 16 * 1024) return cudaSuccess;
     constexpr int MAX_DEV = 16, SLOTS = 256;
     struct Entry { const void *fn; size_t bytes[MAX_DEV]; };
     static Entry table[SLOTS] = {};
