@@ -173,6 +173,12 @@ __device__ __forceinline__ float rcp_approx(float x) { float y; asm("rcp.approx.
 __device__ __forceinline__ int query_exponent(float top) { return min(126, max(-126, 140 - (int)((__float_as_uint(top) >> 23) & 255u))); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// The scale of a value row in the exponents of its weights.  A row of zeros, which has the scale 0, takes one below all that count, so that the
+// running maximum is that of the rows an output is made of, however much of the weight the zeros have.  Exponentials reach down to 2^-126, so a
+// zero row counts beside values of scales up to 2^62; 4-bit rows with scales below 2^-64 have those as factors of it.  NaN stays NaN.
+constexpr float LEAST_SCALE = 0x1p-64f;
+__device__ __forceinline__ float weight_scale(float scale) { return scale < LEAST_SCALE ? LEAST_SCALE : scale; }
+
 // Constants of the expansion, kept in registers: left to the compiler they are loaded again for every use where registers are short.
 struct Expand {
     uint32_t exponent, hi0, hi1, lo0, lo1;

@@ -2,6 +2,7 @@
 //   score t_ij = (c_i q_i . code_j) ks_j, kept as x_ij = t_ij + log2 vs_j, so that 2^x is the weight already times the value's scale and
 //   every operand of a product is a code (whole numbers up to 127, exact halves) or a weight of at most 2^8;
 //   numerator O_i = sum_j 2^(x_ij - m_i) codev_j, denominator l_i = sum_j 2^(x_ij - m_i) / vs_j, with the running maximum m_i of x.
+// Rows of zeros have vs = 2^-64 (see weight_scale): with 1 they took the digits of the others' weights, which are all of the output.
 // Positions out of sight have ks = 0, log2 vs = -inf, 1 / vs = 0: no mask per element, and nothing of theirs is multiplied.
 //
 // A CTA works with 8 or 16 query rows (queries of one kv head, so a cached row is read once for the heads that share it).  Its four warps
@@ -318,8 +319,8 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
             ks[0][j] = __uint_as_float(pos & 1u ? sc[0][j] & 0xFFFF0000u : sc[0][j] << 16);
             v[0] = __uint_as_float(pos & 1u ? sc[1][j] & 0xFFFF0000u : sc[1][j] << 16);
         }
-        top = G == 1 ? v[0] : fmaxf(v[0], v[G - 1]);          // scales are not negative, and all groups of a row are NaN or none
-        if (top == 0.0f) top = 1.0f;               // a row of zeros: 8-bit codes are 0, groups of 4 bits have a factor
+        // scales are not negative, and all groups of a row are NaN or none; of a row of zeros 8-bit codes are 0, groups of 4 bits have a factor
+        top = weight_scale(G == 1 ? v[0] : fmaxf(v[0], v[G - 1]));
         if (pos < valid) {
             lv[j] = log2_approx(top);
             iv[j] = rcp_approx(top);

@@ -119,14 +119,15 @@ template <int HD, int BITS, int QT> struct Converter {
         row_in = row;
         second = c0 >= 8;
     }
-    __device__ __forceinline__ void expand(uint32_t at, const uint4 &w, uint32_t factor) const {          // `at`: the thread's row and panel
+    static constexpr bool SCALED = BITS == 4 && F::G == 1;          // values of 4 bits whose weights have no factor per group
+    template <bool FACTOR> __device__ __forceinline__ void expand(uint32_t at, const uint4 &w, uint32_t factor) const {          // `at`: the thread's row and panel
         if (BITS == 8) {
             sts4(at + (store_x << 4), ex.halves_lo(w.x), ex.halves_hi(w.x), ex.halves_lo(w.y), ex.halves_hi(w.y));
             sts4(at + ((store_x ^ 1u) << 4), ex.halves_lo(w.z), ex.halves_hi(w.z), ex.halves_lo(w.w), ex.halves_hi(w.w));
         } else {
             const uint32_t x[4] = {w.x, w.y, w.z, w.w};
             auto scaled = [&](uint32_t h) {
-                if (!F::FOLD) return h;
+                if (!FACTOR) return h;
                 const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&h), *reinterpret_cast<const __half2 *>(&factor));
                 return *reinterpret_cast<const uint32_t *>(&y);
             };
@@ -137,11 +138,11 @@ template <int HD, int BITS, int QT> struct Converter {
             }
         }
     }
-    // The thread's group's scale over the row's larger one, in both halves; 0 for a row of zeros and one that is out of sight or not finite.
-    __device__ __forceinline__ uint32_t factor_of(uint32_t scales, bool seen) const {
-        if (!F::FOLD) return 0;
-        const float a = __uint_as_float(scales << 16), b = __uint_as_float(scales & 0xFFFF0000u), top = fmaxf(a, b);
-        const float x = seen && top > 0.0f ? (second ? b : a) * rcp_approx(top) : 0.0f;
+    // The thread's group's scale over the one that the row has in its column's constants (the larger one; of values weight_scale of it), in both
+    // halves; 0 for a row of zeros and one that is out of sight or not finite.  Of a single group 1, or 0 and little more.
+    __device__ __forceinline__ uint32_t factor_of(uint32_t scales, bool seen, bool value) const {
+        const float a = __uint_as_float(scales << 16), b = __uint_as_float(scales & 0xFFFF0000u), mine = (F::FOLD ? second : (row_in & 1u) != 0) ? b : a, top = F::FOLD ? fmaxf(a, b) : mine;
+        const float x = seen && top > 0.0f ? mine * rcp_approx(value ? weight_scale(top) : top) : 0.0f;
         return half2_bits(x, x);
     }
     // A raw tile at shared address `raw` becomes an operand tile; in sight are the first `end` positions of blocks with their bit set.
@@ -156,17 +157,17 @@ template <int HD, int BITS, int QT> struct Converter {
 #pragma unroll
         for (uint32_t i = 0; i < PER; ++i) {
             kf[i] = vf[i] = 0;
-            if (F::FOLD) {
-                const uint32_t b = first + i * STEP, at = raw + b * B::BYTES + row_in * 4;
+            if (SCALED) {
+                const uint32_t b = first + i * STEP, at = raw + b * B::BYTES + (row_in * B::G & ~1u) * 2;          // one row's two groups, or two rows
                 const bool there = (blocks >> b & 1u) != 0 && b * POOL_ROWS + row_in < end;
-                kf[i] = factor_of(lds1(at + B::KS_AT), there);
-                vf[i] = factor_of(lds1(at + B::VS_AT), there);
+                if (F::FOLD) kf[i] = factor_of(lds1(at + B::KS_AT), there, false);
+                vf[i] = factor_of(lds1(at + B::VS_AT), there, true);
             }
         }
 #pragma unroll
-        for (uint32_t i = 0; i < PER; ++i) expand(s_tile + store_at + (first + i * STEP) * (POOL_ROWS * 128), k[i], kf[i]);
+        for (uint32_t i = 0; i < PER; ++i) expand<F::FOLD>(s_tile + store_at + (first + i * STEP) * (POOL_ROWS * 128), k[i], kf[i]);
 #pragma unroll
-        for (uint32_t i = 0; i < PER; ++i) expand(s_tile + F::K_TILE + store_at + (first + i * STEP) * (POOL_ROWS * 128), v[i], vf[i]);
+        for (uint32_t i = 0; i < PER; ++i) expand<SCALED>(s_tile + F::K_TILE + store_at + (first + i * STEP) * (POOL_ROWS * 128), v[i], vf[i]);
         if (ct < FL_KT) {
             constexpr uint32_t G = F::G;
             const uint32_t at = raw + ct / POOL_ROWS * B::BYTES, row = ct % POOL_ROWS;
@@ -185,9 +186,7 @@ template <int HD, int BITS, int QT> struct Converter {
                 }
             }
             if (seen) {
-                // a row of zeros: 8-bit codes are 0, and two groups have factors; a single group of 4-bit codes, which has neither, is
-                // given a scale below everything that counts
-                const float top = G == 1 ? vs[0] : fmaxf(vs[0], vs[1]), u = vs[0] != vs[0] ? vs[0] : top == 0.0f ? (BITS == 4 && B::G == 1 ? 0x1p-100f : 1.0f) : top;
+                const float u = weight_scale(G == 1 ? vs[0] : fmaxf(vs[0], vs[1]));          // of zeros 8-bit codes are 0, 4-bit ones have factors
                 lv = log2_approx(u);
                 iv = rcp_approx(u);
 #pragma unroll
