@@ -179,6 +179,10 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 constexpr float LEAST_SCALE = 0x1p-64f;
 __device__ __forceinline__ float weight_scale(float scale) { return scale < LEAST_SCALE ? LEAST_SCALE : scale; }
 
+// A running maximum m stands 7 below the largest exponent that it was set by and follows where one has come 15 above it, so that weights are up to 2^15
+// (halves reach 2^16) and those down to 2^-21 of the largest are ordinary halves: the grid of 2^-24 below is 2^-31 of it or finer.
+constexpr float MAX_BELOW = 7.0f, MAX_ROOM = 15.0f;
+
 // Constants of the expansion, kept in registers: left to the compiler they are loaded again for every use where registers are short.
 struct Expand {
     uint32_t exponent, hi0, hi1, lo0, lo1;

@@ -1,6 +1,6 @@
 // Attention over the pool for few query rows at a time: tables of pages, chosen pages, and a shared prefix with up to a tile of rows.
 //   score t_ij = (c_i q_i . code_j) ks_j, kept as x_ij = t_ij + log2 vs_j, so that 2^x is the weight already times the value's scale and
-//   every operand of a product is a code (whole numbers up to 127, exact halves) or a weight of at most 2^8;
+//   every operand of a product is a code (whole numbers up to 127, exact halves) or a weight of at most 2^15;
 //   numerator O_i = sum_j 2^(x_ij - m_i) codev_j, denominator l_i = sum_j 2^(x_ij - m_i) / vs_j, with the running maximum m_i of x.
 // Rows of zeros have vs = 2^-64 (see weight_scale): with 1 they took the digits of the others' weights, which are all of the output.
 // Positions out of sight have ks = 0, log2 vs = -inf, 1 / vs = 0: no mask per element, and nothing of theirs is multiplied.
@@ -345,9 +345,9 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
         }
         top[r][0] = fmaxf(x[r][0], x[r][2]);
         top[r][1] = fmaxf(x[r][1], x[r][3]);
-        grows |= top[r][0] > st.m[r][0] + 8.0f || top[r][1] > st.m[r][1] + 8.0f;
+        grows |= top[r][0] > st.m[r][0] + MAX_ROOM || top[r][1] > st.m[r][1] + MAX_ROOM;
     }
-    // the maximum follows only where it has grown by more than 2^8: weights stay within halves, sums are exact in either case
+    // weights stay within halves, sums are exact in either case
     if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
         for (int r = 0; r < NR; ++r)
@@ -356,7 +356,7 @@ __device__ __forceinline__ void block_step(uint32_t at, uint32_t valid, uint32_t
                 float y = top[r][e];
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
-                const float m = fmaxf(st.m[r][e], y), al = m == -INFINITY ? 1.0f : exp2_approx(st.m[r][e] - m);
+                const float m = fmaxf(st.m[r][e], y - MAX_BELOW), al = m == -INFINITY ? 1.0f : exp2_approx(st.m[r][e] - m);
                 st.m[r][e] = m;
                 st.l[r][e] *= al;
 #pragma unroll

@@ -10,7 +10,7 @@
 //     run along and an elected one issues, which keeps descriptors in uniform registers: as a branch of lane 0, or with a predicate of lanes,
 //     a product took 75 (scores) and 97 cycles to issue and was the bound (160 sequences behind 32768 positions 323 us, 286 elected).
 //   * Eight warps of softmax read S in fragments of 16x256b: a lane then has 4 rows and a quarter of the columns, so that it reads a quarter
-//     of the column constants; O is rescaled only where a row's maximum has grown by more than 2^8.
+//     of the column constants; O is rescaled only where a row's maximum has grown by 2^8 or more.
 // The tiles of all items form one line that is cut into equal parts, one per CTA; partial results are joined by pool_merge_kernel.
 #include "k2t_flash_tc.cuh"
 #include "k2t_kv_pool.cuh"
@@ -488,13 +488,13 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
                         unpair(x[k][1], lo, hi);
                         tb = max3(tb, lo, hi);
                     }
-                    if (__any_sync(0xffffffffu, ta > m[2 * half] + 8.0f || tb > m[2 * half + 1] + 8.0f)) {
+                    if (__any_sync(0xffffffffu, ta > m[2 * half] + MAX_ROOM || tb > m[2 * half + 1] + MAX_ROOM)) {
 #pragma unroll
                         for (uint32_t o = 1; o < 4; o <<= 1) {
                             ta = fmaxf(ta, __shfl_xor_sync(0xffffffffu, ta, o));
                             tb = fmaxf(tb, __shfl_xor_sync(0xffffffffu, tb, o));
                         }
-                        const float ma = fmaxf(m[2 * half], ta), mb = fmaxf(m[2 * half + 1], tb);
+                        const float ma = fmaxf(m[2 * half], ta - MAX_BELOW), mb = fmaxf(m[2 * half + 1], tb - MAX_BELOW);
                         if (i > 0) {
                             ok = mbar_wait_warp(b_o + 8 * st, (use - 1) & 1u, FL_WAIT, s_abort);
                             if (!ok) break;

@@ -58,7 +58,7 @@ def value_parts(v, bits):
     return np.full_like(v, 127.0) * (scale > 0)[:, None], scale
 
 
-def check_tight(c, got, q, rows, scale=None):
+def check_tight(c, got, q, rows, scale=None, sums=0.0):
     """Outputs of tokens that see all of `rows` (keys, values), without room for anything absolute: the bound of kv_pool_ref.attend, and what weights
     lose as halves: the largest weight times scale of those that share a maximum is kept at 2^7 or more (2^6 for the logarithm's rounding and
     the like), and the smallest step of a half is 2^-24, so each weight times scale is off by at most 2^-25 / 2^6 of the largest.  bf16 calls over
@@ -75,7 +75,7 @@ def check_tight(c, got, q, rows, scale=None):
             p = np.exp(s - s.max())
             p /= p.sum()
             code, of = value_parts(v[:, kv].astype(np.float64), c.bits)
-            lost = 2.0 ** -31 * (p * np.maximum(of, 2.0 ** -64)).max() * np.linalg.norm(np.abs(code).sum(0).reshape(-1, 64), axis=-1)
+            lost = 2.0 ** -31 * (p * np.maximum(of, 2.0 ** -64)).max() * np.linalg.norm(np.abs(code).sum(0).reshape(-1, 64), axis=-1) + sums * np.linalg.norm((p @ np.abs(v[:, kv])).reshape(-1, 64), axis=-1)
             off = np.linalg.norm((got[t, h] - want[0]).reshape(-1, 64), axis=-1)
             allowed = (bound[0] + lost) * (1 + OUT[c.dtype]) + OUT[c.dtype] * np.linalg.norm(want[0].reshape(-1, 64), axis=-1)
             if c.dtype == "f16":
@@ -120,3 +120,19 @@ def test_values_of_zero_with_most_of_the_weight(ctx, d, bits, dtype, where, toke
         check_tight(c, attend(q)[pick], q[pick], rows)
     rows = rewrite(c, rounded(k, dtype), np.zeros_like(rounded(v, dtype)), where == "prefix")          # nothing else
     assert not attend(q).any()
+
+
+@pytest.mark.parametrize("where,kh,tokens,n", [("own", 1, 600, 8000), ("prefix", 1, 3, 8000), ("prefix", 4, 2400, 8200)])
+def test_weights_of_fp32_calls_keep_their_digits(ctx, where, kh, tokens, n):  # noqa: F811
+    """The first 64 values of a few rows, the last 64 of all others, whose scale is far below: as halves on a grid of 2^-24 of the largest their
+    weights would all be off by the same part.  Beside the bound: a sum of equal terms in fp32 is off by a step of 2^-23 an addition, of
+    which an accumulator has fewer than one in 16 rows."""
+    c, attend = place(ctx, where, tokens, n, 128, 8, "f32", kh)
+    one = c.rng.standard_normal((1, kh, 128)).astype(np.float32)
+    v = np.repeat(np.float32(48.5 * 2.0 ** -24) * one, n, 0)
+    v[:, :, :64] = 0
+    v[::2003, :, :64], v[::2003, :, 64:] = one[:, :, :64], 0
+    rows = rewrite(c, np.zeros_like(v), v, where == "prefix")
+    q = c.queries(tokens, kh)
+    pick = c.rng.permutation(tokens)[:3]
+    check_tight(c, attend(q)[pick], q[pick], rows, sums=n / 16 * 2.0 ** -23)
