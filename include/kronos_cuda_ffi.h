@@ -544,7 +544,8 @@ int32_t kronos_cuda_kv_pool_attend_dev(KronosCudaContext *ctx, KronosCudaKvPool 
 /* For every token and kv head the `top` pages of its sequence to attend to, ascending, -1 behind them where the sequence has fewer: the
  * first `sinks` and the last `local` (>= 1, a last page may be partly filled), and of the others those of the highest score, the lower
  * index first among equals.  Score = (integer product of the block key and the query) * the key's scale; the query is the sum of the kv
- * head's queries, quantized as an int8 row.  A page with a key that is not finite comes behind all others. */
+ * head's queries, quantized as an int8 row.  Behind all others come, as equals, pages with a key that is not finite and entries of the table outside
+ * the pool (which attend_chosen skips). */
 int32_t kronos_cuda_kv_pool_select_dev(KronosCudaContext *ctx, KronosCudaKvPool *pool, const KronosCudaPoolAttention *args);
 
 /* attend over the positions below lens[t] of the chosen pages alone (any order; entries below 0 or behind the sequence's last page are

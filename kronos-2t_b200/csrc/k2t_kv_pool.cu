@@ -315,7 +315,7 @@ template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_TH
         }
 #pragma unroll
         for (uint32_t u = 0; u < AHEAD; ++u) {
-            const bool bad = page[u] < 0 || (uint32_t)page[u] >= d.num_pages;          // scores 0
+            const bool bad = page[u] < 0 || (uint32_t)page[u] >= d.num_pages;          // out of sight: behind everything
             if (bad) pool_bad_page(a.pool);
             const size_t at = (size_t)(bad ? 0 : page[u]) * d.kv_heads + h;
             const uint32_t *k = reinterpret_cast<const uint32_t *>(a.pool.block_keys + at * HD) + sub * W;
@@ -327,7 +327,7 @@ template <int HD, uint32_t SEL_THREADS> __global__ void __launch_bounds__(SEL_TH
                 key[u][0] = x.x; key[u][1] = x.y;
             }
             const float s = __ldcg(a.pool.block_key_scales + at);
-            scale[u] = bad ? 0.0f : s;
+            scale[u] = bad ? __uint_as_float(0x7FC00000u) : s;
         }
     };
     ask(from + warp * 4);

@@ -136,3 +136,24 @@ def test_weights_of_fp32_calls_keep_their_digits(ctx, where, kh, tokens, n):  # 
     q = c.queries(tokens, kh)
     pick = c.rng.permutation(tokens)[:3]
     check_tight(c, attend(q)[pick], q[pick], rows, sums=n / 16 * 2.0 ** -23)
+
+
+# ------------------------------------------------------------------------------------------------ pages outside the pool
+@pytest.mark.parametrize("d,bits", SHAPES)
+def test_choice_leaves_pages_outside_the_pool_to_the_last(ctx, d, bits):  # noqa: F811
+    """Their positions are out of sight, so any other page comes before them, also one that scores below zero."""
+    from kronos_2t_b200 import KronosCudaError
+    page, n = 16, 12 * 16
+    c = Cache(ctx, [n], 1, d, bits, page, "f32", block_keys=True)
+    k = np.repeat(c.rng.standard_normal((1, 1, d)), n, 0) * np.repeat(1 + np.arange(12) / 8, page)[:, None, None]
+    k = k.astype(np.float32)
+    rewrite(c, k, k, False)
+    q = -k[:1].reshape(1, 1, d)                     # the first page scores best
+    assert c.select(q, [n], 6, 0, 1)[0, 0].tolist() == [0, 1, 2, 3, 4, 11]
+    for bad in (-1, c.pool.num_pages, 1 << 30):
+        c.table[0, [1, 7]] = bad
+        got = [c.select(q, [n], top, 0, 1)[0, 0].tolist() for top in (6, 10, 11)]
+        with pytest.raises(KronosCudaError, match="outside the pool"):
+            ctx.synchronize()
+        assert got == [[0, 2, 3, 4, 5, 11], [0, 2, 3, 4, 5, 6, 8, 9, 10, 11], [0, 1, 2, 3, 4, 5, 6, 8, 9, 10, 11]]
+    ctx.synchronize()
