@@ -65,8 +65,9 @@ struct PoolAttnArgs {
 };
 cudaError_t launch_pool_attend(cudaStream_t s, const PoolAttnArgs &a, uint32_t *launched);
 cudaError_t launch_pool_select(cudaStream_t s, const PoolAttnArgs &a, uint32_t *launched);
-// of either attention over n_tok tokens
+// of either attention over n_tok tokens, for sizes that are not refused; 0 for those that are
 size_t pool_work_bytes(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint32_t prefix_len, uint32_t sm_count);
+size_t pool_workspace(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint32_t prefix_len, uint32_t sm_count);
 
 // Argument checks that need no device: false and a message.
 enum { POOL_ATTEND = 0, POOL_CHOSEN = 1, POOL_SELECT = 2 };

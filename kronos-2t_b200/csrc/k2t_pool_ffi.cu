@@ -52,16 +52,25 @@ bool pool_rows(const PoolShape &d, uint32_t type, uint32_t heads, size_t n_tok, 
     return true;
 }
 
+// Sizes that no attention call takes: the message, or null.
+static const char *size_refusal(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint32_t prefix_len) {
+    if (heads < d.kv_heads || heads % d.kv_heads != 0 || heads / d.kv_heads > 256) return "heads must be 1..256 times the kv heads";
+    if (n_tok > (1u << 20) || (uint64_t)n_tok * heads > 0x7fffffffu) return "too many tokens";
+    if (prefix_len > 0x7fffffffu) return "prefix too long";
+    if (((uint64_t)n_tok * heads / 64 + d.kv_heads) * (prefix_len / 64 + 1) >= 1ull << 32) return "prefix too long for so many tokens";
+    return nullptr;
+}
+size_t pool_workspace(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint32_t prefix_len, uint32_t sm_count) {
+    return size_refusal(d, heads, n_tok, prefix_len) != nullptr ? 0 : pool_work_bytes(d, heads, n_tok, prefix_len, sm_count);
+}
+
 bool pool_attention(const PoolShape &d, const KronosCudaPoolAttention &c, int what, uint32_t sm_count, PoolAttnArgs &a, std::string &why) {
     auto no = [&](const char *m) { why = std::string("kv_pool: ") + m; return false; };
     const bool selects = what == POOL_SELECT, chosen = what != POOL_ATTEND;
     if (c.struct_size != sizeof(KronosCudaPoolAttention)) return no("struct_size does not match this library");
-    if (c.heads < d.kv_heads || c.heads % d.kv_heads != 0 || c.heads / d.kv_heads > 256) return no("heads must be 1..256 times the kv heads");
-    if (c.n_tok > (1u << 20) || (uint64_t)c.n_tok * c.heads > 0x7fffffffu) return no("too many tokens");
+    if (const char *m = size_refusal(d, c.heads, c.n_tok, c.prefix_len)) return no(m);
     if (!c.lens || !c.pages) return no("NULL table or lengths");
     if (c.pages_stride < 1 || c.pages_stride > (1u << 27)) return no("pages_stride must be 1..2^27");
-    if (c.prefix_len > 0x7fffffffu) return no("prefix too long");
-    if (((uint64_t)c.n_tok * c.heads / 64 + d.kv_heads) * (c.prefix_len / 64 + 1) >= 1ull << 32) return no("prefix too long for so many tokens");
     if (c.prefix_len > 0 && (chosen || !c.prefix_pages)) return no(chosen ? "chosen pages do not go with a prefix" : "prefix without its pages");
     if (!(c.scale >= 0.0f) || c.scale > 1e30f) return no("scale must be a number from 0 on (0: 1 / sqrt(head_dim))");
     if (chosen) {
@@ -224,8 +233,7 @@ int32_t kronos_cuda_kv_pool_load_dev(KronosCudaContext *ctx, KronosCudaKvPool *p
 }
 
 size_t kronos_cuda_kv_pool_workspace(const KronosCudaKvPool *pool, uint32_t heads, uint32_t n_tok, uint32_t prefix_len) {
-    if (!pool || heads < pool->view.d.kv_heads || heads % pool->view.d.kv_heads != 0 || heads / pool->view.d.kv_heads > 256 || n_tok > (1u << 20)) return 0;
-    return pool_work_bytes(pool->view.d, heads, n_tok, prefix_len, pool->sm_count);
+    return pool ? pool_workspace(pool->view.d, heads, n_tok, prefix_len, pool->sm_count) : 0;
 }
 
 int32_t kronos_cuda_kv_pool_attend_dev(KronosCudaContext *ctx, KronosCudaKvPool *pool, const KronosCudaPoolAttention *args) { return attention(ctx, pool, args, POOL_ATTEND); }

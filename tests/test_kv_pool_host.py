@@ -100,6 +100,19 @@ def test_workspaces_cover_what_calls_need(kv_heads, head_dim, bits, heads):
                     assert "workspace too small" in refusal(cfg, arguments(**a, workspace_bytes=need - 1))
 
 
+@pytest.mark.parametrize("heads,n_tok,prefix,refused", [
+    (28, 3, 1000, False), (30, 3, 0, True), (0, 3, 0, True), (4 * 257, 3, 0, True), (28, 1 << 20, 0, False), (28, (1 << 20) + 1, 0, True), (1024, 1 << 20, 0, False),
+    (28, 3, (1 << 31) - 1, False), (28, 3, 1 << 31, True), (28, 3, (1 << 32) - 1, True), (1024, 1 << 20, 16383, True), (28, 1 << 20, 600000, True)])
+def test_workspaces_of_sizes_that_are_refused(heads, n_tok, prefix, refused):
+    """0, as the header says: what attention refuses is not planned."""
+    f = internal("pool_workspace", C.c_size_t, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32)
+    shape = (C.c_uint32 * 6)(4, 128, 8, 6, 10, 1)
+    size = f(shape, heads, n_tok, prefix, 148)
+    assert (size == 0) == refused
+    call = refusal(config(), arguments(heads=heads, n_tok=n_tok, prefix_len=prefix, prefix_pages=4096, workspace_bytes=size))
+    assert (call is not None) == refused
+
+
 def test_null_handles_are_tolerated():
     import kronos_2t_b200 as k2
     L = k2.load_library()
