@@ -469,9 +469,9 @@ int32_t kronos_cuda_k2tb_save(const char *path, const uint64_t mode_words[6], co
  * One pool holds one layer; which page belongs to whom is the host's to say.
  *
  * All buffers named d_* and all pointers inside the argument structs are DEVICE addresses.  Calls are queued on the context's stream and
- * return without synchronizing; they allocate nothing and may be captured into graphs.  A page or slot outside the pool is skipped (its
- * positions count as out of sight) and reported by the next synchronizing call.  Results do not depend on timing: the same call gives
- * the same bits. */
+ * return without synchronizing; they allocate nothing and may be captured into graphs.  A call of no tokens does nothing, and its buffers
+ * may be NULL.  A page or slot outside the pool is skipped (its positions count as out of sight) and reported by the next synchronizing
+ * call.  Results do not depend on timing: the same call gives the same bits. */
 typedef struct KronosCudaKvPool KronosCudaKvPool;
 
 #define KRONOS_CUDA_TYPE_F32  0u

@@ -36,7 +36,7 @@ bool pool_shape(const KronosCudaKvPoolConfig &c, PoolShape &d, std::string &why)
 bool pool_rows(const PoolShape &d, uint32_t type, uint32_t heads, size_t n_tok, const KronosCudaRows &r, const char *name, bool written, RowsArg &out, std::string &why) {
     auto no = [&](const char *m) { why = std::string("kv_pool: ") + name + m; return false; };
     if (type != KRONOS_CUDA_TYPE_F32 && type != KRONOS_CUDA_TYPE_BF16 && type != KRONOS_CUDA_TYPE_F16) return no(": unknown type");
-    if (r.data == nullptr) return no(" is NULL");
+    if (r.data == nullptr && n_tok > 0) return no(" is NULL");          // of no token every address will do: empty buffers have none
     const uint64_t size = type == KRONOS_CUDA_TYPE_F32 ? 4 : 2;
     const uint64_t hs = r.head_stride != 0 ? r.head_stride : d.head_dim, ts = r.token_stride != 0 ? r.token_stride : heads * hs;
     if (hs >> 40 || ts >> 40) return no(": stride too large");
@@ -69,12 +69,13 @@ bool pool_attention(const PoolShape &d, const KronosCudaPoolAttention &c, int wh
     const bool selects = what == POOL_SELECT, chosen = what != POOL_ATTEND;
     if (c.struct_size != sizeof(KronosCudaPoolAttention)) return no("struct_size does not match this library");
     if (const char *m = size_refusal(d, c.heads, c.n_tok, c.prefix_len)) return no(m);
-    if (!c.lens || !c.pages) return no("NULL table or lengths");
+    const bool some = c.n_tok > 0;
+    if (some && (!c.lens || !c.pages)) return no("NULL table or lengths");
     if (c.pages_stride < 1 || c.pages_stride > (1u << 27)) return no("pages_stride must be 1..2^27");
-    if (c.prefix_len > 0 && (chosen || !c.prefix_pages)) return no(chosen ? "chosen pages do not go with a prefix" : "prefix without its pages");
+    if (c.prefix_len > 0 && (chosen || (some && !c.prefix_pages))) return no(chosen ? "chosen pages do not go with a prefix" : "prefix without its pages");
     if (!(c.scale >= 0.0f) || c.scale > 1e30f) return no("scale must be a number from 0 on (0: 1 / sqrt(head_dim))");
     if (chosen) {
-        if (!c.chosen) return no("chosen is NULL");
+        if (some && !c.chosen) return no("chosen is NULL");
         if (c.top < 1 || c.top > KRONOS_CUDA_POOL_MAX_CHOSEN) return no("top must be 1..32768");
     } else if (c.chosen || c.top) {
         return no("attend takes no chosen pages (kronos_cuda_kv_pool_attend_chosen_dev)");

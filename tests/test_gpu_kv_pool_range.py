@@ -157,3 +157,15 @@ def test_choice_leaves_pages_outside_the_pool_to_the_last(ctx, d, bits):  # noqa
             ctx.synchronize()
         assert got == [[0, 2, 3, 4, 5, 11], [0, 2, 3, 4, 5, 6, 8, 9, 10, 11], [0, 1, 2, 3, 4, 5, 6, 8, 9, 10, 11]]
     ctx.synchronize()
+
+
+def test_calls_without_a_token(ctx):  # noqa: F811
+    c = Cache(ctx, [20], 2, 64, 8, 16, "bf16", block_keys=True)
+    launches = ctx.launch_count
+    c.pool.store_dev("bf16", 0, 0, 0, 0)
+    c.pool.load_dev("f32", 0, 0, 0, 0)
+    c.pool.attend_dev("bf16", 4, 0, 0, 0, 0, 3, 0, (0, 0), d_prefix_pages=0, prefix_len=50)
+    c.pool.select_dev("bf16", 4, 0, 0, 0, 0, 3, 5, 0)
+    c.pool.attend_chosen_dev("bf16", 4, 0, 0, 0, 0, 3, 5, 0, 0, (0, 0))
+    ctx.synchronize()
+    assert ctx.launch_count == launches

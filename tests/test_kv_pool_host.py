@@ -83,6 +83,17 @@ def test_calls_without_a_token_need_nothing():
     assert "prefix too long" in refusal(config(), arguments(n_tok=1 << 20, prefix_len=(1 << 31) - 1, prefix_pages=4096))
 
 
+def test_calls_without_a_token_take_empty_buffers():
+    """An empty tensor has no address."""
+    none = dict(n_tok=0, q=rows(None), out=rows(None), lens=None, pages=None, workspace=None, workspace_bytes=0)
+    assert refusal(config(), arguments(**none)) is None
+    assert refusal(config(), arguments(**none, prefix_len=1000)) is None
+    for what in (1, 2):
+        assert refusal(config(), arguments(**none, top=3, sinks=1, local=1), what) is None
+    assert "type" in refusal(config(), arguments(**none, row_type=3))
+    assert "heads" in refusal(config(), arguments(**{**none, "heads": 30}))
+
+
 @pytest.mark.parametrize("kv_heads,head_dim,bits,heads", [(4, 128, 8, 28), (1, 64, 4, 20), (8, 128, 4, 64), (3, 64, 8, 3)])
 def test_workspaces_cover_what_calls_need(kv_heads, head_dim, bits, heads):
     """A call is refused one byte below the size that is asked for some type, never at it; with a prefix it is enough without one."""
