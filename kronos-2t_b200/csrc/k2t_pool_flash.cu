@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) pool_flash_kernel(const __grid_
             const uint32_t head = g.item / f.row_tiles;
             auto page_of = [&](uint32_t tile) {
                 const uint32_t pos = tile * FL_KT + lane * POOL_ROWS;
-                return lane < F::BLOCKS && tile < g.last && pos < p.a.prefix_len ? __ldg(p.a.prefix_pages + (pos >> d.page_shift)) : 0;
+                return lane < F::BLOCKS && tile < g.last && pos < p.a.prefix_len ? __ldcg(p.a.prefix_pages + (pos >> d.page_shift)) : 0;
             };
             int32_t page = page_of(g.first);
             for (uint32_t t = g.first; t < g.last; ++t, ++n) {
