@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t lds1(uint32_t at) { uint32_t v; asm volatile
 struct Segment { uint32_t item, first, last; };          // tiles [first, last) of an item
 // Segment s of a CTA's part of the line; false behind the last.
 __device__ __forceinline__ bool segment_of(const FlashArgs &f, uint32_t s, Segment &g) {
-    const uint32_t x0 = blockIdx.x * f.part, x1 = min(f.items * f.tiles, x0 + f.part);
+    const uint32_t x0 = blockIdx.x * f.part, x1 = x0 + min(f.items * f.tiles - x0, f.part);          // a line may be nearly 2^32 tiles long
     const uint32_t item = x0 / f.tiles + s, b = item * f.tiles;
     if (b >= x1) return false;
     g.item = item;
@@ -617,7 +617,7 @@ template <int HD, int BITS, int QT, int PT> cudaError_t flash_go(cudaStream_t s,
     const uint32_t line = p.flash.items * p.flash.tiles, rows = p.flash.items * (p.flash.halved ? 1 : 2) * FLASH_ROWS;
     const cudaError_t q = launch_kernel(pool_query_kernel<HD, QT>, dim3(rows * (HD / 8) / QK_THREADS), dim3(QK_THREADS), 0, s, true, p);
     if (q != cudaSuccess) return q;
-    return launch_kernel(pool_flash_kernel<HD, BITS, QT, PT>, dim3((line + p.flash.part - 1) / p.flash.part), dim3(FL_THREADS), smem, s, true, p);
+    return launch_kernel(pool_flash_kernel<HD, BITS, QT, PT>, dim3((line - 1) / p.flash.part + 1), dim3(FL_THREADS), smem, s, true, p);
 }
 template <int HD, int BITS> cudaError_t flash_type(cudaStream_t s, const SplitArgs &p) {
     const uint32_t type = p.a.q.type;
