@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import kv_pool_ref as ref
-from test_gpu_kv_pool import HALF, OUT, SHAPES, Cache, ctx, rounded  # noqa: F401
+from test_gpu_kv_pool import HALF, OUT, SHAPES, Cache, ctx, device, rounded, torch_type  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -169,3 +169,135 @@ def test_calls_without_a_token(ctx):  # noqa: F811
     c.pool.attend_chosen_dev("bf16", 4, 0, 0, 0, 0, 3, 5, 0, 0, (0, 0))
     ctx.synchronize()
     assert ctx.launch_count == launches
+
+
+# ------------------------------------------------------------------------------------------------ the prefix of many rows
+MANY = [(64, 8200), (200, 3000)]                    # rows of one tile and of two, both for the kernel of many rows
+
+
+@pytest.mark.parametrize("d,bits", SHAPES)
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("tokens,n", MANY)
+def test_a_row_of_a_prefix_that_is_not_finite(ctx, d, bits, dtype, tokens, n):  # noqa: F811
+    """A key reaches every query of its kv head, a value likewise; a query that is not finite reaches its own row alone."""
+    c = Cache(ctx, [3] * 2, 2, d, bits, 64, dtype, prefix=n)
+    q = c.queries(tokens, 2)
+    lens, seq = [3] * tokens, np.arange(tokens) % 2
+    hurt = q.copy()
+    hurt[5, 1, 3] = np.inf
+    hurt[7, 0, d - 1] = np.nan
+    got = c.attend(hurt, lens, seq)
+    assert np.isnan(got[5, 1]).all() and np.isnan(got[7, 0]).all()
+    keep = np.ones((tokens, 2), bool)
+    keep[5, 1] = keep[7, 0] = False
+    assert np.isfinite(got[keep]).all()
+    c.check(got[:4], q[:4], lens[:4], seq[:4])
+    good, bad = np.ones((1, 2, d), np.float32), np.ones((1, 2, d), np.float32)
+    bad[0, 1, 9] = np.nan
+    for at, (k, v) in ((n - 1, (bad, good)), (70, (good, bad))):
+        slot = np.array([int(c.prefix_pages[at // 64]) * 64 + at % 64])
+        c.store(slot, k, v)
+        got = c.attend(q, lens, seq)
+        assert np.isnan(got[:, 1]).all() and np.isfinite(got[:, 0]).all()
+        c.store(slot, good, good)
+        assert np.isfinite(c.attend(q, lens, seq)).all()
+
+
+@pytest.mark.parametrize("d,bits", SHAPES)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("where,tokens,n", [("own", 3, 700), ("prefix", 64, 8200), ("prefix", 200, 3000)])
+def test_scales_far_apart_and_queries_of_all_sizes(ctx, d, bits, dtype, where, tokens, n):  # noqa: F811
+    c, attend = place(ctx, where, tokens, n, d, bits, dtype)
+    rng = c.rng
+    k, v = (rng.standard_normal((n, 1, d)) for _ in range(2))
+    v *= 10.0 ** rng.integers(-6, 7, (n, 1, 1))
+    v[::7], k[::11] = 0, 0
+    rows = rewrite(c, rounded(k, dtype), rounded(v, dtype), where == "prefix")
+    q = rng.standard_normal((tokens, 2, d)) * 1.5
+    pick = rng.permutation(tokens)[:2]
+    for size in (0.0, 1e-30, 1e-3, 1.0, 3.0):
+        x = rounded(q * size, dtype)
+        check_tight(c, attend(x)[pick], x[pick], rows)
+    x = rounded(q, dtype)
+    check_tight(c, attend(x, scale=0.31)[pick], x[pick], rows, scale=0.31)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("tokens,n", [(3, 200)] + MANY)
+def test_strided_rows_behind_a_prefix(ctx, dtype, tokens, n):  # noqa: F811
+    """Heads outermost, at addresses that allow no wide access; what lies between the rows stays as it was."""
+    import torch
+    d, heads = 64, 4
+    c = Cache(ctx, [5] * tokens, 2, d, 8, 16, dtype, prefix=n)
+    q, lens = c.queries(tokens, heads), [5] * tokens
+    straight = c.attend(q, lens)
+    wide = torch.full((heads, tokens, d + 3), 2.0, device="cuda", dtype=torch_type(dtype))
+    wide[:, :, 1:d + 1] = device(q, dtype).transpose(0, 1)
+    out, dl, dt, far = torch.full_like(wide, 9.0), device(np.array(lens, np.int32)), device(c.table), device(c.prefix_pages)
+    work, size = torch.empty(c.pool.workspace_bytes(heads, tokens, n), dtype=torch.uint8, device="cuda"), wide.element_size()
+    c.pool.attend_dev(dtype, heads, tokens, (wide.data_ptr() + size, d + 3, tokens * (d + 3)), dl.data_ptr(), dt.data_ptr(), dt.shape[1],
+                      (out.data_ptr() + size, d + 3, tokens * (d + 3)), (work.data_ptr(), work.numel()), d_prefix_pages=far.data_ptr(), prefix_len=n)
+    ctx.synchronize()
+    got = out.float().cpu().numpy()
+    assert np.array_equal(got[:, :, 1:d + 1].transpose(1, 0, 2), straight)
+    assert (got[:, :, 0] == 9).all() and (got[:, :, d + 1:] == 9).all()
+
+
+# ------------------------------------------------------------------------------------------------ other calls
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("bits", [8, 4])
+def test_strided_rows_of_other_types(ctx, dtype, bits):  # noqa: F811
+    """Rows in and out, and queries of a choice, at odd places of a wider buffer."""
+    import torch
+    d, kh, heads, n, page = 128, 2, 6, 75, 16
+    c = Cache(ctx, [n], kh, d, bits, page, dtype, block_keys=True)
+    k, v = (rounded(c.rng.standard_normal((n, kh, d)), dtype) for _ in range(2))
+    wide = [torch.full((n, kh, d + 5), 2.0, device="cuda", dtype=torch_type(dtype)) for _ in range(4)]
+    wide[0][:, :, 3:d + 3], wide[1][:, :, 3:d + 3] = device(k, dtype), device(v, dtype)
+    rows = [(w.data_ptr() + 3 * w.element_size(), kh * (d + 5), d + 5) for w in wide]
+    at = np.arange(n)
+    slots = device(c.table[0][at // page].astype(np.int64) * page + at % page)
+    c.pool.store_dev(dtype, rows[0], rows[1], slots.data_ptr(), n)
+    c.pool.load_dev(dtype, slots.data_ptr(), n, rows[2], rows[3])
+    ctx.synchronize()
+    for x, w in ((k, wide[2]), (v, wide[3])):
+        got = w.float().cpu().numpy()
+        assert np.array_equal(got[:, :, 3:d + 3], rounded(ref.read_back(x, bits).reshape(n, kh, d), dtype))
+        assert (got[:, :, :3] == 2).all() and (got[:, :, d + 3:] == 2).all()
+    q, lens = c.queries(4, heads), [n, 40, 3, n - 1]
+    want = c.select(q, lens, 3, 0, 1, seq=[0] * 4)
+    x = torch.full((heads, 4, d + 7), 2.0, device="cuda", dtype=torch_type(dtype))
+    x[:, :, 1:d + 1] = device(q, dtype).transpose(0, 1)
+    dl, dt, ds, out = device(np.array(lens, np.int32)), device(c.table), device(np.zeros(4, np.int32)), torch.full((4, kh, 3), 77, dtype=torch.int32, device="cuda")
+    c.pool.select_dev(dtype, heads, 4, (x.data_ptr() + x.element_size(), d + 7, 4 * (d + 7)), dl.data_ptr(), dt.data_ptr(), dt.shape[1], 3, out.data_ptr(), sinks=0, local=1, d_seq=ds.data_ptr())
+    ctx.synchronize()
+    assert np.array_equal(out.cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype,d,bits", [("bf16", 128, 8), ("f32", 64, 4)])
+def test_a_page_named_twice_counts_twice(ctx, dtype, d, bits):  # noqa: F811
+    page, n = 16, 70
+    c = Cache(ctx, [n], 2, d, bits, page, dtype)
+    q = c.queries(1, 4)
+    chosen = np.array([[[1, 3, 1, -1, 4], [4, 4, 0, 0, 0]]], np.int32)
+    rows = [np.concatenate([np.arange(p * page, min(n, (p + 1) * page)) for p in x if p >= 0]) for x in chosen[0]]
+    c.check(c.attend(q, [n], chosen=chosen), q, [n], rows_of=lambda t, h: rows[h])
+
+
+@pytest.mark.parametrize("kh,heads,d,bits,prefix", [(256, 256, 64, 8, 0), (256, 256, 64, 4, 40), (1, 256, 64, 4, 0), (1, 256, 64, 4, 3000), (2, 512, 128, 8, 40), (2, 512, 128, 8, 3000)])
+def test_most_heads(ctx, kh, heads, d, bits, prefix):  # noqa: F811
+    """256 kv heads, and 256 query heads of one."""
+    c = Cache(ctx, [20, 0, 37], kh, d, bits, 16, "bf16", prefix=prefix, block_keys=True)
+    q = c.queries(3, heads)
+    lens = [20, 0, 37]
+    got = c.attend(q, lens)
+    some = [0, 1, kh // 2, kh - 1]
+    for h in set(some):
+        mine = slice(h * heads // kh, (h + 1) * heads // kh)
+        for t in range(3):
+            k, v = (np.concatenate((c.far[i][:, h:h + 1], c.own[t][i][:, h:h + 1])) for i in range(2))
+            want, bound = ref.attend(q[t, mine], k, v, d ** -0.5, HALF["bf16"])
+            off = np.linalg.norm((got[t, mine] - want).reshape(-1, d // 64, 64), axis=-1)
+            assert (off <= bound * (1 + OUT["bf16"]) + OUT["bf16"] * np.linalg.norm(want.reshape(-1, d // 64, 64), axis=-1) + 1e-7).all()
+    pages = c.select(q, lens, 2, 0, 1)
+    assert (pages[0] == [0, 1]).all() and (pages[1] == -1).all() and (pages[2, :, 1] == 2).all()

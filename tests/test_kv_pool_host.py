@@ -147,3 +147,23 @@ def test_restatement_against_the_oracle(oracle):
     assert np.abs(ref.stored(x, 8) - want).max() <= np.abs(want).max() / 127 * 0.5001
     # 4 bits: centroids are at most 16 half steps of 1/127 apart from their borders, plus the fitted scale
     assert np.abs(ref.stored(x, 4) - want).max() <= np.abs(want).max() * 0.25
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_codes_and_scales_are_the_oracles(oracle, d):
+    """Bit for bit, of both widths of codes: ordinary rows of many sizes, rows of zeros and below what is kept, values that are codes."""
+    rng = np.random.default_rng(d)
+    x = (rng.standard_normal((400, d)) * 10.0 ** rng.uniform(-8, 8, (400, 1))).astype(np.float32)
+    x[::50] = 0
+    x[1::50] = np.float32(1e-9)
+    x[2::50] = ref.rotate_back(np.tile(ref.CENTROIDS * np.float32(0.5), d // 16)[None]).astype(np.float32)
+    x[3::50] = rng.integers(-3, 4, d)
+    code8, scale8 = ref.quant8(ref.rotate(x))
+    code4, scale4 = ref.quant4(ref.rotate(x))
+    for i, row in enumerate(x):
+        q, s = oracle.kv_quant_head(row)
+        assert np.array_equal(q, code8[i]) and s == scale8[i], i
+        q, s = oracle.kv_quant_head_q4(row)
+        nibbles = np.stack((q.reshape(-1, 16) & 15, q.reshape(-1, 16) >> 4), 1).reshape(-1)          # 16 low ones, then 16 high ones
+        assert np.array_equal(ref.CENTROIDS[nibbles], code4[i]), i
+        assert np.array_equal((s.astype(np.uint32) << 16).view(np.float32), scale4[i]), i
