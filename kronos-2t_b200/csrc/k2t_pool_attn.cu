@@ -723,14 +723,20 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
 
 // ------------------------------------------------------------------------------------------------ launches
 // A line of blocks in equal parts, or items in equal pieces, one a CTA?  A piece begins no second item, and nothing has to be looked up for it, but
-// pieces are as equal as the items are long.  The prefix and chosen pages: items of one length, pieces.  Tables: pieces of as many blocks
-// as the widest row of the table gives CTAs that the SMs hold at once (an item that is shorter has fewer: the others leave at once), or of
-// whole items of up to LONGEST blocks where there are a few for every such CTA, or of any length where there are many; else a line.
-constexpr uint32_t LONGEST = 64;
+// pieces are as equal as the items are long.  The prefix and chosen pages: items of one length, pieces.  Tables, by the widest row that the table
+// has room for, in us of the whole call over ragged lengths (8 bits x 128 bf16; 4 x 64 fp16 and 4 x 128 fp32 draw the same lines):
+//   * up to WHOLE blocks, or from 16 items a resident CTA on, an item is one piece: 16 blocks x 48 / 192 items 6.4 / 7.9, cut in two 10.0 / 14.0 (a
+//     merge follows), as a line 18.5 / 26.5; 32 blocks x 96 / 192 items 9.3 / 10.5, in pieces 13.9 / 15.8;
+//   * pieces of as many blocks as give CTAs that the SMs hold at once (a shorter item has fewer: the others leave at once), of LONGEST at most:
+//     256 blocks x 48 items 21 in eight pieces, 47 whole, 26 as a line; 192 items 48 in two, 36 as a line;
+//   * more items than that: whole up to 2 LONGEST blocks (2400 items of 4 / 64 / 128 blocks 23 / 70 / 117, as a line 65 / 110 / 161), a line from there
+//     (1200 items of 512 blocks 221, whole 250; at 256 the two are alike).
+constexpr uint32_t WHOLE = 32, LONGEST = 64;
 uint32_t own_pieces(uint64_t items, uint64_t widest, uint64_t room) {
+    if (widest <= WHOLE || items >= 16 * room) return 1;
     for (uint64_t part = MIN_PART; part <= LONGEST; part *= 2)
         if (items * ((widest + part - 1) / part) <= room) return (uint32_t)((widest + part - 1) / part);
-    return (widest <= LONGEST && items <= 4 * room) || items >= 16 * room ? 1 : 0;
+    return widest <= 2 * LONGEST ? 1 : 0;
 }
 SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     SplitArgs p{};
