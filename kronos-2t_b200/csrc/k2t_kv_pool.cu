@@ -70,7 +70,8 @@ __device__ __forceinline__ uint8_t *block_of(const PoolView &p, int64_t slot, ui
 // ------------------------------------------------------------------------------------------------ rows in, rows out
 // head_dim / 8 lanes hold a row, eight values each; rows are numbered (token, keys | values, head).  A thread has its part of ROW_AHEAD rows on
 // the way at a time: two (16384 tokens x 8 heads of 128 written and read: one 98, two 95.6, four 96.9 us; 4001 x 32 of 64, 4 bits: 65, 63, 67), or one
-// where the rows are too few to fill the SMs even so (a decode batch of 96 tokens: two kernels 4.4 us, 9.8 with four, which only follow one another).
+// where the rows are too few for the second to hide behind the first.  In us, one | two, by CTAs of one: written, 8 bits, 300 CTAs 2.4 | 2.9, 1200 4.8 | 5.2,
+// 2400 8.0 | 8.2, 5000 14.7 | 14.4; 4 bits 300 3.9 | 4.8, 1200 8.8 | 9.6, 5000 29.5 | 28.7; read, 300 2.1 | 2.5, 600 3.3 | 3.0, 2400 6.8 | 6.6.
 constexpr uint32_t ROW_THREADS = 256;
 struct RowAt { uint32_t t, value, head; };
 __device__ __forceinline__ RowAt row_at(const PoolStoreArgs &a, uint32_t r) {          // r below 2^31: a division by a multiplication (and a shift) that is exact there
@@ -450,7 +451,8 @@ uint32_t row_ctas(const PoolStoreArgs &a, uint32_t ahead) {
     const uint32_t per = ROW_THREADS * 8 / a.pool.d.head_dim * ahead;
     return (uint32_t)(((uint64_t)a.n_tok * 2 * a.pool.d.kv_heads + per - 1) / per);
 }
-bool few_rows(const PoolStoreArgs &a) { return row_ctas(a, 1) <= 4 * a.sm_count; }
+constexpr uint32_t FEW_WRITTEN = 16, FEW_READ = 3;          // CTAs an SM
+bool few_rows(const PoolStoreArgs &a, uint32_t few) { return row_ctas(a, 1) <= few * a.sm_count; }
 // r / (2 kv heads) for r below 2^31
 PoolStoreArgs divided(PoolStoreArgs a) {
     const uint32_t per = 2 * a.pool.d.kv_heads;
@@ -462,7 +464,7 @@ PoolStoreArgs divided(PoolStoreArgs a) {
 }
 template <int HD, int BITS> cudaError_t store_rows(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched) {
     *launched += 1;
-    const cudaError_t e = few_rows(a) ? launch_kernel(pool_store_kernel<HD, BITS, 1>, dim3(row_ctas(a, 1)), dim3(ROW_THREADS), 0, s, true, a)
+    const cudaError_t e = few_rows(a, FEW_WRITTEN) ? launch_kernel(pool_store_kernel<HD, BITS, 1>, dim3(row_ctas(a, 1)), dim3(ROW_THREADS), 0, s, true, a)
                                       : launch_kernel(pool_store_kernel<HD, BITS, 2>, dim3(row_ctas(a, 2)), dim3(ROW_THREADS), 0, s, true, a);
     if (e != cudaSuccess || !a.pool.d.block_keys) return e;
     const uint64_t warps = ((uint64_t)a.n_tok + 31) / 32 * a.pool.d.kv_heads;
@@ -471,7 +473,7 @@ template <int HD, int BITS> cudaError_t store_rows(cudaStream_t s, const PoolSto
 }
 template <int HD, int BITS> cudaError_t load_rows(cudaStream_t s, const PoolStoreArgs &a, uint32_t *launched) {
     *launched += 1;
-    return few_rows(a) ? launch_kernel(pool_load_kernel<HD, BITS, 1>, dim3(row_ctas(a, 1)), dim3(ROW_THREADS), 0, s, true, a)
+    return few_rows(a, FEW_READ) ? launch_kernel(pool_load_kernel<HD, BITS, 1>, dim3(row_ctas(a, 1)), dim3(ROW_THREADS), 0, s, true, a)
                        : launch_kernel(pool_load_kernel<HD, BITS, 2>, dim3(row_ctas(a, 2)), dim3(ROW_THREADS), 0, s, true, a);
 }
 

@@ -301,3 +301,26 @@ def test_most_heads(ctx, kh, heads, d, bits, prefix):  # noqa: F811
             assert (off <= bound * (1 + OUT["bf16"]) + OUT["bf16"] * np.linalg.norm(want.reshape(-1, d // 64, 64), axis=-1) + 1e-7).all()
     pages = c.select(q, lens, 2, 0, 1)
     assert (pages[0] == [0, 1]).all() and (pages[1] == -1).all() and (pages[2, :, 1] == 2).all()
+
+
+@pytest.mark.parametrize("d,bits", SHAPES)
+@pytest.mark.parametrize("n,kh", [(9001, 4), (1301, 5), (20003, 2)])
+def test_many_rows(ctx, d, bits, n, kh):  # noqa: F811
+    """As many as one and two rows on their way a thread are for, the last CTA's part full; every fifth token is left out."""
+    import torch
+
+    from kronos_2t_b200 import KvPool
+    rng = np.random.default_rng(n)
+    pages = -(-n // 64) + 2
+    slots = rng.permutation(pages * 64)[:n].astype(np.int64)
+    slots[::5] = -1
+    x = [rounded(rng.standard_normal((n, kh, d)), "bf16") for _ in range(2)]
+    pool, dx, ds = KvPool(ctx, kh, d, bits, 64, pages), [device(a, "bf16") for a in x], device(slots)
+    pool.store_dev("bf16", dx[0].data_ptr(), dx[1].data_ptr(), ds.data_ptr(), n)
+    out = [torch.full((n, kh, d), 5.0, device="cuda") for _ in x]
+    pool.load_dev("f32", ds.data_ptr(), n, out[0].data_ptr(), out[1].data_ptr())
+    ctx.synchronize()
+    for a, o in zip(x, out):
+        want = ref.read_back(a, bits).reshape(n, kh, d)
+        want[::5] = 5.0
+        assert np.array_equal(o.cpu().numpy(), want)
