@@ -272,7 +272,8 @@ template <int HD, int BITS> __global__ void __launch_bounds__(ROW_THREADS) pool_
 // with its block key times the key's scale (one rounding, so that scores are the same wherever they are computed).  The order of
 // scores is that of their bits as numbers; the pages are those at or above a threshold (found byte by byte), of its equals the first.
 // Two sizes of CTA: with few (token, kv head) pairs the time is one CTA's chain of loads, and 512 threads have a whole sequence's keys in
-// flight; with many, smaller CTAs have fewer threads idle at their barriers.
+// flight; with many, smaller CTAs have fewer threads idle at their barriers.  In us, 512 | 128 threads, for tables of 250 / 625 / 2000 pages: 192 pairs
+// 8.1 | 10.4, 12.4 | 17.8, 22.5 | 46.7; 400 pairs 12.6 | 11.1, 21 | 18.7, 36.7 | 48.6; 800 pairs 18.9 | 13.7, 32 | 23, 59.6 | 61.3; 2000 pairs 40 | 23, 70 | 41, 133 | 111.
 __device__ __forceinline__ uint32_t ordered(float x) {           // NaN behind everything
     if (x != x) return 0;
     const uint32_t b = __float_as_uint(x == 0.0f ? 0.0f : x);
@@ -492,7 +493,8 @@ cudaError_t launch_pool_load(cudaStream_t s, const PoolStoreArgs &args, uint32_t
 cudaError_t launch_pool_select(cudaStream_t s, const PoolAttnArgs &a, uint32_t *launched) {
     const size_t smem = (size_t)a.pages_stride * 4;
     const uint32_t pairs = a.n_tok * a.pool.d.kv_heads;
-    const bool small = pairs >= 4 * a.sm_count && a.pages_stride <= 4096;
+    // by the table's width, which is all that is known here of how long the sequences are; the widest leave room for few small CTAs
+    const bool small = a.pages_stride <= 4096 && 2 * pairs >= (a.pages_stride <= 1024 ? 5 : 16) * a.sm_count;
     const auto kernel = a.pool.d.head_dim == 128 ? (small ? pool_select_kernel<128, 128> : pool_select_kernel<128, 512>) : small ? pool_select_kernel<64, 128> : pool_select_kernel<64, 512>;
     const cudaError_t e = allow_dynamic_smem(reinterpret_cast<const void *>(kernel), smem);
     if (e != cudaSuccess) return e;

@@ -745,8 +745,10 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
     const uint32_t group = a.heads / d.kv_heads;
     const uint32_t rows = a.n_tok * group;
     // More rows than a tile of this kernel: k2t_pool_flash.cu, which expands a cached row once for 128 or 256 query rows where this one does for
-    // 16.  Its start costs more, so it takes FLASH_WORK tiles of 16 rows x 16 positions and up (24 sequences x 28 heads over 4 kv heads behind
-    // 500 / 1000 / 4000 / 16000 positions, the whole call: 19 / 24 / 31 / 53 us here, 24 / 25 / 28 / 39 there).
+    // 16.  Its start costs more, so it takes FLASH_WORK tiles of 16 rows x 16 positions and up.  Time here over time there for 24 to 384 rows of 1 to 8 kv
+    // heads, widths 64 and 128, 8 and 4 bits, all types (the whole call; median, and the range that the shapes leave): below 1024 tiles 0.75
+    // (0.63 .. 1.10), to 2048 0.84 (0.74 .. 0.97), to 8192 1.0 (0.87 .. 1.29), to 16384 1.0 (0.88 .. 1.35), above 1.39 (1.13 .. 2.67); the low ends are 24 or 32
+    // rows, which fill a fifth of a tile, and fp32, the high ends 320 rows.
     constexpr uint64_t FLASH_WORK = 2048;
     p.flash.on = a.prefix_len > 0 && rows > 16 && (uint64_t)((rows + 15) / 16) * d.kv_heads * prefix_blocks(p) >= FLASH_WORK;
     if (p.flash.on) {
