@@ -725,15 +725,16 @@ template <int HD> __global__ void __launch_bounds__(MERGE_WARPS * 32) pool_merge
 // A line of blocks in equal parts, or items in equal pieces, one a CTA?  A piece begins no second item, and nothing has to be looked up for it, but
 // pieces are as equal as the items are long.  The prefix and chosen pages: items of one length, pieces.  Tables, by the widest row that the table
 // has room for, in us of the whole call over ragged lengths (8 bits x 128 bf16; 4 x 64 fp16 and 4 x 128 fp32 draw the same lines):
-//   * up to WHOLE blocks, or from 16 items a resident CTA on, an item is one piece: 16 blocks x 48 / 192 items 6.4 / 7.9, cut in two 10.0 / 14.0 (a
-//     merge follows), as a line 18.5 / 26.5; 32 blocks x 96 / 192 items 9.3 / 10.5, in pieces 13.9 / 15.8;
+//   * up to WHOLE blocks, unless a prefix has to be joined anyway, and from 16 items a resident CTA on, an item is one piece: 16 blocks x 48 / 192
+//     items 6.4 / 7.9, cut in two 10.0 / 14.0 (a merge follows), as a line 18.5 / 26.5; 32 blocks x 96 / 192 items 9.3 / 10.5, in pieces 13.9 / 15.8 (32
+//     blocks x 32 items behind a prefix, 4 bits: whole 93, in pieces 83);
 //   * pieces of as many blocks as give CTAs that the SMs hold at once (a shorter item has fewer: the others leave at once), of LONGEST at most:
 //     256 blocks x 48 items 21 in eight pieces, 47 whole, 26 as a line; 192 items 48 in two, 36 as a line;
 //   * more items than that: whole up to 2 LONGEST blocks (2400 items of 4 / 64 / 128 blocks 23 / 70 / 117, as a line 65 / 110 / 161), a line from there
 //     (1200 items of 512 blocks 221, whole 250; at 256 the two are alike).
 constexpr uint32_t WHOLE = 32, LONGEST = 64;
-uint32_t own_pieces(uint64_t items, uint64_t widest, uint64_t room) {
-    if (widest <= WHOLE || items >= 16 * room) return 1;
+uint32_t own_pieces(uint64_t items, uint64_t widest, uint64_t room, bool joined) {
+    if ((widest <= WHOLE && !joined) || items >= 16 * room) return 1;
     for (uint64_t part = MIN_PART; part <= LONGEST; part *= 2)
         if (items * ((widest + part - 1) / part) <= room) return (uint32_t)((widest + part - 1) / part);
     return widest <= 2 * LONGEST ? 1 : 0;
@@ -769,7 +770,7 @@ SplitArgs split_plan(const PoolAttnArgs &a, uint32_t type) {
         p.near_pieces = pieces_of((uint64_t)d.kv_heads * p.rbp, prefix_blocks(p));
         p.near_units = d.kv_heads * p.rbp * p.near_pieces;
     }
-    p.pieces = a.chosen != nullptr ? pieces_of(items, (uint64_t)a.top << (d.page_shift - 4)) : own_pieces(items, std::max<uint64_t>(1, (uint64_t)a.pages_stride << (d.page_shift - 4)), room);
+    p.pieces = a.chosen != nullptr ? pieces_of(items, (uint64_t)a.top << (d.page_shift - 4)) : own_pieces(items, std::max<uint64_t>(1, (uint64_t)a.pages_stride << (d.page_shift - 4)), room, a.prefix_len > 0);
     p.units = (uint32_t)(p.pieces != 0 ? items * p.pieces : room);
     return p;
 }
