@@ -505,7 +505,7 @@ void kronos_cuda_kv_pool_free(KronosCudaContext *ctx, KronosCudaKvPool *pool);
 size_t kronos_cuda_kv_pool_bytes(const KronosCudaKvPool *pool);
 
 /* Writes the keys and values of n_tok tokens (kv_heads rows each, of `type`) into slots d_slots[t] = page * page_tokens + row; a token with
- * a slot below 0 is left out.  Slots of one call must differ.  A row that holds a value that is not finite reads back as NaN.
+ * a slot below 0 is left out.  Slots of one call must differ.  A row that is not finite, or whose transform is not, reads back as NaN.
  * With block keys: writing the LAST row of a page makes the page's block key from the rows the page then holds (rows of a page are
  * written in order, so that these are the page's own): the mean of its keys as stored, fp32 in row order, quantized as an int8 row.
  * load reads rows back (code times scale, inverse transform, rounded once to `type`); left-out tokens' rows stay as they are. */
@@ -538,7 +538,11 @@ typedef struct KronosCudaPoolAttention {
 size_t kronos_cuda_kv_pool_workspace(const KronosCudaKvPool *pool, uint32_t heads, uint32_t n_tok, uint32_t prefix_len);
 
 /* out = softmax(scale q k^T) v over the prefix and the first lens[t] positions of the token's sequence.  A token that sees nothing gets
- * zeros.  Queries, weights and sums are fp32; fp32 operands of the products are split in two halves, bf16 / fp16 ones rounded to one. */
+ * zeros.  Sums and maxima are fp32.  Operands of the products are halves (11 bits): the codes exactly; queries, which are not quantized
+ * (the engines' attention quantizes them, so its numbers for the same cache differ), and weights each as the sum of two halves in fp32 calls, queries
+ * as two and weights as one in fp16 calls, one each in bf16 calls.  bf16 calls over 4-bit rows of 128 also round codes times the ratio of
+ * the row's two scales to one half for a prefix that many rows share (2048 products of 16 rows x 16 positions or more).  Values whose scales are more
+ * than 2^126 apart, or 2^62 above 1 beside rows of zeros, are outside what weights can tell apart. */
 int32_t kronos_cuda_kv_pool_attend_dev(KronosCudaContext *ctx, KronosCudaKvPool *pool, const KronosCudaPoolAttention *args);
 
 /* For every token and kv head the `top` pages of its sequence to attend to, ascending, -1 behind them where the sequence has fewer: the

@@ -9,9 +9,9 @@
 // take every fourth block of 16 positions, which bulk copies bring into a ring of each warp's own, and join their results at the end of an item.  Positions are the ROWS of the products
 // (m16n8k16, halves): S^T = K Q^T, O^T = V^T P^T, so eight queries cost one tile where queries as rows would pad them to sixteen; scores,
 // exponentials and accumulators halve with them.  What is left is the expansion of codes to halves, 2.25 instructions a value pair.
-// The blocks of all items (token, kv head) are one long line cut into equal parts, one per CTA: ragged lengths and a single
-// long sequence alike keep every CTA busy to the end.  An item that lies in one part is finished there; the others leave partial
-// results, which pool_merge_kernel joins.
+// Items (token, kv head) are cut into equal pieces, one per CTA, or, where there are more of them than CTAs and they are long, their blocks are one
+// line cut into equal parts, so that ragged lengths keep every CTA busy to the end (own_pieces).  An item that lies in one part is finished
+// there; the others leave partial results, which pool_merge_kernel joins.
 #include <algorithm>
 
 #include "k2t_flash_tc.cuh"
