@@ -93,6 +93,7 @@ inline cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block
 // 48 KB of static and dynamic shared memory TOGETHER; kernels have less than 32 KB of static (the largest 18 KB), so up to 16 KB need nothing.
 inline cudaError_t allow_dynamic_smem(const void *kernel, size_t bytes) {
     if (bytes <= 16 * 1024) return cudaSuccess;
+    bytes = bytes < 48 * 1024 ? 48 * 1024 : bytes;          // no launch's limit is lowered
     constexpr int MAX_DEV = 16, SLOTS = 256;
     struct Entry { const void *fn; size_t bytes[MAX_DEV]; };
     static Entry table[SLOTS] = {};
