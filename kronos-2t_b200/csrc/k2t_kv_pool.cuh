@@ -173,6 +173,31 @@ __device__ __forceinline__ float rcp_approx(float x) { float y; asm("rcp.approx.
 __device__ __forceinline__ int query_exponent(float top) { return min(126, max(-126, 140 - (int)((__float_as_uint(top) >> 23) & 255u))); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// Eight elements of a query row as operands, the row over HD / 8 lanes: transformed, times a power of two that brings its largest to 2^13 .. 2^14 (so
+// that both terms are ordinary halves), and split.  Returns the power's inverse.  Rows that are not there are zeros.
+template <int HD> __device__ __forceinline__ float query_halves(const PoolView &pool, const RowsArg &q, bool there, size_t at, uint32_t l, uint32_t lane, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    float v[8], top = 0.0f;
+    Row8 x;
+    x.clear();
+    if (there) x.ask(q, at + l * 8);
+    x.values(q.type, v);
+    transform8(v, signs8(pool, l * 8), lane);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+#pragma unroll
+    for (uint32_t m = HD / 16; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+    const int e = query_exponent(top);
+    const float up = power_of_two(e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float y = v[2 * i] * up, z = v[2 * i + 1] * up;
+        hi[i] = half2_bits(y, z);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
+        lo[i] = half2_bits(y - f.x, z - f.y);
+    }
+    return power_of_two(-e);
+}
+
 // The scale of a value row in the exponents of its weights.  A row of zeros, which has the scale 0, takes one below all that count, so that the
 // running maximum is that of the rows an output is made of, however much of the weight the zeros have.  Exponentials reach down to 2^-126, so a
 // zero row counts beside values of scales up to 2^62; 4-bit rows with scales below 2^-64 have those as factors of it.  NaN stays NaN.

@@ -161,37 +161,18 @@ __device__ __forceinline__ bool item_row(const SplitArgs &p, const Item &it, uin
     return it.prefix ? t < p.a.n_tok : r < group;
 }
 
-// The tile's rows, HD / 8 lanes each: transformed, times a power of two that brings the row's largest to 2^13 .. 2^14 (so that both terms of a
-// row are ordinary halves), to shared memory: [row][term][element], the 16-byte chunks of a row turned by its number; and their factors.
+// The tile's rows, HD / 8 lanes each, to shared memory: [row][term][element], the 16-byte chunks of a row turned by its number; and their factors.
 template <int HD, int QT, int NR> __device__ __forceinline__ void put_queries(const SplitArgs &p, const Item &it, uint32_t tid, uint8_t *s_query, float *s_factor) {
     constexpr uint32_t LANES = HD / 8;
-    const uint32_t lane = tid & 31u, l = tid % LANES, signs = p.a.pool.signs[l / 4] >> (l % 4 * 8);
+    const uint32_t lane = tid & 31u, l = tid % LANES;
 #pragma unroll
     for (uint32_t row0 = 0; row0 < 8 * NR; row0 += SP_WARPS * 32 / LANES) {
         const uint32_t row = row0 + tid / LANES;
         if (row0 + (tid & ~31u) / LANES >= 8 * NR) break;          // whole warps
-        uint32_t t, head;
-        float v[8], top = 0.0f;
-        Row8 x;
-        x.clear();
-        if (item_row(p, it, row, t, head)) x.ask(p.a.q, t * p.a.q.token_stride + head * p.a.q.head_stride + l * 8);
-        x.values(p.a.q.type, v);
-        transform8(v, signs, lane);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
-#pragma unroll
-        for (uint32_t m = LANES / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-        const int e = query_exponent(top);
-        const float up = power_of_two(e);
-        if (l == 0) s_factor[row] = p.a.scale * LOG2E * power_of_two(-e);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float y = v[2 * i] * up, z = v[2 * i + 1] * up;
-            hi[i] = half2_bits(y, z);
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
-            lo[i] = half2_bits(y - f.x, z - f.y);
-        }
+        uint32_t t, head, hi[4], lo[4];
+        const bool there = item_row(p, it, row, t, head);
+        const float down = query_halves<HD>(p.a.pool, p.a.q, there, t * p.a.q.token_stride + head * p.a.q.head_stride, l, lane, hi, lo);
+        if (l == 0) s_factor[row] = p.a.scale * LOG2E * down;
         uint4 *to = reinterpret_cast<uint4 *>(s_query + row * QT * HD * 2) + (l ^ (row & 7u));
         to[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         if (QT == 2) to[HD / 8] = make_uint4(lo[0], lo[1], lo[2], lo[3]);

@@ -225,27 +225,9 @@ template <int HD, int QT> __global__ void __launch_bounds__(QK_THREADS) pool_que
     pdl_trigger();
     const uint32_t h = item / f.row_tiles, r = item % f.row_tiles * per + row;
     if (item >= f.items) return;
-    float v[8], top = 0.0f;
-    Row8 x;
-    x.clear();
-    if (r < all) x.ask(p.a.q, r / group * p.a.q.token_stride + (h * group + r % group) * p.a.q.head_stride + l * 8);
-    x.values(p.a.q.type, v);
-    transform8(v, p.a.pool.signs[l / 4] >> (l % 4 * 8), lane);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
-#pragma unroll
-    for (uint32_t m = LANES / 2; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-    const int e = query_exponent(top);
-    const float up = power_of_two(e);
-    if (l == 0) f.factors[item * per + row] = p.a.scale * LOG2E * power_of_two(-e);
     uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float y = v[2 * k] * up, z = v[2 * k + 1] * up;
-        hi[k] = half2_bits(y, z);
-        const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&hi[k]));
-        lo[k] = half2_bits(y - g.x, z - g.y);
-    }
+    const float down = query_halves<HD>(p.a.pool, p.a.q, r < all, r / group * p.a.q.token_stride + (h * group + r % group) * p.a.q.head_stride, l, lane, hi, lo);
+    if (l == 0) f.factors[item * per + row] = p.a.scale * LOG2E * down;
     uint8_t *to = f.queries + ((size_t)item * (per / FLASH_ROWS) + row / FLASH_ROWS) * QT * TILE + (l / 8) * (FLASH_ROWS * 128) + row % FLASH_ROWS * 128 + (((l % 8) ^ (row & 7u)) << 4);
     *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     if (QT == 2) *reinterpret_cast<uint4 *>(to + TILE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
