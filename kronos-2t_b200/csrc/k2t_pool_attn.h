@@ -7,6 +7,8 @@ namespace k2t {
 // The prefix over many rows (k2t_pool_flash.cu): items are (kv head, 2 FLASH_ROWS rows), tiles of 64 positions; a line of items * tiles, `part` of it
 // a CTA.  halved: an item has FLASH_ROWS rows, and its tiles are dealt out to two streams over the same rows.
 constexpr uint32_t FLASH_ROWS = 128, FLASH_MIN_PART = 2;          // tiles of a CTA at least (2 against 4: 24 against 25 us behind 2000 positions)
+// Tiles of a call's line, and a part behind it, are counted in 32 bits; a part is at most a 64th of the line (SMs).
+constexpr uint64_t MOST_TILES = (1ull << 32) - (1ull << 26);
 struct FlashArgs {
     bool on, halved;
     uint32_t items, row_tiles, tiles, part;

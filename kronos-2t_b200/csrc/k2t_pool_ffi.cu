@@ -3,6 +3,7 @@
 
 #include "k2t_context.h"
 #include "k2t_kv_pool.h"
+#include "k2t_pool_attn.h"
 
 namespace k2t {
 
@@ -57,7 +58,7 @@ static const char *size_refusal(const PoolShape &d, uint32_t heads, uint32_t n_t
     if (heads < d.kv_heads || heads % d.kv_heads != 0 || heads / d.kv_heads > 256) return "heads must be 1..256 times the kv heads";
     if (n_tok > (1u << 20) || (uint64_t)n_tok * heads > 0x7fffffffu) return "too many tokens";
     if (prefix_len > 0x7fffffffu) return "prefix too long";
-    if (((uint64_t)n_tok * heads / 64 + d.kv_heads) * (prefix_len / 64 + 1) >= 1ull << 32) return "prefix too long for so many tokens";
+    if (((uint64_t)n_tok * heads / 64 + d.kv_heads) * (prefix_len / 64 + 1) >= MOST_TILES) return "prefix too long for so many tokens";
     return nullptr;
 }
 size_t pool_workspace(const PoolShape &d, uint32_t heads, uint32_t n_tok, uint32_t prefix_len, uint32_t sm_count) {

@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t lds1(uint32_t at) { uint32_t v; asm volatile
 struct Segment { uint32_t item, first, last; };          // tiles [first, last) of an item
 // Segment s of a CTA's part of the line; false behind the last.
 __device__ __forceinline__ bool segment_of(const FlashArgs &f, uint32_t s, Segment &g) {
-    const uint32_t x0 = blockIdx.x * f.part, x1 = x0 + min(f.items * f.tiles - x0, f.part);          // a line may be nearly 2^32 tiles long
+    const uint32_t x0 = blockIdx.x * f.part, x1 = min(f.items * f.tiles, x0 + f.part);          // below 2^32: see MOST_TILES
     const uint32_t item = x0 / f.tiles + s, b = item * f.tiles;
     if (b >= x1) return false;
     g.item = item;

@@ -124,6 +124,18 @@ def test_workspaces_of_sizes_that_are_refused(heads, n_tok, prefix, refused):
     assert (call is not None) == refused
 
 
+def test_lines_of_tiles_are_counted_in_32_bits():
+    """The tiles of all items, with a CTA's part of them behind, stay below 2^32: the limit is as far below it as the largest part is long."""
+    most = dict(n_tok=1 << 20, heads=1024, prefix_pages=4096, workspace_bytes=1 << 63)
+    assert refusal(config(), arguments(**most, prefix_len=64 * 251 - 1)) is None
+    assert "so many tokens" in refusal(config(), arguments(**most, prefix_len=64 * 251))
+    few = dict(n_tok=1, heads=256, prefix_pages=4096, workspace_bytes=1 << 63)          # 256 kv heads: (4 + 256) tiles a 64 positions
+    last = 64 * ((1 << 32) - (1 << 26)) // 260 // 64 * 64
+    assert refusal(config(kv_heads=256), arguments(**few, prefix_len=last - 64)) is None
+    assert "so many tokens" in refusal(config(kv_heads=256), arguments(**few, prefix_len=last))
+    assert (1 << 32) - (1 << 26) + ((1 << 32) - (1 << 26)) // 64 < 1 << 32
+
+
 def test_null_handles_are_tolerated():
     import kronos_2t_b200 as k2
     L = k2.load_library()
